@@ -245,7 +245,7 @@ def _own_run(s):
     op = case["op"]
     x = s["x"]
     if isinstance(x, tuple):
-        x = pkg.Fp8Tensor(*x)
+        x = pkg.Fp8Tensor(*x, 1)
     if op == "quantize":
         q = pkg.fp8_quantize(x, case["block"])
         return [q.codes, q.scales]
