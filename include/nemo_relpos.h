@@ -586,6 +586,77 @@ int nrp_qlinear(nrp_context* ctx, void* stream, const void* x, int M, int K, con
                 const void* scales, const void* biases, int N, int group_size, int bits,
                 const void* bias, void* y);
 
+/* ------------------------- 8-bit floating-point linears and LayerNorm,
+ * with their gradients (fine-tuning a pre-norm linear in 8 bits; the
+ * reference only serves and has no counterpart).
+ *
+ * A matrix in 8 bits is `codes`, e4m3 bytes [rows, cols] (4 exponent and 3
+ * mantissa bits, largest value 448, 0x7F and 0xFF NaN, no infinity), and
+ * `scales`, f32 [ceil(rows / block_rows), ceil(cols / 128)], one per
+ * block_rows x 128 block; it stands for code * scale.  block_rows is 1 for
+ * activations and gradients, 128 for weights.  cols is a multiple of 16,
+ * codes 16-byte aligned.  All matrices are contiguous.  `dtype` is the type
+ * of the unquantised operands and outputs (NRP_DTYPE_F32 or _BF16); sums are
+ * f32.  A matrix without rows is allowed; its pointers are not looked at.
+ * These calls allocate nothing and use no buffers but their arguments,
+ * so calls and captured graphs on different streams do not share state. */
+
+/* codes and scales of x [rows, cols] (16-byte aligned).  A block's scale is
+ * the smallest power of two s with amax / s <= 448 (amax over its finite
+ * elements; the exponent clamped to [-117, 119]; 1 for zeros), its codes x /
+ * s rounded to nearest even and saturated; NaN and infinities give NaN.
+ * code * scale is then exact in bf16 and f32. */
+int nrp_fp8_quantize(nrp_context* ctx, void* stream, int dtype, const void* x, int64_t rows,
+                     int cols, int block_rows, uint8_t* codes, float* scales);
+/* x [rows, cols] (16-byte aligned) = codes * scales, rounded once. */
+int nrp_fp8_dequantize(nrp_context* ctx, void* stream, const uint8_t* codes, const float* scales,
+                       int64_t rows, int cols, int block_rows, int dtype, void* x);
+
+/* y[M, N] = x^[M, K] . w^[N, K]^T (+ bias[N]), x^ and w^ the values of xq, xs
+ * (block_rows 1) and wq, ws (block_rows 128).  x NULL: xq and xs are inputs.
+ * Otherwise x [M, K] (16-byte aligned) is quantised into them first, as by
+ * nrp_fp8_quantize: they are outputs, the checkpoint that
+ * nrp_fp8_linear_weight_grad takes.  K % 16 == 0; scales may be any f32. */
+int nrp_fp8_linear(nrp_context* ctx, void* stream, int dtype, const void* x, uint8_t* xq,
+                   float* xs, int M, int K, const uint8_t* wq, const float* ws, int N,
+                   const void* bias, void* y);
+/* The input's gradient dx[M, K] = g^[M, N] . w^[N, K], with the forward
+ * product's wq and ws; dy, gq and gs as x, xq and xs above.  N % 16 == 0 and
+ * K % 16 == 0. */
+int nrp_fp8_linear_input_grad(nrp_context* ctx, void* stream, int dtype, const void* dy,
+                              uint8_t* gq, float* gs, int M, int N, const uint8_t* wq,
+                              const float* ws, int K, void* dx);
+/* The weight's gradient dw[N, K] = dy[M, N]^T . x^[M, K] and, when dbias is
+ * not NULL, dbias[N] = the column sums of dy, both in `dtype`.  dy bf16
+ * (16-byte aligned, N % 8 == 0), xq and xs the input's checkpoint
+ * (block_rows 1).  x^ enters as bf16: exact with nrp_fp8_quantize's scales,
+ * rounded once with others.  M == 0 writes zeros. */
+int nrp_fp8_linear_weight_grad(nrp_context* ctx, void* stream, const void* dy, const uint8_t* xq,
+                               const float* xs, int M, int N, int K, int dtype, void* dw,
+                               void* dbias);
+
+/* LayerNorm over the rows of x [rows, cols], any cols >= 1: y = (x - mean) *
+ * rstd * gamma + beta, rstd = (variance + eps)^-1/2; gamma, beta f32 [cols];
+ * mean, rstd f32 [rows], or both NULL.  y may be x. */
+int nrp_layer_norm(nrp_context* ctx, void* stream, int dtype, const void* x, int64_t rows,
+                   int cols, const float* gamma, const float* beta, float eps, void* y,
+                   float* mean, float* rstd);
+/* Bytes of workspace nrp_layer_norm_backward needs for dgamma and dbeta. */
+int nrp_layer_norm_backward_workspace(int64_t rows, int cols, int64_t* bytes);
+/* Gradients of nrp_layer_norm: dx [rows, cols], dgamma and dbeta f32 [cols]
+ * (both NULL: not computed).  x_scales NULL: x [rows, cols] is the exact
+ * input; else x holds its e4m3 codes (block_rows 1) with scales x_scales, and
+ * their values stand in for it, with the mean and rstd given.  workspace:
+ * device memory of at least nrp_layer_norm_backward_workspace bytes, 16-byte
+ * aligned, not shared with work that may run at the same time; unused
+ * without dgamma.  dx must not overlap x or dy.  rows == 0 gives zero dgamma
+ * and dbeta. */
+int nrp_layer_norm_backward(nrp_context* ctx, void* stream, int dtype, const void* x,
+                            const float* x_scales, const void* dy, const float* mean,
+                            const float* rstd, const float* gamma, int64_t rows, int cols,
+                            void* dx, float* dgamma, float* dbeta, void* workspace,
+                            int64_t workspace_bytes);
+
 /* ------------------------------------------------------------ profiling */
 /* Per-kernel device time from CUDA events the library records on the
  * launching stream around each launch while enabled (the reference has no
@@ -604,7 +675,12 @@ typedef enum {
   NRP_KERNEL_ELEMENTWISE = 10, /* input scaling, transposes, copies */
   NRP_KERNEL_DEQUANT = 11,    /* 8-bit weights to bf16 (large-M quantised GEMM) */
   NRP_KERNEL_SUBSAMPLE = 12,  /* the subsampling's direct (non-GEMM) convolutions */
-  NRP_KERNEL_KINDS = 13
+  NRP_KERNEL_GEMM_FP8 = 13,    /* block-scaled e4m3 GEMM, both directions */
+  NRP_KERNEL_FP8_SMALL = 14,   /* the same for few rows */
+  NRP_KERNEL_FP8_QUANT = 15,   /* e4m3 quantisation and dequantisation */
+  NRP_KERNEL_FP8_WGRAD = 16,   /* weight gradient from e4m3 activations */
+  NRP_KERNEL_LAYERNORM_BWD = 17, /* LayerNorm gradients (both kernels) */
+  NRP_KERNEL_KINDS = 18
 } nrp_kernel_kind;
 int nrp_profile_enable(nrp_context* ctx, int enable);
 int nrp_profile_reset(nrp_context* ctx);

@@ -114,6 +114,15 @@ def lib():
             "nrp_attn_forward_with_cache": ([vp, vp, vp, i, i, vp, vp, i, i, vp, vp], i),
             "nrp_linear": ([vp, vp, i, vp, i, i, vp, i, vp, vp], i),
             "nrp_qlinear": ([vp, vp, vp, i, i, vp, vp, vp, i, i, i, vp, vp], i),
+            "nrp_fp8_quantize": ([vp, vp, i, vp, C.c_int64, i, i, vp, vp], i),
+            "nrp_fp8_dequantize": ([vp, vp, vp, vp, C.c_int64, i, i, i, vp], i),
+            "nrp_fp8_linear": ([vp, vp, i, vp, vp, vp, i, i, vp, vp, i, vp, vp], i),
+            "nrp_fp8_linear_input_grad": ([vp, vp, i, vp, vp, vp, i, i, vp, vp, i, vp], i),
+            "nrp_fp8_linear_weight_grad": ([vp, vp, vp, vp, vp, i, i, i, i, vp, vp], i),
+            "nrp_layer_norm": ([vp, vp, i, vp, C.c_int64, i, vp, vp, f, vp, vp, vp], i),
+            "nrp_layer_norm_backward_workspace": ([C.c_int64, i, vp], i),
+            "nrp_layer_norm_backward": ([vp, vp, i] + [vp] * 6 + [C.c_int64, i] + [vp] * 4
+                                        + [C.c_int64], i),
             "nrp_seq_shard": ([i, i, i, vp, vp], i),
             "nrp_partition_utterances": ([vp, i, i, i, vp, vp], i),
             "nrp_copy_frames": ([vp, vp, vp, i, i, C.c_int64, vp, vp], i),
@@ -238,7 +247,7 @@ class Context:
 
     KERNELS = ("gemm_bf16", "gemm_q8", "qgemv", "gemm_f32", "attn_sm100", "attn_simt",
                "attn_stream", "ring_append", "layernorm", "dwconv", "elementwise", "dequant",
-               "subsample")
+               "subsample", "gemm_fp8", "fp8_small", "fp8_quant", "fp8_wgrad", "layernorm_bwd")
 
     def profile(self, enable: bool = True):
         _check(lib().nrp_profile_enable(self.handle, int(enable)))
@@ -1516,3 +1525,6 @@ def qlinear(x, wq, scales, biases, bias=None, group_size=64, bits=8,
 from .checkpoint import (CheckpointError, NemoCheckpoint, SafetensorsLoader,  # noqa: E402
                          WeightFormat, load_safetensors_weights, read_safetensors,
                          read_safetensors_metadata, transform_weights_to_mlx, write_safetensors)
+# 8-bit floating-point linears and the LayerNorm with their gradients
+from .fp8 import (Fp8Tensor, fp8_dequantize, fp8_linear, fp8_linear_input_grad,  # noqa: E402
+                  fp8_linear_weight_grad, fp8_quantize, layer_norm, layer_norm_backward)

@@ -1,0 +1,194 @@
+// fp8_api.cpp -- C ABI of the 8-bit floating-point linears, their gradients
+// and the LayerNorm's forward and backward pass (include/nemo_relpos.h).
+#include <cuda_runtime.h>
+
+#include "../../include/nemo_relpos.h"
+#include "fp8.h"
+#include "handles.h"
+#include "internal.h"
+
+using nrp::failf;
+using nrp::ProfScope;
+
+namespace {
+
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// cudaSuccess -> NRP_OK; else the error, also taken out of the runtime's
+// last-error slot.
+int status(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return NRP_OK;
+  cudaGetLastError();
+  return failf(e == cudaErrorMemoryAllocation ? NRP_ERR_NOMEM : NRP_ERR_CUDA, "%s: %s", what,
+               cudaGetErrorString(e));
+}
+
+int check_dtype(int dtype) {
+  if (dtype == NRP_DTYPE_F32 || dtype == NRP_DTYPE_BF16) return NRP_OK;
+  return failf(NRP_ERR_UNSUPPORTED, "dtype %d", dtype);
+}
+
+// A matrix of codes: 16-byte rows (TMA and 16-byte loads), 16-byte aligned.
+// One without rows may have null pointers (an empty tensor's).
+int check_codes(const char* name, const void* codes, const void* scales, int64_t cols,
+                bool empty = false) {
+  if (!empty && (!codes || !scales)) return failf(NRP_ERR_INVALID, "%s: null codes or scales", name);
+  if (cols % 16)
+    return failf(NRP_ERR_UNSUPPORTED, "%s: %lld columns (codes need a multiple of 16)", name,
+                 static_cast<long long>(cols));
+  if (!aligned(codes, 16) || !aligned(scales, 4))
+    return failf(NRP_ERR_INVALID, "%s: codes must be 16-byte and scales 4-byte aligned", name);
+  return NRP_OK;
+}
+
+// Quantises x (when given) into xq, xs and multiplies by the weight.
+int product(nrp_context* ctx, cudaStream_t st, bool trans, int dtype, const void* x, uint8_t* xq,
+            float* xs, int M, int R, const uint8_t* wq, const float* ws, int NO, const void* bias,
+            void* y) {
+  const bool bf16 = dtype == NRP_DTYPE_BF16;
+  if (x) {
+    ProfScope ps(ctx, NRP_KERNEL_FP8_QUANT, st);
+    if (int rc = status(nrp::launch_fp8_quantize(bf16, x, M, R, 1, xq, xs, ctx->num_sms, st),
+                        "fp8 quantize"))
+      return rc;
+  }
+  ProfScope ps(ctx, NRP_KERNEL_GEMM_FP8, st);
+  return status(nrp::launch_gemm_fp8(bf16, trans, xq, xs, M, R, wq, ws, NO, bias, y, ctx->num_sms,
+                                     ctx->d_err, st),
+                "fp8 linear");
+}
+
+}  // namespace
+
+extern "C" {
+
+int nrp_fp8_quantize(nrp_context* ctx, void* stream, int dtype, const void* x, int64_t rows,
+                     int cols, int block_rows, uint8_t* codes, float* scales) {
+  if (!ctx || (rows && !x) || rows < 0 || cols <= 0)
+    return failf(NRP_ERR_INVALID, "invalid quantize arguments");
+  if (int rc = check_dtype(dtype)) return rc;
+  if (block_rows != 1 && block_rows != 128)
+    return failf(NRP_ERR_UNSUPPORTED, "block_rows %d (supported: 1, 128)", block_rows);
+  if (int rc = check_codes("quantize", codes, scales, cols, rows == 0)) return rc;
+  if (!aligned(x, 16)) return failf(NRP_ERR_INVALID, "the input must be 16-byte aligned");
+  if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ProfScope ps(ctx, NRP_KERNEL_FP8_QUANT, st);
+  return status(nrp::launch_fp8_quantize(dtype == NRP_DTYPE_BF16, x, rows, cols, block_rows, codes,
+                                         scales, ctx->num_sms, st),
+                "fp8 quantize");
+}
+
+int nrp_fp8_dequantize(nrp_context* ctx, void* stream, const uint8_t* codes, const float* scales,
+                       int64_t rows, int cols, int block_rows, int dtype, void* x) {
+  if (!ctx || (rows && !x) || rows < 0 || cols <= 0)
+    return failf(NRP_ERR_INVALID, "invalid dequantize arguments");
+  if (int rc = check_dtype(dtype)) return rc;
+  if (block_rows != 1 && block_rows != 128)
+    return failf(NRP_ERR_UNSUPPORTED, "block_rows %d (supported: 1, 128)", block_rows);
+  if (int rc = check_codes("dequantize", codes, scales, cols, rows == 0)) return rc;
+  if (!aligned(x, 16)) return failf(NRP_ERR_INVALID, "the output must be 16-byte aligned");
+  if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ProfScope ps(ctx, NRP_KERNEL_FP8_QUANT, st);
+  return status(nrp::launch_fp8_dequantize(dtype == NRP_DTYPE_BF16, codes, scales, rows, cols,
+                                           block_rows, x, ctx->num_sms, st),
+                "fp8 dequantize");
+}
+
+int nrp_fp8_linear(nrp_context* ctx, void* stream, int dtype, const void* x, uint8_t* xq,
+                   float* xs, int M, int K, const uint8_t* wq, const float* ws, int N,
+                   const void* bias, void* y) {
+  if (!ctx || (M && !y) || M < 0 || K <= 0 || N <= 0)
+    return failf(NRP_ERR_INVALID, "invalid fp8 linear arguments");
+  if (int rc = check_dtype(dtype)) return rc;
+  if (int rc = check_codes("fp8 linear: input", xq, xs, K, M == 0)) return rc;
+  if (int rc = check_codes("fp8 linear: weight", wq, ws, K)) return rc;
+  if (!aligned(x, 16)) return failf(NRP_ERR_INVALID, "the input must be 16-byte aligned");
+  if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
+  return product(ctx, static_cast<cudaStream_t>(stream), false, dtype, x, xq, xs, M, K, wq, ws, N,
+                 bias, y);
+}
+
+int nrp_fp8_linear_input_grad(nrp_context* ctx, void* stream, int dtype, const void* dy,
+                              uint8_t* gq, float* gs, int M, int N, const uint8_t* wq,
+                              const float* ws, int K, void* dx) {
+  if (!ctx || (M && !dx) || M < 0 || K <= 0 || N <= 0)
+    return failf(NRP_ERR_INVALID, "invalid fp8 input gradient arguments");
+  if (int rc = check_dtype(dtype)) return rc;
+  if (int rc = check_codes("fp8 input gradient: output gradient", gq, gs, N, M == 0)) return rc;
+  if (int rc = check_codes("fp8 input gradient: weight", wq, ws, K)) return rc;
+  if (!aligned(dy, 16)) return failf(NRP_ERR_INVALID, "the output gradient must be 16-byte aligned");
+  if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
+  return product(ctx, static_cast<cudaStream_t>(stream), true, dtype, dy, gq, gs, M, N, wq, ws, K,
+                 nullptr, dx);
+}
+
+int nrp_fp8_linear_weight_grad(nrp_context* ctx, void* stream, const void* dy, const uint8_t* xq,
+                               const float* xs, int M, int N, int K, int dtype, void* dw,
+                               void* dbias) {
+  if (!ctx || (M && !dy) || !dw || M < 0 || K <= 0 || N <= 0)
+    return failf(NRP_ERR_INVALID, "invalid fp8 weight gradient arguments");
+  if (int rc = check_dtype(dtype)) return rc;
+  if (int rc = check_codes("fp8 weight gradient: input", xq, xs, K, M == 0)) return rc;
+  if (N % 8)
+    return failf(NRP_ERR_UNSUPPORTED, "fp8 weight gradient: N = %d (needs a multiple of 8)", N);
+  if (!aligned(dy, 16)) return failf(NRP_ERR_INVALID, "the output gradient must be 16-byte aligned");
+  if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ProfScope ps(ctx, NRP_KERNEL_FP8_WGRAD, st);
+  return status(nrp::launch_fp8_weight_grad(dtype == NRP_DTYPE_BF16, dy, xq, xs, M, N, K, dw,
+                                            dbias, ctx->num_sms, ctx->d_err, st),
+                "fp8 weight gradient");
+}
+
+int nrp_layer_norm(nrp_context* ctx, void* stream, int dtype, const void* x, int64_t rows,
+                   int cols, const float* gamma, const float* beta, float eps, void* y,
+                   float* mean, float* rstd) {
+  if (!ctx || !gamma || !beta || (rows && (!x || !y)) || rows < 0 || cols <= 0)
+    return failf(NRP_ERR_INVALID, "invalid layer norm arguments");
+  if (rows && !mean != !rstd) return failf(NRP_ERR_INVALID, "layer norm: mean and rstd go together");
+  if (!(eps >= 0.f)) return failf(NRP_ERR_INVALID, "layer norm: eps must not be negative");
+  if (int rc = check_dtype(dtype)) return rc;
+  if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ProfScope ps(ctx, NRP_KERNEL_LAYERNORM, st);
+  return status(nrp::launch_norm_fwd(dtype == NRP_DTYPE_BF16, x, rows, cols, gamma, beta, eps, y,
+                                     mean, rstd, ctx->num_sms, st),
+                "layer norm");
+}
+
+int nrp_layer_norm_backward_workspace(int64_t rows, int cols, int64_t* bytes) {
+  if (!bytes || rows < 0 || cols <= 0) return failf(NRP_ERR_INVALID, "invalid layer norm size");
+  *bytes = 4 * nrp::norm_bwd_partials(rows, cols);
+  return NRP_OK;
+}
+
+int nrp_layer_norm_backward(nrp_context* ctx, void* stream, int dtype, const void* x,
+                            const float* x_scales, const void* dy, const float* mean,
+                            const float* rstd, const float* gamma, int64_t rows, int cols,
+                            void* dx, float* dgamma, float* dbeta, void* workspace,
+                            int64_t workspace_bytes) {
+  if (!ctx || !gamma || (rows && (!x || !dy || !mean || !rstd || !dx)) || rows < 0 || cols <= 0)
+    return failf(NRP_ERR_INVALID, "invalid layer norm backward arguments");
+  if (!dgamma != !dbeta) return failf(NRP_ERR_INVALID, "layer norm: dgamma and dbeta go together");
+  if (int rc = check_dtype(dtype)) return rc;
+  if (x_scales)
+    if (int rc = check_codes("layer norm backward: input", x, x_scales, cols)) return rc;
+  if (dgamma) {
+    const int64_t need = 4 * nrp::norm_bwd_partials(rows, cols);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+      return failf(NRP_ERR_INVALID,
+                   "layer norm backward: workspace of %lld bytes (16-byte aligned) needed, got %lld",
+                   static_cast<long long>(need), static_cast<long long>(workspace_bytes));
+  }
+  if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ProfScope ps(ctx, NRP_KERNEL_LAYERNORM_BWD, st);
+  return status(nrp::launch_norm_bwd(dtype == NRP_DTYPE_BF16, x, x_scales, dy, mean, rstd, gamma,
+                                     rows, cols, dx, dgamma, dbeta,
+                                     static_cast<float*>(workspace), st),
+                "layer norm backward");
+}
+
+}  // extern "C"

@@ -1,0 +1,358 @@
+// gemm_fp8.cu -- products of block-scaled e4m3 matrices on tcgen05
+// (kind::f8f6f4, f32 accumulation), the forward product and the input's
+// gradient of an 8-bit linear:
+//
+//   y[m, n] = sum_b xs[m, b] * ws[b, n / 128] * sum_{r in block b} xq[m, r] * w(r, n)
+//
+// with r over the reduction in blocks of 128.  A block's scales are constant
+// over its 128 products, so the tensor cores sum one block (four K = 32 steps)
+// into a TMEM accumulator, and the epilogue warps read it, multiply by the two
+// scales' product (one number per row and 128 columns) and add to f32
+// registers; the accumulator is double buffered, so block b + 1 runs meanwhile.
+// The scales may be any f32 values.
+//
+// The weight is stored once, [out, in].  The forward product reads it with
+// the reduction contiguous (K-major B operand); the input's gradient reduces
+// over the output features, so its B tile comes from the same bytes with the
+// reduction along rows (MN-major descriptor), with no transposed copy.
+//
+// Warp roles (10 warps): 0 TMA producer, 1 TMEM allocator and MMA issuer,
+// 2..9 epilogue (two groups of four, each half of the tile's columns).  The
+// grid is persistent, one CTA per SM.
+#include <algorithm>
+
+#include "fp8.h"
+#include "sm100.cuh"
+
+namespace nrp {
+namespace {
+
+constexpr int kBM = 128;
+constexpr int kBR = 128;  // reduction per stage: one scale block, one swizzle row
+constexpr uint32_t kABytes = kBM * kBR;
+constexpr int kThreads = 320;
+constexpr int kMaxStages = 6;
+constexpr uint32_t kSlabBytes = 32 * 128;  // per epilogue warp: 32 rows x 128 B
+
+template <int kBN>
+struct Cfg {
+  static constexpr int kStages = kBN == 256 ? 4 : 6;
+  static constexpr uint32_t kBBytes = kBN * kBR;
+  static constexpr size_t kSmem = 1024 + kStages * (kABytes + kBBytes) + 8 * kSlabBytes + 256;
+};
+static_assert(Cfg<256>::kSmem <= 232448 && Cfg<128>::kSmem <= 232448 && Cfg<64>::kSmem <= 232448,
+              "shared memory budget");
+
+struct Bars {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t tfull[2];
+  uint64_t tempty[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+};
+
+__device__ __forceinline__ void umma_f8_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
+                                           uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// kind::f8f6f4 instruction descriptor: f32 accumulator (bit 4), A and B e4m3
+// (format 0), A K-major, B major at bit 16, N >> 3 at 17, M >> 4 at 24.
+__host__ __device__ constexpr uint32_t idesc_e4m3_f32(int M, int N, int b_mn_major) {
+  return (1u << 4) | (static_cast<uint32_t>(b_mn_major) << 16) |
+         (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+struct Args {
+  const float* xs;   // [M, rb]
+  const float* ws;   // forward [ceil(NO/128), rb], trans [rb, ceil(NO/128)]
+  const void* bias;  // [NO] in the output's type, or null
+  void* y;           // [M, NO]
+  int M, NO, rb;     // rb: reduction blocks
+  int tma_out;       // y's rows are 16-byte multiples: stored through map_y
+  int* err;
+};
+
+template <typename TO>
+__device__ __forceinline__ float to_f32(TO v) {
+  if constexpr (sizeof(TO) == 4) return v;
+  else return __bfloat162float(v);
+}
+
+template <int kBN, bool kTrans, typename TO>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_x,
+                    const __grid_constant__ CUtensorMap map_w,
+                    const __grid_constant__ CUtensorMap map_y, const Args a) {
+  constexpr int kStages = Cfg<kBN>::kStages;
+  constexpr uint32_t kBBytes = Cfg<kBN>::kBBytes;
+  constexpr int kHalfN = kBN / 2;  // columns of one epilogue group
+  constexpr int kSlabCols = 128 / static_cast<int>(sizeof(TO));
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* base = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  uint8_t* sA = base;
+  uint8_t* sB = sA + kStages * kABytes;
+  uint8_t* sE = sB + kStages * kBBytes;
+  Bars* ss = reinterpret_cast<Bars*>(sE + 8 * kSlabBytes);
+  const int warp = warp_id(), lane = lane_id();
+  const int tiles_m = (a.M + kBM - 1) / kBM;
+  const int tiles_n = (a.NO + kBN - 1) / kBN;
+  const int num_tiles = tiles_m * tiles_n;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&ss->full[s], 1);
+      mbar_init(&ss->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&ss->tfull[b], 1);
+      mbar_init(&ss->tempty[b], 8);
+    }
+    mbar_init(&ss->drain, 1);
+    ss->abort = 0;
+    fence_mbar_init();
+    prefetch_tensormap(&map_x);
+    prefetch_tensormap(&map_w);
+  }
+  if (warp == 1) {
+    tmem_alloc(&ss->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ss->tmem_base;
+  volatile int* abort_flag = &ss->abort;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  if (warp == 0) {
+    // ---------------------------------------------------------- producer
+    if (lane == 0) {
+      uint32_t it = 0;
+      for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
+        const int m0 = t / tiles_n * kBM, n0 = t % tiles_n * kBN;
+        for (int b = 0; b < a.rb; ++b, ++it) {
+          const int s = it % kStages;
+          if (!mbar_wait(&ss->empty[s], ((it / kStages) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
+            *abort_flag = 1;
+            break;
+          }
+          mbar_arrive_expect_tx(&ss->full[s], kABytes + kBBytes);
+          tma_load_2d(sA + s * kABytes, &map_x, &ss->full[s], b * kBR, m0);
+          uint8_t* B = sB + s * kBBytes;
+          if constexpr (!kTrans) {
+            tma_load_2d(B, &map_w, &ss->full[s], b * kBR, n0);  // [n][128 r]
+          } else {
+            // [r][min(128, kBN) n]: one box per 128 columns
+#pragma unroll
+            for (int j = 0; j < kBN; j += 128)
+              tma_load_2d(B + j * kBR, &map_w, &ss->full[s], n0 + j, b * kBR);
+          }
+        }
+      }
+      // after an abort: the copies in flight land before the CTA goes
+      if (*abort_flag)
+        for (uint32_t j = it > static_cast<uint32_t>(kStages) ? it - kStages : 0; j < it; ++j)
+          mbar_wait(&ss->full[j % kStages], (j / kStages) & 1, nullptr, 0);
+    }
+  } else if (warp == 1) {
+    // -------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_e4m3_f32(kBM, kBN, kTrans ? 1 : 0);
+      uint32_t it = 0;
+      for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
+        for (int b = 0; b < a.rb; ++b, ++it) {
+          const int s = it % kStages, buf = it & 1;
+          if (!mbar_wait(&ss->tempty[buf], ((it >> 1) & 1) ^ 1, a.err, kDevTimeoutEpi) ||
+              !mbar_wait(&ss->full[s], (it / kStages) & 1, a.err, kDevTimeoutLoad)) {
+            *abort_flag = 1;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(sA + s * kABytes), b0 = smem_u32(sB + s * kBBytes);
+#pragma unroll
+          for (int k = 0; k < kBR / 32; ++k) {
+            const uint64_t ad = sdesc_sw128(a0 + k * 32, 16, 1024);
+            // MN-major: 32 reduction rows of 128 bytes per step, 128-column
+            // blocks kBR * 128 bytes apart
+            const uint64_t bd = kTrans ? sdesc_sw128(b0 + k * 32 * 128, kBR * 128, 1024)
+                                       : sdesc_sw128(b0 + k * 32, 16, 1024);
+            umma_f8_ss(tmem + buf * kBN, ad, bd, idesc, k != 0);
+          }
+          umma_commit(&ss->empty[s]);
+          umma_commit(&ss->tfull[buf]);
+        }
+      }
+      if (*abort_flag) {
+        umma_commit(&ss->drain);
+        mbar_wait(&ss->drain, 0, nullptr, 0);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------- epilogue
+    const int quad = warp & 3, group = (warp - 2) >> 2;
+    uint8_t* slab = sE + (warp - 2) * kSlabBytes;
+    const int ncb = (a.NO + 127) / 128;
+    uint32_t it = 0;
+    for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
+      const int m0 = t / tiles_n * kBM, n0 = t % tiles_n * kBN + group * kHalfN;
+      const int row = m0 + quad * 32 + lane;
+      const int nb = min(n0 / 128, ncb - 1);  // (a group past NO stores nothing)
+      const float* xsr = a.xs + static_cast<int64_t>(min(row, a.M - 1)) * a.rb;
+      const float* wsr = kTrans ? a.ws + nb : a.ws + static_cast<int64_t>(nb) * a.rb;
+      const int wstep = kTrans ? ncb : 1;
+      float acc[kHalfN];
+#pragma unroll
+      for (int e = 0; e < kHalfN; ++e) acc[e] = 0.f;
+      float sc = xsr[0] * wsr[0];
+      bool ok = true;
+      for (int b = 0; b < a.rb; ++b, ++it) {
+        const int buf = it & 1;
+        const float s = sc;
+        if (b + 1 < a.rb) sc = xsr[b + 1] * wsr[static_cast<int64_t>(b + 1) * wstep];
+        if (!mbar_wait(&ss->tfull[buf], (it >> 1) & 1, a.err, kDevTimeoutMma)) {
+          *abort_flag = 1;
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t taddr =
+            tmem + (static_cast<uint32_t>(quad * 32) << 16) + buf * kBN + group * kHalfN;
+#pragma unroll
+        for (int c = 0; c < kHalfN; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(taddr + c, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            fma_f32x2v(acc[c + e], acc[c + e + 1], __uint_as_float(r[e]),
+                       __uint_as_float(r[e + 1]), s, acc[c + e], acc[c + e + 1]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ss->tempty[buf]);
+      }
+      if (!ok) break;
+      const TO* bias = static_cast<const TO*>(a.bias);
+      TO* y = static_cast<TO*>(a.y);
+#pragma unroll
+      for (int c = 0; c < kHalfN; c += kSlabCols) {
+        if (n0 + c >= a.NO) break;  // warp-uniform
+        if (bias) {
+#pragma unroll
+          for (int e = 0; e < kSlabCols; ++e)
+            if (n0 + c + e < a.NO) acc[c + e] += to_f32(bias[n0 + c + e]);
+        }
+        if (a.tma_out) {
+          if (lane == 0) bulk_wait_read<0>();  // the store before has read the slab
+          __syncwarp();
+#pragma unroll
+          for (int ch = 0; ch < 8; ++ch) {
+            uint4 q;
+            if constexpr (sizeof(TO) == 4)
+              q = make_uint4(__float_as_uint(acc[c + 4 * ch]), __float_as_uint(acc[c + 4 * ch + 1]),
+                             __float_as_uint(acc[c + 4 * ch + 2]),
+                             __float_as_uint(acc[c + 4 * ch + 3]));
+            else
+              q = make_uint4(pack_bf16x2(acc[c + 8 * ch], acc[c + 8 * ch + 1]),
+                             pack_bf16x2(acc[c + 8 * ch + 2], acc[c + 8 * ch + 3]),
+                             pack_bf16x2(acc[c + 8 * ch + 4], acc[c + 8 * ch + 5]),
+                             pack_bf16x2(acc[c + 8 * ch + 6], acc[c + 8 * ch + 7]));
+            *reinterpret_cast<uint4*>(slab + sw128_offset(lane, ch)) = q;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&map_y, slab, n0 + c, m0 + quad * 32);
+            bulk_commit();
+          }
+        } else if (row < a.M) {
+#pragma unroll
+          for (int e = 0; e < kSlabCols; ++e)
+            if (n0 + c + e < a.NO) {
+              TO* o = y + static_cast<int64_t>(row) * a.NO + n0 + c + e;
+              if constexpr (sizeof(TO) == 4) *o = acc[c + e];
+              else *o = __float2bfloat16_rn(acc[c + e]);
+            }
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int kBN, bool kTrans, typename TO>
+cudaError_t launch(const uint8_t* xq, int R, const uint8_t* wq, Args a, int num_sms,
+                   cudaStream_t stream) {
+  static std::atomic<uint64_t> attr{0};
+  constexpr int kSmem = static_cast<int>(Cfg<kBN>::kSmem);
+  auto* kernel = gemm_fp8_kernel<kBN, kTrans, TO>;
+  if (cudaError_t e = smem_attr_once(kernel, kSmem, attr)) return e;
+  constexpr int es = sizeof(TO);
+  CUtensorMap mx, mw, my;
+  bool ok = make_tmap_2d(&mx, xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, R, a.M, R, kBR, kBM, true);
+  ok = ok && (kTrans ? make_tmap_2d(&mw, wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.NO, R, a.NO, 128,
+                                    kBR, true)
+                     : make_tmap_2d(&mw, wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, R, a.NO, R, kBR,
+                                    kBN, true));
+  a.tma_out = (static_cast<int64_t>(a.NO) * es) % 16 == 0 &&
+              reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
+  my = mx;
+  if (ok && a.tma_out)
+    ok = make_tmap_2d(&my, a.y,
+                      es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                      es, a.NO, a.M, static_cast<uint64_t>(a.NO) * es, 128 / es, 32, true);
+  if (!ok) return cudaErrorInvalidValue;
+  const int64_t tiles =
+      ((a.M + kBM - 1) / kBM) * static_cast<int64_t>((a.NO + kBN - 1) / kBN);
+  if (tiles > 0x7fffffff) return cudaErrorInvalidValue;
+  const int grid = static_cast<int>(std::min<int64_t>(tiles, num_sms));
+  return launch_pdl(kernel, dim3(grid), dim3(kThreads), static_cast<size_t>(kSmem), stream, mx, mw,
+                    my, a);
+}
+
+template <bool kTrans, typename TO>
+cudaError_t pick(const uint8_t* xq, int R, const uint8_t* wq, const Args& a, int num_sms,
+                 cudaStream_t stream) {
+  const int64_t tm = (a.M + kBM - 1) / kBM;
+  if (tm * ((a.NO + 255) / 256) >= num_sms) return launch<256, kTrans, TO>(xq, R, wq, a, num_sms, stream);
+  return launch<128, kTrans, TO>(xq, R, wq, a, num_sms, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_gemm_fp8(bool bf16_out, bool trans, const uint8_t* xq, const float* xs, int M,
+                            int R, const uint8_t* wq, const float* ws, int NO, const void* bias,
+                            void* y, int num_sms, int* err, cudaStream_t stream) {
+  if (M <= 0) return cudaSuccess;
+  Args a{};
+  a.xs = xs;
+  a.ws = ws;
+  a.bias = bias;
+  a.y = y;
+  a.M = M;
+  a.NO = NO;
+  a.rb = static_cast<int>(qblocks(R));
+  a.err = err;
+  if (trans)
+    return bf16_out ? pick<true, __nv_bfloat16>(xq, R, wq, a, num_sms, stream)
+                    : pick<true, float>(xq, R, wq, a, num_sms, stream);
+  return bf16_out ? pick<false, __nv_bfloat16>(xq, R, wq, a, num_sms, stream)
+                  : pick<false, float>(xq, R, wq, a, num_sms, stream);
+}
+
+}  // namespace nrp

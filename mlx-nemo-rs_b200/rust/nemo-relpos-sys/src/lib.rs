@@ -52,7 +52,12 @@ pub const NRP_KERNEL_DWCONV: c_int = 9;
 pub const NRP_KERNEL_ELEMENTWISE: c_int = 10;
 pub const NRP_KERNEL_DEQUANT: c_int = 11;
 pub const NRP_KERNEL_SUBSAMPLE: c_int = 12;
-pub const NRP_KERNEL_KINDS: c_int = 13;
+pub const NRP_KERNEL_GEMM_FP8: c_int = 13;
+pub const NRP_KERNEL_FP8_SMALL: c_int = 14;
+pub const NRP_KERNEL_FP8_QUANT: c_int = 15;
+pub const NRP_KERNEL_FP8_WGRAD: c_int = 16;
+pub const NRP_KERNEL_LAYERNORM_BWD: c_int = 17;
+pub const NRP_KERNEL_KINDS: c_int = 18;
 
 #[repr(C)] pub struct nrp_context { _p: [u8; 0] }
 #[repr(C)] pub struct nrp_attn { _p: [u8; 0] }
@@ -250,6 +255,27 @@ extern "C" {
                                    features: *const c_float, layout: c_int, batch: c_int,
                                    frames: c_int, lengths: *const i32, out: *mut c_void) -> c_int;
     pub fn nrp_subsampling_set_chunk_frames(s: *mut nrp_subsampling, frames: c_int) -> c_int;
+    pub fn nrp_fp8_quantize(ctx: *mut nrp_context, stream: *mut c_void, dtype: c_int, x: *const c_void,
+        rows: i64, cols: c_int, block_rows: c_int, codes: *mut u8, scales: *mut f32) -> c_int;
+    pub fn nrp_fp8_dequantize(ctx: *mut nrp_context, stream: *mut c_void, codes: *const u8,
+        scales: *const f32, rows: i64, cols: c_int, block_rows: c_int, dtype: c_int, x: *mut c_void) -> c_int;
+    pub fn nrp_fp8_linear(ctx: *mut nrp_context, stream: *mut c_void, dtype: c_int, x: *const c_void,
+        xq: *mut u8, xs: *mut f32, m: c_int, k: c_int, wq: *const u8, ws: *const f32, n: c_int,
+        bias: *const c_void, y: *mut c_void) -> c_int;
+    pub fn nrp_fp8_linear_input_grad(ctx: *mut nrp_context, stream: *mut c_void, dtype: c_int,
+        dy: *const c_void, gq: *mut u8, gs: *mut f32, m: c_int, n: c_int, wq: *const u8,
+        ws: *const f32, k: c_int, dx: *mut c_void) -> c_int;
+    pub fn nrp_fp8_linear_weight_grad(ctx: *mut nrp_context, stream: *mut c_void, dy: *const c_void,
+        xq: *const u8, xs: *const f32, m: c_int, n: c_int, k: c_int, dtype: c_int, dw: *mut c_void,
+        dbias: *mut c_void) -> c_int;
+    pub fn nrp_layer_norm(ctx: *mut nrp_context, stream: *mut c_void, dtype: c_int, x: *const c_void,
+        rows: i64, cols: c_int, gamma: *const f32, beta: *const f32, eps: f32, y: *mut c_void,
+        mean: *mut f32, rstd: *mut f32) -> c_int;
+    pub fn nrp_layer_norm_backward_workspace(rows: i64, cols: c_int, bytes: *mut i64) -> c_int;
+    pub fn nrp_layer_norm_backward(ctx: *mut nrp_context, stream: *mut c_void, dtype: c_int,
+        x: *const c_void, x_scales: *const f32, dy: *const c_void, mean: *const f32, rstd: *const f32,
+        gamma: *const f32, rows: i64, cols: c_int, dx: *mut c_void, dgamma: *mut f32, dbeta: *mut f32,
+        workspace: *mut c_void, workspace_bytes: i64) -> c_int;
     pub fn nrp_qlinear(ctx: *mut nrp_context, stream: *mut c_void, x: *const c_void, m: c_int, k: c_int,
                        wq: *const u32, scales: *const c_void, biases: *const c_void, n: c_int,
                        group: c_int, bits: c_int, bias: *const c_void, y: *mut c_void) -> c_int;
