@@ -1525,6 +1525,15 @@ def qlinear(x, wq, scales, biases, bias=None, group_size=64, bits=8,
 from .checkpoint import (CheckpointError, NemoCheckpoint, SafetensorsLoader,  # noqa: E402
                          WeightFormat, load_safetensors_weights, read_safetensors,
                          read_safetensors_metadata, transform_weights_to_mlx, write_safetensors)
-# 8-bit floating-point linears and the LayerNorm with their gradients
-from .fp8 import (Fp8Tensor, fp8_dequantize, fp8_linear, fp8_linear_input_grad,  # noqa: E402
-                  fp8_linear_weight_grad, fp8_quantize, layer_norm, layer_norm_backward)
+# 8-bit floating-point linears and the LayerNorm with their gradients: the
+# module needs torch, which the host-side logic above does without
+_FP8_NAMES = ("Fp8Tensor", "fp8_dequantize", "fp8_linear", "fp8_linear_input_grad",
+              "fp8_linear_weight_grad", "fp8_quantize", "layer_norm", "layer_norm_backward")
+
+
+def __getattr__(name):
+    if name in _FP8_NAMES:
+        from . import fp8
+        globals().update({n: getattr(fp8, n) for n in _FP8_NAMES})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
