@@ -18,7 +18,8 @@
 //
 // Warp roles (10 warps): 0 TMA producer, 1 TMEM allocator and MMA issuer,
 // 2..9 epilogue (two groups of four, each half of the tile's columns).  The
-// grid is persistent, one CTA per SM.
+// grid is persistent, one CTA per SM.  An epilogue thread keeps 128 sums and
+// two 16-column reads of TMEM in its 168 registers.
 #include <algorithm>
 
 #include "fp8.h"
@@ -31,6 +32,7 @@ constexpr int kBM = 128;
 constexpr int kBR = 128;  // reduction per stage: one scale block, one swizzle row
 constexpr uint32_t kABytes = kBM * kBR;
 constexpr int kThreads = 320;
+constexpr int kEpiWarp0 = 2;
 constexpr int kMaxStages = 6;
 constexpr uint32_t kSlabBytes = 32 * 128;  // per epilogue warp: 32 rows x 128 B
 
@@ -40,7 +42,7 @@ struct Cfg {
   static constexpr uint32_t kBBytes = kBN * kBR;
   static constexpr size_t kSmem = 1024 + kStages * (kABytes + kBBytes) + 8 * kSlabBytes + 256;
 };
-static_assert(Cfg<256>::kSmem <= 232448 && Cfg<128>::kSmem <= 232448 && Cfg<64>::kSmem <= 232448,
+static_assert(Cfg<256>::kSmem <= 232448 && Cfg<128>::kSmem <= 232448,
               "shared memory budget");
 
 struct Bars {
@@ -198,8 +200,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------------------------------------------------- epilogue
-    const int quad = warp & 3, group = (warp - 2) >> 2;
-    uint8_t* slab = sE + (warp - 2) * kSlabBytes;
+    const int quad = warp & 3, group = (warp - kEpiWarp0) >> 2;
+    uint8_t* slab = sE + (warp - kEpiWarp0) * kSlabBytes;
     const int ncb = (a.NO + 127) / 128;
     uint32_t it = 0;
     for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
@@ -212,12 +214,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       float acc[kHalfN];
 #pragma unroll
       for (int e = 0; e < kHalfN; ++e) acc[e] = 0.f;
-      float sc = xsr[0] * wsr[0];
+      // the next block's scales are loaded a block ahead, multiplied at use
+      float xs_next = xsr[0], ws_next = wsr[0];
       bool ok = true;
       for (int b = 0; b < a.rb; ++b, ++it) {
         const int buf = it & 1;
-        const float s = sc;
-        if (b + 1 < a.rb) sc = xsr[b + 1] * wsr[static_cast<int64_t>(b + 1) * wstep];
+        const float xs_now = xs_next, ws_now = ws_next;
+        if (b + 1 < a.rb) {
+          xs_next = xsr[b + 1];
+          ws_next = wsr[static_cast<int64_t>(b + 1) * wstep];
+        }
         if (!mbar_wait(&ss->tfull[buf], (it >> 1) & 1, a.err, kDevTimeoutMma)) {
           *abort_flag = 1;
           ok = false;
@@ -226,30 +232,55 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t taddr =
             tmem + (static_cast<uint32_t>(quad * 32) << 16) + buf * kBN + group * kHalfN;
+        // 16 columns are added up while the next 16 come from TMEM
+        uint32_t r[2][16];
+        tmem_ld16(taddr, r[0]);
+        const float s = xs_now * ws_now;
 #pragma unroll
-        for (int c = 0; c < kHalfN; c += 32) {
-          uint32_t r[32];
-          tmem_ld32(taddr + c, r);
+        for (int c = 0; c < kHalfN; c += 16) {
+          uint32_t(&cur)[16] = r[(c / 16) & 1];
           tmem_ld_wait();
+          if (c + 16 < kHalfN) {
+            tmem_ld16(taddr + c + 16, r[(c / 16 + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ss->tempty[buf]);
+          }
 #pragma unroll
-          for (int e = 0; e < 32; e += 2)
-            fma_f32x2v(acc[c + e], acc[c + e + 1], __uint_as_float(r[e]),
-                       __uint_as_float(r[e + 1]), s, acc[c + e], acc[c + e + 1]);
+          for (int e = 0; e < 16; e += 2)
+            fma_f32x2v(acc[c + e], acc[c + e + 1], __uint_as_float(cur[e]),
+                       __uint_as_float(cur[e + 1]), s, acc[c + e], acc[c + e + 1]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ss->tempty[buf]);
       }
       if (!ok) break;
       const TO* bias = static_cast<const TO*>(a.bias);
+      const bool bias_vec = (reinterpret_cast<uintptr_t>(bias) & 15) == 0;
       TO* y = static_cast<TO*>(a.y);
 #pragma unroll
       for (int c = 0; c < kHalfN; c += kSlabCols) {
         if (n0 + c >= a.NO) break;  // warp-uniform
         if (bias) {
+          if (bias_vec && n0 + c + kSlabCols <= a.NO) {
 #pragma unroll
-          for (int e = 0; e < kSlabCols; ++e)
-            if (n0 + c + e < a.NO) acc[c + e] += to_f32(bias[n0 + c + e]);
+            for (int e = 0; e < kSlabCols; e += 16 / static_cast<int>(sizeof(TO))) {
+              const uint4 q = *reinterpret_cast<const uint4*>(bias + n0 + c + e);
+              const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(TO) == 4) {
+                  acc[c + e + i] += __uint_as_float(w[i]);
+                } else {
+                  acc[c + e + 2 * i] += __uint_as_float(w[i] << 16);
+                  acc[c + e + 2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
+                }
+              }
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < kSlabCols; ++e)
+              if (n0 + c + e < a.NO) acc[c + e] += to_f32(bias[n0 + c + e]);
+          }
         }
         if (a.tma_out) {
           if (lane == 0) bulk_wait_read<0>();  // the store before has read the slab

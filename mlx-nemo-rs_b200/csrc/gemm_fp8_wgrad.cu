@@ -16,14 +16,25 @@
 // The bf16 checkpoint never exists in HBM, and the codes are half its bytes.
 // The kernel is bound by the bf16 tensor rate.
 //
-// One tile per CTA.  Where the tiles do not fill the SMs, a cluster of 2, 4 or
-// 8 CTAs splits the tokens of one tile; the partial tiles are summed in rank
-// order through distributed shared memory, so the result does not depend on
-// timing and needs no workspace.
+// Tiles are 128 k x 256 n, one per CTA.  Where they do not fill the SMs, a
+// cluster of 2, 4 or 8 CTAs splits the tokens of one tile; the partial tiles
+// are summed in rank order through distributed shared memory, so the result
+// does not depend on timing and needs no workspace.  The bias' gradient is
+// summed from the dy tiles in shared memory, which all of a column's tiles
+// hold: each takes every tiles_k-th 8 columns, so that no CTA is the slowest.
 //
-// Warp roles (16 warps): 0 TMA producer, 1 TMEM allocator and MMA issuer,
-// 4..7 the bias sums (in the tiles with k0 = 0, from the dy tiles in shared
-// memory), 8..15 dequantisation; all store the result.
+// Shared-memory traffic costs most: per 64 tokens 48 KB of MMA operands, 40 KB
+// of TMA writes and 24 KB of conversion, 896 cycles at 128 bytes each against
+// the tensor cores' 512.  Tried and slower at 16000 x 4096 x 1024 (133 us
+// here): CTA pairs with 256 x 256 tiles (165, the hand-off of both CTAs'
+// conversions to one issuer), 512-wide tiles (145), the k0 = 0 tiles summing
+// all of the bias (170 to 195), CTAs of its own for the bias (133, but a
+// second wave of clusters at 1024 x 1024).
+//
+// Warp roles (23 warps): 0 TMA producer of dy, 1 TMEM allocator and MMA
+// issuer, 2 TMA producer of the codes, 3..6 the bias, 7..22 dequantisation:
+// four sets of four warps that take every fourth step, so that a set's waits
+// hide under the other sets' work.  Warps 0..15 store the result.
 #include <algorithm>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -34,26 +45,29 @@
 namespace nrp {
 namespace {
 
-constexpr int kTK = 128;   // k columns of a tile: MMA M, one scale block
-constexpr int kTN = 256;   // n columns of a tile: MMA N
-constexpr int kTok = 64;   // tokens per stage
+constexpr int kTK = 128;    // k columns of a CTA: one scale block
+constexpr int kTN = 256;    // n columns of a tile: MMA N
+constexpr int kTok = 64;    // tokens per stage
 constexpr int kStages = 4;
-constexpr int kRaw = 4;    // stages of the code ring
-constexpr uint32_t kABytes = kTok * kTK * 2;   // two 64-column blocks of 8 KB
-constexpr uint32_t kBBytes = kTok * kTN * 2;   // four of 8 KB
-constexpr uint32_t kBlk = kTok * 128;          // bytes of a 64-column bf16 block
+constexpr int kSets = 4;    // dequantising sets of four warps
+constexpr int kBiasWarp0 = 3, kBiasWarps = 4;
+constexpr int kDeqWarp0 = kBiasWarp0 + kBiasWarps;
+constexpr int kThreads = 32 * (kDeqWarp0 + 4 * kSets);
+constexpr int kStoreThreads = 512;
+constexpr uint32_t kBlk = kTok * 128;         // bytes of a 64-column bf16 block
+constexpr uint32_t kABytes = kTK / 64 * kBlk;
+constexpr uint32_t kBBytes = kTN / 64 * kBlk;
 constexpr uint32_t kRawBytes = kTok * kTK;
-constexpr int kThreads = 512;
-constexpr size_t kSmem = 1024 + kStages * (kABytes + kBBytes) + kRaw * kRawBytes + 512;
+constexpr size_t kSmem = 1024 + kStages * (kABytes + kBBytes + kRawBytes) + kTN * 4 + 256;
 static_assert(kSmem <= 232448, "shared memory budget");
-static_assert(kTN * kTK * 4 + kTN * 4 <= kStages * (kABytes + kBBytes), "partial tile fits the stages");
+static_assert(kTN * kTK * 4 <= kStages * (kABytes + kBBytes), "a partial tile fits the stages");
 
 struct Bars {
   uint64_t full[kStages];   // dy by TMA
   uint64_t deq[kStages];    // codes dequantised
   uint64_t empty[kStages];
-  uint64_t rfull[kRaw];
-  uint64_t rempty[kRaw];
+  uint64_t rfull[kStages];   // codes by TMA
+  uint64_t rempty[kStages];
   uint64_t done;
   uint32_t tmem_base;
   int abort;
@@ -85,6 +99,62 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
   return v;
 }
 
+// The sum of four floats at one shared-memory offset over the cluster's first
+// `ranks` (2, 4 or 8) CTAs, in rank order, all loads in flight together.
+__device__ __forceinline__ float4 cluster_sum4(uint32_t at, int ranks) {
+  float4 v[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    if (q < ranks) v[q] = ld_cluster_f4(at, q);
+  float4 s = v[0];
+#pragma unroll
+  for (int q = 1; q < 8; ++q)
+    if (q < ranks) {
+      s.x += v[q].x;
+      s.y += v[q].y;
+      s.z += v[q].z;
+      s.w += v[q].w;
+    }
+  return s;
+}
+
+__device__ __forceinline__ float cluster_sum1(uint32_t at, int ranks) {
+  float v[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    if (q < ranks)
+      asm volatile(
+          "{\n\t.reg .b32 ra;\n\t"
+          "mapa.shared::cluster.u32 ra, %1, %2;\n\t"
+          "ld.shared::cluster.f32 %0, [ra];\n\t}\n"
+          : "=f"(v[q])
+          : "r"(at), "r"(q)
+          : "memory");
+  float s = v[0];
+#pragma unroll
+  for (int q = 1; q < 8; ++q)
+    if (q < ranks) s += v[q];
+  return s;
+}
+
+// Two bf16 (low half first) of two codes in bytes 0 and 1 (sel 0x1404 of the
+// word) or 2 and 3 (0x3424), times f.  A code's seven exponent and mantissa
+// bits, moved to bf16's places, read as value * 2^-120 (the biases are 7 and
+// 127; subnormal codes come out as bf16 subnormals, which the multiply
+// takes); f is the block's scale * 2^120.  The NaN code is not one here.
+template <uint32_t kSel>
+__device__ __forceinline__ uint32_t codes_to_bf16(uint32_t w, uint32_t f) {
+  const uint32_t t = __byte_perm(w, 0u, kSel);  // each code in the high byte of its half
+  const uint32_t v = (t & 0x80008000u) | ((t >> 4) & 0x07F007F0u);
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(f));
+  return d;
+}
+// Whether a byte of w is the NaN code.
+__device__ __forceinline__ bool has_nan_code(uint32_t w) {
+  return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
+}
+
 template <typename TO>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy,  // bf16 [M, N], box (64, 64)
@@ -96,13 +166,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sA = base;
   uint8_t* sB = sA + kStages * kABytes;
   uint8_t* sR = sB + kStages * kBBytes;
-  Bars* ss = reinterpret_cast<Bars*>(sR + kRaw * kRawBytes);
+  float* sBias = reinterpret_cast<float*>(sR + kStages * kRawBytes);  // [kTN]
+  Bars* ss = reinterpret_cast<Bars*>(sBias + kTN);
   const int warp = warp_id(), lane = lane_id();
   const int tiles_k = (a.K + kTK - 1) / kTK;
-  const int tile = blockIdx.x / a.split, rank = blockIdx.x % a.split;
+  const int tile = static_cast<int>(blockIdx.x) / a.split;
+  const int rank = static_cast<int>(blockIdx.x) % a.split;
   const int kt = tile % tiles_k;
   const int k0 = kt * kTK, n0 = tile / tiles_k * kTN;
-  const bool bias = a.db != nullptr && kt == 0;
   const int all = (a.M + kTok - 1) / kTok;
   const int st0 = static_cast<int>(static_cast<int64_t>(all) * rank / a.split);
   const int steps = static_cast<int>(static_cast<int64_t>(all) * (rank + 1) / a.split) - st0;
@@ -110,12 +181,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&ss->full[s], 1);
-      mbar_init(&ss->deq[s], 8);
-      mbar_init(&ss->empty[s], bias ? 5 : 1);  // the MMAs, and the bias warps
-    }
-    for (int s = 0; s < kRaw; ++s) {
+      mbar_init(&ss->deq[s], 4);
       mbar_init(&ss->rfull[s], 1);
-      mbar_init(&ss->rempty[s], 8);
+      mbar_init(&ss->rempty[s], 4);
+      mbar_init(&ss->empty[s], a.db ? 1 + kBiasWarps : 1);  // the MMAs, the bias warps
     }
     mbar_init(&ss->done, 1);
     ss->abort = 0;
@@ -135,39 +204,42 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
 
-  float bsum0 = 0.f, bsum1 = 0.f;  // bias warps: columns n0 + 2 * (thread - 128), + 1
   if (warp == 0) {
     // ---------------------------------------------------------- producer
     if (lane == 0) {
-      int i = 0, r = 0;  // dy stages and code stages issued
-      // the code ring runs ahead of the dy ring by up to its depth: each
-      // round issues whatever has room, codes first
+      int i = 0;
       for (; i < steps && !*abort_flag; ++i) {
-        const int m0 = (st0 + i) * kTok;
-        const int sr = r % kRaw;
-        if (!mbar_wait(&ss->rempty[sr], ((r / kRaw) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
-          *abort_flag = 1;
-          break;
-        }
-        mbar_arrive_expect_tx(&ss->rfull[sr], kRawBytes);
-        tma_load_2d(sR + sr * kRawBytes, &map_xq, &ss->rfull[sr], k0, m0);
-        ++r;
         const int s = i % kStages;
-        if (!mbar_wait(&ss->empty[s], ((i / kStages) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
+        if (!mbar_wait_hot(&ss->empty[s], ((i / kStages) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
           *abort_flag = 1;
           break;
         }
         mbar_arrive_expect_tx(&ss->full[s], kBBytes);
 #pragma unroll
         for (int j = 0; j < kTN / 64; ++j)
-          tma_load_2d(sB + s * kBBytes + j * kBlk, &map_dy, &ss->full[s], n0 + j * 64, m0);
+          tma_load_2d(sB + s * kBBytes + j * kBlk, &map_dy, &ss->full[s], n0 + j * 64,
+                      (st0 + i) * kTok);
       }
-      if (*abort_flag) {  // the copies in flight land before the CTA goes
+      if (*abort_flag)  // the copies in flight land before the CTA goes
         for (int j = i > kStages ? i - kStages : 0; j < i; ++j)
-          mbar_wait(&ss->full[j % kStages], (j / kStages) & 1, nullptr, 0);
-        for (int j = r > kRaw ? r - kRaw : 0; j < r; ++j)
-          mbar_wait(&ss->rfull[j % kRaw], (j / kRaw) & 1, nullptr, 0);
+          mbar_wait_hot(&ss->full[j % kStages], (j / kStages) & 1, nullptr, 0);
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------- producer of the codes
+    if (lane == 0) {
+      int i = 0;
+      for (; i < steps && !*abort_flag; ++i) {
+        const int s = i % kStages;
+        if (!mbar_wait_hot(&ss->rempty[s], ((i / kStages) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
+          *abort_flag = 1;
+          break;
+        }
+        mbar_arrive_expect_tx(&ss->rfull[s], kRawBytes);
+        tma_load_2d(sR + s * kRawBytes, &map_xq, &ss->rfull[s], k0, (st0 + i) * kTok);
       }
+      if (*abort_flag)
+        for (int j = i > kStages ? i - kStages : 0; j < i; ++j)
+          mbar_wait_hot(&ss->rfull[j % kStages], (j / kStages) & 1, nullptr, 0);
     }
   } else if (warp == 1) {
     // -------------------------------------------------------- MMA issuer
@@ -175,8 +247,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t idesc = idesc_bf16_f32(kTK, kTN, 1, 1);
       for (int i = 0; i < steps; ++i) {
         const int s = i % kStages;
-        if (*abort_flag || !mbar_wait(&ss->full[s], (i / kStages) & 1, a.err, kDevTimeoutLoad) ||
-            !mbar_wait(&ss->deq[s], (i / kStages) & 1, a.err, kDevTimeoutLoad)) {
+        if (*abort_flag || !mbar_wait_hot(&ss->full[s], (i / kStages) & 1, a.err, kDevTimeoutLoad) ||
+            !mbar_wait_hot(&ss->deq[s], (i / kStages) & 1, a.err, kDevTimeoutLoad)) {
           *abort_flag = 1;
           break;
         }
@@ -190,159 +262,198 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       umma_commit(&ss->done);
     }
-  } else if (warp >= 8) {
+  } else if (warp >= kBiasWarp0 && warp < kDeqWarp0) {
+    // ----------------------------------------------------------- bias sums
+    // the tile's 8-column chunks kt, kt + tiles_k, ...: four to a round over
+    // the warps, a lane tokens lane and lane + 32
+    if (a.db) {
+      constexpr int kOwn = kTN / 8 / kBiasWarps;  // chunks a warp has at most
+      const int c0 = kt + (warp - kBiasWarp0) * tiles_k, cstep = kBiasWarps * tiles_k;
+      float sum[kOwn][8];
+#pragma unroll
+      for (int j = 0; j < kOwn; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[j][e] = 0.f;
+      for (int i = 0; i < steps; ++i) {
+        const int s = i % kStages;
+        if (*abort_flag || !mbar_wait_hot(&ss->full[s], (i / kStages) & 1, a.err, kDevTimeoutLoad)) {
+          *abort_flag = 1;
+          break;
+        }
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) {
+          const int c = c0 + j * cstep;
+          if (c >= kTN / 8) break;
+#pragma unroll
+          for (int h = 0; h < kTok; h += 32) {
+            const uint4 q = *reinterpret_cast<const uint4*>(
+                sB + s * kBBytes + (c >> 3) * kBlk + sw128_offset(h + lane, c & 7));
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              sum[j][2 * e] += __uint_as_float(w[e] << 16);
+              sum[j][2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ss->empty[s]);
+      }
+#pragma unroll
+      for (int j = 0; j < kOwn; ++j) {
+        const int c = c0 + j * cstep;
+        if (c >= kTN / 8) break;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float v = sum[j][e];
+#pragma unroll
+          for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+          if (lane == 0) sBias[c * 8 + e] = v;
+        }
+      }
+    }
+  } else {
     // ------------------------------------------------------ dequantisation
-    // thread: 16 codes (one 16-byte chunk c of the 128-byte row) of tokens
-    // row and row + 32
-    const int t = threadIdx.x - 256;
+    // set `set` of four warps takes steps set, set + kSets, ...; a thread 16
+    // codes (one 16-byte chunk c of the 128-byte row) of tokens row, row + 16, ...
+    constexpr int kRowsT = kTok / 16;
+    const int set = (warp - kDeqWarp0) >> 2;
+    const int t = threadIdx.x - 32 * (kDeqWarp0 + 4 * set);
     const int row = t >> 3, c = t & 7;
+    // chunk c: columns 16 c .. 16 c + 15 = 16-byte chunks 2 (c % 4), + 1 of
+    // 64-column block c / 4.  Chunks 4..7 store their second half first, so
+    // that the 16-byte stores of a row's eight threads fall on different banks
     const int flip = c >> 2;
+    const uint32_t at0 = (c >> 2) * kBlk + sw128_offset(row, 2 * (c & 3) + flip);
+    const uint32_t at1 = (c >> 2) * kBlk + sw128_offset(row, 2 * (c & 3) + (flip ^ 1));
     const float* xs = a.xs + kt;
-    float sc[2];
+    float sc[kRowsT];
     auto scales = [&](int i) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int m = (st0 + i) * kTok + row + 32 * h;
+      for (int h = 0; h < kRowsT; ++h) {
+        const int m = (st0 + i) * kTok + row + 16 * h;
         sc[h] = i < steps && m < a.M ? xs[static_cast<int64_t>(m) * a.kb] : 0.f;
       }
     };
-    scales(0);
-    for (int i = 0; i < steps; ++i) {
-      const int s = i % kStages, sr = i % kRaw;
-      const float s0 = sc[0], s1 = sc[1];
-      scales(i + 1);
-      if (*abort_flag || !mbar_wait(&ss->rfull[sr], (i / kRaw) & 1, a.err, kDevTimeoutLoad)) {
+    scales(set);
+    for (int i = set; i < steps; i += kSets) {
+      const int s = i % kStages;
+      const uint32_t round = i / kStages;
+      float sn[kRowsT];
+#pragma unroll
+      for (int h = 0; h < kRowsT; ++h) sn[h] = sc[h];
+      scales(i + kSets);
+      if (*abort_flag || !mbar_wait_hot(&ss->rfull[s], round & 1, a.err, kDevTimeoutLoad)) {
         *abort_flag = 1;
         break;
       }
-      uint4 q[2];
+      uint4 q[kRowsT];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        q[h] = *reinterpret_cast<const uint4*>(sR + sr * kRawBytes + (row + 32 * h) * 128 + c * 16);
+      for (int h = 0; h < kRowsT; ++h)
+        q[h] = *reinterpret_cast<const uint4*>(sR + s * kRawBytes + (row + 16 * h) * 128 + c * 16);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ss->rempty[sr]);
-      if (!mbar_wait(&ss->empty[s], ((i / kStages) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
+      if (lane == 0) mbar_arrive(&ss->rempty[s]);
+      uint32_t out[kRowsT][8];
+#pragma unroll
+      for (int h = 0; h < kRowsT; ++h) {
+        const float f = sn[h];
+        const uint32_t w[4] = {flip ? q[h].z : q[h].x, flip ? q[h].w : q[h].y,
+                               flip ? q[h].x : q[h].z, flip ? q[h].y : q[h].w};
+        uint32_t(&o)[8] = out[h];
+        // a power of two in [2^-117, 2^7] and no NaN code: the product is
+        // exact, by bits; anything else through f32 (rounded once)
+        const uint32_t fb = __float_as_uint(f);
+        const bool nan = has_nan_code(w[0]) | has_nan_code(w[1]) | has_nan_code(w[2]) |
+                         has_nan_code(w[3]);
+        if ((fb & 0x807fffffu) == 0 && fb - (10u << 23) <= (124u << 23) && !nan) {
+          const uint32_t f2 = ((fb >> 16) + (120u << 7)) * 0x10001u;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            o[2 * e] = codes_to_bf16<0x1404>(w[e], f2);
+            o[2 * e + 1] = codes_to_bf16<0x3424>(w[e], f2);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(
+                static_cast<__nv_fp8x2_storage_t>((w[e >> 1] >> (16 * (e & 1))) & 0xffffu),
+                __NV_E4M3);
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hr));
+            o[e] = pack_bf16x2(v.x * f, v.y * f);
+          }
+        }
+      }
+      // only the stores wait for the MMAs that still read the stage
+      if (!mbar_wait_hot(&ss->empty[s], (round & 1) ^ 1, a.err, kDevTimeoutLoad)) {
         *abort_flag = 1;
         break;
       }
-      // chunk c: columns 16 c .. 16 c + 15 = 16-byte chunks 2 (c % 4), + 1 of
-      // 64-column block c / 4
-      uint8_t* dst = sA + s * kABytes + (c >> 2) * kBlk;
+      uint8_t* dst = sA + s * kABytes;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float f = h ? s1 : s0;
-        const uint32_t w[4] = {q[h].x, q[h].y, q[h].z, q[h].w};
-        uint32_t o[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(
-              static_cast<__nv_fp8x2_storage_t>((w[e >> 1] >> (16 * (e & 1))) & 0xffffu),
-              __NV_E4M3);
-          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hr));
-          o[e] = pack_bf16x2(v.x * f, v.y * f);
-        }
-        // the two halves of a quarter warp's rows take the chunks in opposite
-        // order, so their 16-byte stores fall on different banks
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const int hi = p ^ flip;
-          const uint4 v = hi ? make_uint4(o[4], o[5], o[6], o[7]) : make_uint4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<uint4*>(dst + sw128_offset(row + 32 * h, 2 * (c & 3) + hi)) = v;
-        }
+      for (int h = 0; h < kRowsT; ++h) {
+        // (16 rows on: two 1024-byte atoms, the same place in them)
+        *reinterpret_cast<uint4*>(dst + at0 + 2048 * h) =
+            make_uint4(out[h][0], out[h][1], out[h][2], out[h][3]);
+        *reinterpret_cast<uint4*>(dst + at1 + 2048 * h) =
+            make_uint4(out[h][4], out[h][5], out[h][6], out[h][7]);
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ss->deq[s]);
     }
-  } else if (warp >= 4 && bias) {
-    // ----------------------------------------------------------- bias sums
-    const int t = threadIdx.x - 128;  // columns 2t, 2t + 1
-    const int chunk = (t & 31) >> 2, word = t & 3;
-    for (int i = 0; i < steps; ++i) {
-      const int s = i % kStages;
-      if (*abort_flag || !mbar_wait(&ss->full[s], (i / kStages) & 1, a.err, kDevTimeoutLoad)) {
-        *abort_flag = 1;
-        break;
-      }
-      const uint8_t* b = sB + s * kBBytes + (t >> 5) * kBlk;
-      float p0 = 0.f, p1 = 0.f;
-#pragma unroll 16
-      for (int m = 0; m < kTok; ++m) {
-        const uint32_t u = *reinterpret_cast<const uint32_t*>(b + sw128_offset(m, chunk) + word * 4);
-        p0 += __uint_as_float(u << 16);
-        p1 += __uint_as_float(u & 0xffff0000u);
-      }
-      bsum0 += p0;
-      bsum1 += p1;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ss->empty[s]);
-    }
   }
 
   // ------------------------------------------------------------- the result
   __syncwarp();
-  const bool fine = mbar_wait(&ss->done, 0, a.err, kDevTimeoutMma);
+  const bool fine = mbar_wait_hot(&ss->done, 0, a.err, kDevTimeoutMma);
   if (!fine) *abort_flag = 1;
   tc_fence_after();
   __syncthreads();
-  const int quad = warp & 3, grp = warp >> 2;  // 64 columns of n each
-  const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + grp * 64;
+  const int quad = warp & 3, grp = warp >> 2;  // a quarter of n each
+  const bool storer = threadIdx.x < kStoreThreads;
+  const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16);
   TO* dw = static_cast<TO*>(a.dw);
   TO* db = static_cast<TO*>(a.db);
+  // bias columns this CTA summed (this rank writes its share of them)
+  auto bias_here = [&](int c) { return db && (c >> 3) % tiles_k == kt && n0 + c < a.N; };
   if (a.split == 1) {
-    if (!*abort_flag) {
+    if (!*abort_flag && storer) {
       const int k = k0 + quad * 32 + lane;
-#pragma unroll
-      for (int c = 0; c < 64; c += 32) {
+#pragma unroll 1
+      for (int c = grp * 64; c < grp * 64 + 64; c += 32) {
         uint32_t r[32];
         tmem_ld32(taddr + c, r);
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const int n = n0 + grp * 64 + c + e;
+          const int n = n0 + c + e;
           if (n < a.N && k < a.K)
-            store_one(dw + static_cast<int64_t>(n) * a.K + k,
-                      steps > 0 ? __uint_as_float(r[e]) : 0.f);
+            store_one(dw + static_cast<int64_t>(n) * a.K + k, __uint_as_float(r[e]));
         }
       }
-      if (bias && warp >= 4 && warp < 8) {
-        const int n = n0 + 2 * (static_cast<int>(threadIdx.x) - 128);
-        if (n < a.N) store_one(db + n, bsum0);
-        if (n + 1 < a.N) store_one(db + n + 1, bsum1);
-      }
+      if (threadIdx.x < kTN && bias_here(threadIdx.x))
+        store_one(db + n0 + threadIdx.x, sBias[threadIdx.x]);
     }
   } else {
-    // partial tile [n][k] f32 and bias sums over the (drained) stages
+    // partial sums [256 n][128 k] f32 over the (drained) stages
     float* part = reinterpret_cast<float*>(base);
-    float* bpart = part + kTN * kTK;
+    if (storer) {
+#pragma unroll 1
+      for (int c = grp * 64; c < grp * 64 + 64; c += 32) {
+        uint32_t r[32];
+        tmem_ld32(taddr + c, r);
+        tmem_ld_wait();
 #pragma unroll
-    for (int c = 0; c < 64; c += 32) {
-      uint32_t r[32];
-      tmem_ld32(taddr + c, r);
-      tmem_ld_wait();
-#pragma unroll
-      for (int e = 0; e < 32; ++e)
-        part[(grp * 64 + c + e) * kTK + quad * 32 + lane] =
-            steps > 0 ? __uint_as_float(r[e]) : 0.f;
-    }
-    if (bias && warp >= 4 && warp < 8) {
-      bpart[2 * (threadIdx.x - 128)] = bsum0;
-      bpart[2 * (threadIdx.x - 128) + 1] = bsum1;
+        for (int e = 0; e < 32; ++e)
+          part[(c + e) * kTK + quad * 32 + lane] = __uint_as_float(r[e]);
+      }
     }
     cluster_sync();
     // this rank's columns, four k at a time, the ranks' tiles in order
     const int cols = kTN / a.split;
     for (int u = threadIdx.x; u < cols * (kTK / 4); u += kThreads) {
       const int nn = rank * cols + u / (kTK / 4), kk = (u % (kTK / 4)) * 4;
-      const uint32_t at = smem_u32(part + nn * kTK + kk);
-      float4 sum = ld_cluster_f4(at, 0);
-      for (int q = 1; q < a.split; ++q) {
-        const float4 v = ld_cluster_f4(at, q);
-        sum.x += v.x;
-        sum.y += v.y;
-        sum.z += v.z;
-        sum.w += v.w;
-      }
+      const float4 sum = cluster_sum4(smem_u32(part + nn * kTK + kk), a.split);
       const int n = n0 + nn, k = k0 + kk;
       if (n < a.N && k < a.K) {  // K % 16 == 0: the four are inside together
         TO* o = dw + static_cast<int64_t>(n) * a.K + k;
@@ -352,21 +463,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         store_one(o + 3, sum.w);
       }
     }
-    if (bias)
-      for (int u = threadIdx.x; u < cols / 4; u += kThreads) {
-        const int nn = rank * cols + 4 * u;
-        float4 sum = ld_cluster_f4(smem_u32(bpart + nn), 0);
-        for (int q = 1; q < a.split; ++q) {
-          const float4 v = ld_cluster_f4(smem_u32(bpart + nn), q);
-          sum.x += v.x;
-          sum.y += v.y;
-          sum.z += v.z;
-          sum.w += v.w;
-        }
-        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-        for (int e = 0; e < 4; ++e)
-          if (n0 + nn + e < a.N) store_one(db + n0 + nn + e, v[e]);
-      }
+    for (int c = threadIdx.x; c < cols; c += kThreads) {
+      const int nn = rank * cols + c;
+      if (bias_here(nn)) store_one(db + n0 + nn, cluster_sum1(smem_u32(sBias + nn), a.split));
+    }
     cluster_sync();  // no CTA leaves while another reads its tile
   }
   tc_fence_before();
@@ -377,8 +477,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// The clusters of `size` CTAs of the kernel that fit the device at once.
+template <typename F>
+int max_clusters(F* kernel, int size, size_t smem) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(size));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute la[1];
+  la[0].id = cudaLaunchAttributeClusterDimension;
+  la[0].val.clusterDim.x = static_cast<unsigned>(size);
+  la[0].val.clusterDim.y = 1;
+  la[0].val.clusterDim.z = 1;
+  cfg.attrs = la;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return n;
+}
+
 template <typename TO>
-cudaError_t launch(const void* dy, const uint8_t* xq, Args a, int num_sms, cudaStream_t stream) {
+cudaError_t launch(const void* dy, const uint8_t* xq, Args a, cudaStream_t stream) {
   static std::atomic<uint64_t> attr{0};
   auto* kernel = fp8_wgrad_kernel<TO>;
   if (cudaError_t e = smem_attr_once(kernel, static_cast<int>(kSmem), attr)) return e;
@@ -388,11 +510,21 @@ cudaError_t launch(const void* dy, const uint8_t* xq, Args a, int num_sms, cudaS
       !make_tmap_2d(&mxq, xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.M, a.K, kTK, kTok, false))
     return cudaErrorInvalidValue;
   const int64_t tiles = qblocks(a.K) * ((a.N + kTN - 1) / kTN);
+  // the largest split whose clusters all run at once, and that leaves every
+  // CTA a step (on a B200 33 clusters of four fit, but only 15 of eight)
+  static std::atomic<int> fit[64][4];
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
   const int steps = (a.M + kTok - 1) / kTok;
-  // the largest split whose clusters still fit the SMs at once, and that
-  // leaves every CTA a step
   a.split = 1;
-  while (a.split < 8 && tiles * a.split * 2 <= num_sms && a.split * 2 <= steps) a.split *= 2;
+  for (int l = 1; l <= 3 && (1 << l) <= steps; ++l) {
+    int f = fit[dev & 63][l].load(std::memory_order_relaxed);
+    if (f == 0) {
+      f = max_clusters(kernel, 1 << l, kSmem);
+      fit[dev & 63][l].store(f > 0 ? f : -1, std::memory_order_relaxed);
+    }
+    if (tiles <= f) a.split = 1 << l;
+  }
   if (tiles * a.split > 0x7fffffff) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * a.split));
@@ -415,7 +547,7 @@ cudaError_t launch(const void* dy, const uint8_t* xq, Args a, int num_sms, cudaS
 
 cudaError_t launch_fp8_weight_grad(bool bf16_out, const void* dy, const uint8_t* xq,
                                    const float* xs, int M, int N, int K, void* dw, void* db,
-                                   int num_sms, int* err, cudaStream_t stream) {
+                                   int* err, cudaStream_t stream) {
   if (M <= 0) {  // no tokens: the sums are empty
     const size_t es = bf16_out ? 2 : 4;
     if (cudaError_t e = cudaMemsetAsync(dw, 0, static_cast<size_t>(N) * K * es, stream)) return e;
@@ -430,8 +562,8 @@ cudaError_t launch_fp8_weight_grad(bool bf16_out, const void* dy, const uint8_t*
   a.K = K;
   a.kb = static_cast<int>(qblocks(K));
   a.err = err;
-  return bf16_out ? launch<__nv_bfloat16>(dy, xq, a, num_sms, stream)
-                  : launch<float>(dy, xq, a, num_sms, stream);
+  return bf16_out ? launch<__nv_bfloat16>(dy, xq, a, stream)
+                  : launch<float>(dy, xq, a, stream);
 }
 
 }  // namespace nrp

@@ -90,6 +90,31 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* e
   }
 }
 
+// The same wait for hand-offs a few hundred cycles apart: without the suspend
+// hint the thread is back sooner once the phase completes.
+__device__ __forceinline__ bool mbar_wait_hot(uint64_t* bar, uint32_t parity, int* err, int code) {
+  auto test = [&]() {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+  };
+  if (test()) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t it = 1;; ++it) {
+    if (test()) return true;
+    if ((it & 63u) == 0 && globaltimer_ns() - t0 > kWaitBudgetNs) {
+      if (err) atomicCAS(err, 0, code);
+      return false;
+    }
+  }
+}
+
 // bytes (a multiple of 16, both addresses 16-byte aligned) from global to
 // this CTA's shared memory, completing on `bar` (an untiled bulk copy)
 __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes,

@@ -138,9 +138,12 @@ def test_layer_norm_backward_refusals(nrp, mem):
     n = C.c_int64(-1)
     assert nrp.lib().nrp_layer_norm_backward_workspace(9, 33, C.byref(n)) == 0
     need = n.value
+    assert need == 0  # few rows: none
+    assert nrp.lib().nrp_layer_norm_backward_workspace(3000, 33, C.byref(n)) == 0
+    need = n.value
     assert need > 0
     # ctx, stream, dtype, x, xs, dy, mean, rstd, gamma, rows, cols, dx, dg, db, ws, bytes
-    good = [p, None, F32, p, None, p, p, p, p, 9, 33, p, p, p, p, need]
+    good = [p, None, F32, p, None, p, p, p, p, 3000, 33, p, p, p, p, need]
 
     def bad(code, **kw):
         a = list(good)

@@ -147,7 +147,9 @@ def test_quantize_special_values(nrp, dtype, block):
 SHAPES = [(1, 16, 1), (1, 1024, 4096), (2, 144, 130), (14, 1024, 1024), (15, 528, 97),
           (16, 4096, 512), (17, 128, 256), (33, 256, 64), (64, 1040, 300), (65, 400, 513),
           (127, 128, 128), (128, 384, 384), (129, 640, 255), (300, 1024, 1000), (896, 1024, 1024),
-          (1000, 272, 2048)]
+          (1000, 272, 2048),
+          # 256-column tiles: ragged rows and columns, one to nine reduction blocks
+          (4737, 144, 1008), (2433, 1040, 2040), (2304, 112, 2048), (19000, 128, 250)]
 
 
 def product_tol(x, w, red, y, dtype):
@@ -185,7 +187,8 @@ def test_linear(nrp, m, k, n, kind):
 @pytest.mark.parametrize("m,k,n", [(1, 16, 16), (1, 1024, 4096), (14, 1024, 1024), (15, 144, 528),
                                    (17, 256, 128), (65, 528, 400), (128, 384, 384),
                                    (129, 240, 640), (300, 1008, 1024), (896, 1024, 1024),
-                                   (1000, 2048, 272)])
+                                   (1000, 2048, 272), (4737, 1008, 144), (2433, 2032, 1040),
+                                   (2304, 2048, 112), (19000, 240, 128)])
 @pytest.mark.parametrize("kind", ["bf16", "f32", "fp8-bf16", "fp8-f32"])
 def test_input_grad(nrp, m, k, n, kind):
     import torch
@@ -262,7 +265,9 @@ def test_empty_and_shapes(nrp):
 # ---------------------------------------------------------- weight gradient
 @pytest.mark.parametrize("m,k,n", [(1, 16, 8), (14, 128, 256), (63, 144, 264), (64, 1024, 1024),
                                    (65, 400, 1000), (129, 128, 24), (749, 512, 512),
-                                   (1000, 1040, 504), (2500, 256, 256)])
+                                   (1000, 1040, 504), (2500, 256, 256),
+                                   # one CTA per tile; more k tiles than 8-column chunks
+                                   (1, 1040, 2504), (515, 2320, 2000), (70, 4240, 264)])
 @pytest.mark.parametrize("dtype,bias", [("f32", True), ("f32", False), ("bf16", True)])
 def test_weight_grad(nrp, m, k, n, dtype, bias):
     import torch
