@@ -1,6 +1,7 @@
 """Builds libnemo_relpos.so in place: every CUDA source for sm_100a with
 nvcc (-gencode arch=compute_100a,code=sm_100a -lineinfo), the C ABI host
-code, statically linked against the CUDA runtime.
+code, statically linked against the CUDA runtime; and _nrp_torch, the
+CPython/libtorch binding of the 8-bit linears and the LayerNorm, over it.
 
     python mlx-nemo-rs_b200/build.py [--force]
 """
@@ -16,6 +17,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libnemo_relpos.so")
+BINDING_SRC = os.path.join(HERE, "torch_binding.cpp")
+BINDING = os.path.join(HERE, "_nrp_torch.so")
 NVCC = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
@@ -67,6 +70,32 @@ def _compile(src, force):
     return obj, r.stderr
 
 
+def _build_binding(force):
+    """_nrp_torch.so against the running interpreter's torch (its headers
+    make this the slowest file: about a minute)."""
+    import importlib.util
+    import sysconfig
+    hdr = os.path.join(os.path.dirname(HERE), "include", "nemo_relpos.h")
+    if not force and not _stale(BINDING, [BINDING_SRC, hdr]):
+        return ""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:  # the C library serves without it
+        return ""
+    torch = os.path.dirname(spec.origin)
+    inc = [os.path.join(torch, "include"),
+           os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], "/usr/local/cuda/include"]
+    libs = os.path.join(torch, "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-DTORCH_EXTENSION_NAME=_nrp_torch",
+           *[f"-isystem{d}" for d in inc], BINDING_SRC, "-o", BINDING, f"-L{libs}", f"-L{HERE}",
+           "-l:libnemo_relpos.so", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda",
+           "-lc10", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    return r.stderr
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
@@ -81,6 +110,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    log = _build_binding(force)
+    if verbose and log.strip():
+        print(log)
     return LIB
 
 
