@@ -25,7 +25,7 @@ FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", 
          "--expt-relaxed-constexpr"]
 SOURCES = ["gemm_sm100.cu", "gemm_tf32.cu", "attn_sm100.cu", "attn_simt.cu", "attn_stream.cu", "kernels_misc.cu",
            "noalloc.cu", "block_kernels.cu", "subsampling_kernels.cu", "api.cpp", "halo.cpp",
-           "block.cpp", "subsampling.cpp", "fp8_quant.cu", "gemm_fp8.cu", "gemm_fp8_wgrad.cu",
+           "block.cpp", "subsampling.cpp", "fp8_quant.cu", "gemm_fp8.cu", "gemm_fp8_small.cu", "gemm_fp8_wgrad.cu",
            "norm_kernels.cu", "fp8_api.cpp"]
 
 

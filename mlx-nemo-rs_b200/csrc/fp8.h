@@ -34,6 +34,18 @@ cudaError_t launch_gemm_fp8(bool bf16_out, bool trans, const uint8_t* xq, const 
                             int R, const uint8_t* wq, const float* ws, int NO, const void* bias,
                             void* y, int num_sms, int* err, cudaStream_t stream);
 
+// The forward product for few rows, x quantised on the way: y[M, N] = q(x) .
+// w^T (+ bias).  x (f32 or bf16 as y, 16-byte aligned) is quantised into xq, xs;
+// x null: xq, xs are inputs.  fp8_small_supported: M <= kFp8SmallMaxM and K up
+// to what M rows of codes leave room for in shared memory.
+constexpr int kFp8SmallMaxM = 32;
+// fp8_small_quantizes: M rows are better quantised by it than ahead of it.
+bool fp8_small_supported(int M, int K);
+bool fp8_small_quantizes(int M);
+cudaError_t launch_fp8_small(bool bf16, const void* x, uint8_t* xq, float* xs, int M, int K,
+                             const uint8_t* wq, const float* ws, int N, const void* bias, void* y,
+                             int num_sms, cudaStream_t stream);
+
 // dw[N, K] (f32 or bf16) = sum_m dy[m, n] * x~[m, k], x~ = xq * xs rounded
 // to bf16 (exact for power-of-two scales); db[n] = sum_m dy[m, n] in dw's
 // type (db may be null).  dy bf16 [M, N], N % 8 == 0, K % 16 == 0.

@@ -46,11 +46,19 @@ int product(nrp_context* ctx, cudaStream_t st, bool trans, int dtype, const void
             float* xs, int M, int R, const uint8_t* wq, const float* ws, int NO, const void* bias,
             void* y) {
   const bool bf16 = dtype == NRP_DTYPE_BF16;
-  if (x) {
+  const bool small = !trans && nrp::fp8_small_supported(M, R);
+  if (x && !(small && nrp::fp8_small_quantizes(M))) {
     ProfScope ps(ctx, NRP_KERNEL_FP8_QUANT, st);
     if (int rc = status(nrp::launch_fp8_quantize(bf16, x, M, R, 1, xq, xs, ctx->num_sms, st),
                         "fp8 quantize"))
       return rc;
+    x = nullptr;
+  }
+  if (small) {
+    ProfScope ps(ctx, NRP_KERNEL_FP8_SMALL, st);
+    return status(nrp::launch_fp8_small(bf16, x, xq, xs, M, R, wq, ws, NO, bias, y, ctx->num_sms,
+                                        st),
+                  "fp8 linear");
   }
   ProfScope ps(ctx, NRP_KERNEL_GEMM_FP8, st);
   return status(nrp::launch_gemm_fp8(bf16, trans, xq, xs, M, R, wq, ws, NO, bias, y, ctx->num_sms,

@@ -12,86 +12,28 @@
 // has no infinity, and a saturated one would hide an overflow.
 //
 // Both kernels are bound by HBM: they read and write each element once.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-
 #include "fp8.h"
-#include "sm100.cuh"
+#include "fp8_quant.cuh"
 
 namespace nrp {
 namespace {
 
-// log2 of the scale of a block whose largest finite magnitude is `amax`.
-__device__ __forceinline__ int scale_exp(float amax) {
-  if (!(amax > 0.f)) return 0;
-  if (amax < 1.17549435e-38f) return -117;  // subnormal: the clamp's value
-  const uint32_t u = __float_as_uint(amax);
-  // amax = 1.f * 2^e; 448 = 1.75 * 2^8
-  const int e = static_cast<int>(u >> 23) - 127;
-  const int k = e - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return min(max(k, -117), 119);
-}
-
-__device__ __forceinline__ float exp2_int(int k) {  // 2^k, k in [-126, 127]
-  return __uint_as_float(static_cast<uint32_t>(k + 127) << 23);
-}
-
-// |x| where x is finite, else 0: what amax looks at.
-__device__ __forceinline__ float finite_abs(float x) {
-  const float a = fabsf(x);
-  return a <= 3.40282347e38f ? a : 0.f;
-}
-
-// Two codes (low byte first) of x0 * inv, x1 * inv.
-__device__ __forceinline__ uint32_t codes2(float x0, float x1, float inv) {
-  // an infinity times a finite power of two stays one; inf - inf is the NaN
-  // the conversion needs, and finite - finite * 0 changes nothing
-  const float a = fabsf(x0) <= 3.40282347e38f ? x0 * inv : __uint_as_float(0x7fc00000u);
-  const float b = fabsf(x1) <= 3.40282347e38f ? x1 * inv : __uint_as_float(0x7fc00000u);
-  return static_cast<uint32_t>(
-      __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3));
-}
-
-// 16 consecutive elements as f32.
 template <typename T>
-__device__ __forceinline__ void load16(const T* p, float (&v)[16]) {
-  if constexpr (sizeof(T) == 4) {
+__device__ __forceinline__ void load_raw(const T* p, uint4* raw) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float4 f = __ldg(reinterpret_cast<const float4*>(p) + q);
-      v[4 * q] = f.x;
-      v[4 * q + 1] = f.y;
-      v[4 * q + 2] = f.z;
-      v[4 * q + 3] = f.w;
-    }
-  } else {
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + q);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]));
-        v[8 * q + 2 * e] = f.x;
-        v[8 * q + 2 * e + 1] = f.y;
-      }
-    }
-  }
+  for (int q = 0; q < kRawWords<T>; ++q) raw[q] = __ldg(reinterpret_cast<const uint4*>(p) + q);
 }
-
-__device__ __forceinline__ uint4 codes16(const float (&v)[16], float inv) {
-  uint32_t w[4];
+template <typename T>
+__device__ __forceinline__ void zero_raw(uint4* raw) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q)
-    w[q] = codes2(v[4 * q], v[4 * q + 1], inv) |
-           (codes2(v[4 * q + 2], v[4 * q + 3], inv) << 16);
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  for (int q = 0; q < kRawWords<T>; ++q) raw[q] = make_uint4(0u, 0u, 0u, 0u);
 }
 
 // 1 x 128 blocks: eight lanes of 16 elements each hold a block; a lane group
-// walks the blocks of the matrix (row-major) a grid-stride apart.
-template <typename T>
+// walks the blocks of the matrix (row-major) a grid-stride apart, kFly of them
+// in flight.  kWhole: cols % 128 == 0, so that the blocks are one after another
+// in memory.
+template <typename T, bool kWhole, int kFly>
 __global__ void __launch_bounds__(256)
     quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int cols, int cb,
                          uint8_t* __restrict__ codes, float* __restrict__ scales) {
@@ -100,26 +42,35 @@ __global__ void __launch_bounds__(256)
   const int sub = threadIdx.x & 7;
   const int64_t total = rows * cb;
   const int64_t step = static_cast<int64_t>(gridDim.x) * 32;
-  // the warp's four groups stay together for the shuffles
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x >> 5) * 4;
-       base < total; base += step) {
-    const int64_t blk = base + ((threadIdx.x & 31) >> 3);
+  // element of block blk that the lane starts at, or -1
+  auto place = [&](int64_t blk) -> int64_t {
+    if (blk >= total) return -1;
+    if (kWhole) return blk * kQBlock + sub * 16;
     const int64_t row = blk / cb;
     const int col = static_cast<int>(blk - row * cb) * kQBlock + sub * 16;
-    const bool in = blk < total && col < cols;
-    float v[16];
-    float amax = 0.f;
-    if (in) {
-      load16(x + row * cols + col, v);
+    return col < cols ? row * cols + col : -1;
+  };
+  // the warp's four groups stay together for the shuffles
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x >> 5) * 4;
+       base < total; base += kFly * step) {
+    const int64_t first = base + ((threadIdx.x & 31) >> 3);
+    uint4 raw[kFly][kRawWords<T>];
+    int64_t at[kFly];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) amax = fmaxf(amax, finite_abs(v[e]));
+    for (int i = 0; i < kFly; ++i) {
+      at[i] = place(first + i * step);
+      if (at[i] >= 0) load_raw(x + at[i], raw[i]);
+      else zero_raw<T>(raw[i]);
     }
 #pragma unroll
-    for (int o = 4; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const int k = scale_exp(amax);
-    if (in)
-      *reinterpret_cast<uint4*>(codes + row * cols + col) = codes16(v, exp2_int(-k));
-    if (blk < total && sub == 0) scales[blk] = exp2_int(k);
+    for (int i = 0; i < kFly; ++i) {
+      float scale;
+      const uint4 q = quantize_block<T>(raw[i], scale);
+      if (at[i] >= 0) {
+        *reinterpret_cast<uint4*>(codes + at[i]) = q;
+        if (sub == 0) scales[first + i * step] = scale;
+      }
+    }
   }
 }
 
@@ -128,35 +79,46 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     quantize_tiles_kernel(const T* __restrict__ x, int64_t rows, int cols, int cb,
                           uint8_t* __restrict__ codes, float* __restrict__ scales) {
-  __shared__ float part[8];
+  __shared__ uint32_t part[8];
   pdl_launch_dependents();
   pdl_wait();
   const int64_t rb = blockIdx.x / cb;
   const int col = static_cast<int>(blockIdx.x - rb * cb) * kQBlock + (threadIdx.x & 7) * 16;
-  float v[4][16];
-  float amax = 0.f;
+  uint4 raw[4][kRawWords<T>];
+  uint32_t m = 0;
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     const int64_t row = rb * 128 + p * 32 + (threadIdx.x >> 3);
-    if (row < rows && col < cols) {
-      load16(x + row * cols + col, v[p]);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) amax = fmaxf(amax, finite_abs(v[p][e]));
-    }
+    if (row < rows && col < cols) load_raw(x + row * cols + col, raw[p]);
+    else zero_raw<T>(raw[p]);
   }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
-  __syncthreads();
+  for (int p = 0; p < 4; ++p) m = max(m, amax_bits<T>(raw[p]));
+  auto over_cta = [&](uint32_t v) {
 #pragma unroll
-  for (int w = 0; w < 8; ++w) amax = fmaxf(amax, part[w]);
-  const int k = scale_exp(amax);
+    for (int o = 16; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) v = max(v, part[w]);
+    return v;
+  };
+  m = over_cta(m);
+  const bool finite = m < kInfBits;
+  if (!finite) {  // the whole CTA
+    m = 0;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) m = max(m, finite_amax_bits<T>(raw[p]));
+    __syncthreads();
+    m = over_cta(m);
+  }
+  const int k = scale_exp(m);
   const float inv = exp2_int(-k);
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     const int64_t row = rb * 128 + p * 32 + (threadIdx.x >> 3);
     if (row < rows && col < cols)
-      *reinterpret_cast<uint4*>(codes + row * cols + col) = codes16(v[p], inv);
+      *reinterpret_cast<uint4*>(codes + row * cols + col) = codes16<T>(raw[p], inv, finite);
   }
   if (threadIdx.x == 0) scales[blockIdx.x] = exp2_int(k);
 }
@@ -209,10 +171,16 @@ cudaError_t quantize(const void* x, int64_t rows, int cols, int block_rows, uint
   const int cb = static_cast<int>(qblocks(cols));
   const T* p = static_cast<const T*>(x);
   if (block_rows == 1) {
-    const int64_t want = (rows * cb + 31) / 32;
-    const int grid = static_cast<int>(want < 8 * num_sms ? want : 8 * num_sms);
-    return launch_pdl(quantize_rows_kernel<T>, dim3(grid), dim3(256), 0, stream, p, rows, cols, cb,
-                      codes, scales);
+    // two blocks in flight once every lane group has some (16000 x 4096 bf16:
+    // 32.0 us, one 36.0, four 33.8); before that one (896 x 1024 takes 0.7 us less)
+    const int64_t want = (rows * cb + 31) / 32, most = 8 * num_sms;
+    const bool two = want >= 2 * most;
+    const dim3 grid(static_cast<unsigned>(want < most ? want : most));
+    auto* kernel = cols % kQBlock ? (two ? quantize_rows_kernel<T, false, 2>
+                                         : quantize_rows_kernel<T, false, 1>)
+                                  : (two ? quantize_rows_kernel<T, true, 2>
+                                         : quantize_rows_kernel<T, true, 1>);
+    return launch_pdl(kernel, grid, dim3(256), 0, stream, p, rows, cols, cb, codes, scales);
   }
   const int64_t blocks = qblocks(rows) * cb;
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;

@@ -8,8 +8,8 @@
 // over its 128 products, so the tensor cores sum one block (four K = 32 steps)
 // into a TMEM accumulator, and the epilogue warps read it, multiply by the two
 // scales' product (one number per row and 128 columns) and add to f32
-// registers; the accumulator is double buffered, so block b + 1 runs meanwhile.
-// The scales may be any f32 values.
+// registers; TMEM holds two to four accumulators, so the next blocks run
+// meanwhile.  The scales may be any f32 values.
 //
 // The weight is stored once, [out, in].  The forward product reads it with
 // the reduction contiguous (K-major B operand); the input's gradient reduces
@@ -33,14 +33,22 @@ constexpr int kBR = 128;  // reduction per stage: one scale block, one swizzle r
 constexpr uint32_t kABytes = kBM * kBR;
 constexpr int kThreads = 320;
 constexpr int kEpiWarp0 = 2;
-constexpr int kMaxStages = 6;
+constexpr int kMaxStages = 6, kMaxBufs = 4;
 constexpr uint32_t kSlabBytes = 32 * 128;  // per epilogue warp: 32 rows x 128 B
+
+// An epilogue warp's scales, kChunk blocks ahead: two buffers of 32 rows (an
+// odd pitch, for the banks) and the weight's.
+constexpr int kChunk = 8, kScalePitch = kChunk + 1;
+constexpr int kScaleBuf = 32 * kScalePitch + kChunk;
+constexpr int kScaleFloats = 2 * kScaleBuf;
 
 template <int kBN>
 struct Cfg {
-  static constexpr int kStages = kBN == 256 ? 4 : 6;
+  static constexpr int kStages = kBN == 256 ? 3 : 5;
+  static constexpr int kBufs = 512 / kBN;  // accumulators in TMEM
   static constexpr uint32_t kBBytes = kBN * kBR;
-  static constexpr size_t kSmem = 1024 + kStages * (kABytes + kBBytes) + 8 * kSlabBytes + 256;
+  static constexpr size_t kSmem =
+      1024 + kStages * (kABytes + kBBytes) + 8 * (kSlabBytes + 4 * kScaleFloats) + 256;
 };
 static_assert(Cfg<256>::kSmem <= 232448 && Cfg<128>::kSmem <= 232448,
               "shared memory budget");
@@ -48,8 +56,8 @@ static_assert(Cfg<256>::kSmem <= 232448 && Cfg<128>::kSmem <= 232448,
 struct Bars {
   uint64_t full[kMaxStages];
   uint64_t empty[kMaxStages];
-  uint64_t tfull[2];
-  uint64_t tempty[2];
+  uint64_t tfull[kMaxBufs];
+  uint64_t tempty[kMaxBufs];
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
@@ -69,6 +77,11 @@ __device__ __forceinline__ void umma_f8_ss(uint32_t tmem_d, uint64_t adesc, uint
 __host__ __device__ constexpr uint32_t idesc_e4m3_f32(int M, int N, int b_mn_major) {
   return (1u << 4) | (static_cast<uint32_t>(b_mn_major) << 16) |
          (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void copy4_async(float* dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src)
+               : "memory");
 }
 
 struct Args {
@@ -94,6 +107,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const __grid_constant__ CUtensorMap map_y, const Args a) {
   constexpr int kStages = Cfg<kBN>::kStages;
   constexpr uint32_t kBBytes = Cfg<kBN>::kBBytes;
+  constexpr int kBufs = Cfg<kBN>::kBufs;
   constexpr int kHalfN = kBN / 2;  // columns of one epilogue group
   constexpr int kSlabCols = 128 / static_cast<int>(sizeof(TO));
   extern __shared__ uint8_t smem_raw[];
@@ -102,8 +116,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sA = base;
   uint8_t* sB = sA + kStages * kABytes;
   uint8_t* sE = sB + kStages * kBBytes;
-  Bars* ss = reinterpret_cast<Bars*>(sE + 8 * kSlabBytes);
-  const int warp = warp_id(), lane = lane_id();
+  float* sS = reinterpret_cast<float*>(sE + 8 * kSlabBytes);
+  Bars* ss = reinterpret_cast<Bars*>(sS + 8 * kScaleFloats);
+  const int warp = static_cast<int>(uniform(threadIdx.x >> 5)), lane = lane_id();
   const int tiles_m = (a.M + kBM - 1) / kBM;
   const int tiles_n = (a.NO + kBN - 1) / kBN;
   const int num_tiles = tiles_m * tiles_n;
@@ -113,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&ss->full[s], 1);
       mbar_init(&ss->empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBufs; ++b) {
       mbar_init(&ss->tfull[b], 1);
       mbar_init(&ss->tempty[b], 8);
     }
@@ -130,55 +145,56 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ss->tmem_base;
+  const uint32_t tmem = uniform(ss->tmem_base);
   volatile int* abort_flag = &ss->abort;
   pdl_launch_dependents();
   pdl_wait();
 
   if (warp == 0) {
     // ---------------------------------------------------------- producer
-    if (lane == 0) {
-      uint32_t it = 0;
-      for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
-        const int m0 = t / tiles_n * kBM, n0 = t % tiles_n * kBN;
-        for (int b = 0; b < a.rb; ++b, ++it) {
-          const int s = it % kStages;
-          if (!mbar_wait(&ss->empty[s], ((it / kStages) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
-            *abort_flag = 1;
-            break;
-          }
+    uint32_t it = 0;
+    for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
+      const int m0 = t / tiles_n * kBM, n0 = t % tiles_n * kBN;
+      for (int b = 0; b < a.rb; ++b, ++it) {
+        const int s = it % kStages;
+        if (!warp_mbar_wait(&ss->empty[s], ((it / kStages) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
+          *abort_flag = 1;
+          break;
+        }
+        if (elect_one()) {
+          uint8_t *A = sA + s * kABytes, *B = sB + s * kBBytes;
           mbar_arrive_expect_tx(&ss->full[s], kABytes + kBBytes);
-          tma_load_2d(sA + s * kABytes, &map_x, &ss->full[s], b * kBR, m0);
-          uint8_t* B = sB + s * kBBytes;
+          tma_load_2d(A, &map_x, &ss->full[s], b * kBR, m0);
           if constexpr (!kTrans) {
             tma_load_2d(B, &map_w, &ss->full[s], b * kBR, n0);  // [n][128 r]
           } else {
-            // [r][min(128, kBN) n]: one box per 128 columns
+            // [r][128 n]: one box per 128 columns
 #pragma unroll
             for (int j = 0; j < kBN; j += 128)
               tma_load_2d(B + j * kBR, &map_w, &ss->full[s], n0 + j, b * kBR);
           }
         }
+        __syncwarp();
       }
-      // after an abort: the copies in flight land before the CTA goes
-      if (*abort_flag)
-        for (uint32_t j = it > static_cast<uint32_t>(kStages) ? it - kStages : 0; j < it; ++j)
-          mbar_wait(&ss->full[j % kStages], (j / kStages) & 1, nullptr, 0);
     }
+    // after an abort: the copies in flight land before the CTA goes
+    if (*abort_flag && lane == 0)
+      for (uint32_t j = it > static_cast<uint32_t>(kStages) ? it - kStages : 0; j < it; ++j)
+        mbar_wait(&ss->full[j % kStages], (j / kStages) & 1, nullptr, 0);
   } else if (warp == 1) {
     // -------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_e4m3_f32(kBM, kBN, kTrans ? 1 : 0);
-      uint32_t it = 0;
-      for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
-        for (int b = 0; b < a.rb; ++b, ++it) {
-          const int s = it % kStages, buf = it & 1;
-          if (!mbar_wait(&ss->tempty[buf], ((it >> 1) & 1) ^ 1, a.err, kDevTimeoutEpi) ||
-              !mbar_wait(&ss->full[s], (it / kStages) & 1, a.err, kDevTimeoutLoad)) {
-            *abort_flag = 1;
-            break;
-          }
-          tc_fence_after();
+    constexpr uint32_t idesc = idesc_e4m3_f32(kBM, kBN, kTrans ? 1 : 0);
+    uint32_t it = 0;
+    for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
+      for (int b = 0; b < a.rb; ++b, ++it) {
+        const int s = it % kStages, buf = it % kBufs;
+        if (!warp_mbar_wait(&ss->tempty[buf], ((it / kBufs) & 1) ^ 1, a.err, kDevTimeoutEpi) ||
+            !warp_mbar_wait(&ss->full[s], (it / kStages) & 1, a.err, kDevTimeoutLoad)) {
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        if (elect_one()) {
           const uint32_t a0 = smem_u32(sA + s * kABytes), b0 = smem_u32(sB + s * kBBytes);
 #pragma unroll
           for (int k = 0; k < kBR / 32; ++k) {
@@ -192,39 +208,69 @@ __global__ void __launch_bounds__(kThreads, 1)
           umma_commit(&ss->empty[s]);
           umma_commit(&ss->tfull[buf]);
         }
+        __syncwarp();
       }
-      if (*abort_flag) {
-        umma_commit(&ss->drain);
-        mbar_wait(&ss->drain, 0, nullptr, 0);
-      }
+    }
+    if (*abort_flag) {
+      if (elect_one()) umma_commit(&ss->drain);
+      __syncwarp();
+      mbar_wait(&ss->drain, 0, nullptr, 0);
     }
   } else {
     // ---------------------------------------------------------- epilogue
     const int quad = warp & 3, group = (warp - kEpiWarp0) >> 2;
     uint8_t* slab = sE + (warp - kEpiWarp0) * kSlabBytes;
     const int ncb = (a.NO + 127) / 128;
+    float* scales = sS + (warp - kEpiWarp0) * kScaleFloats;
+    // Blocks 8 c .. 8 c + 7 of tile t's scales, asked for while the eight
+    // before them are used.  (A load of each lane's own row per block, one block
+    // ahead, touches 32 sectors an instruction: 16000 x 1024 x 4096 took 77 us
+    // with it, 68 with these.)
+    auto prefetch = [&](int t, int c, int buf) {
+      const int nb = min((t % tiles_n * kBN + group * kHalfN) / 128, ncb - 1);
+      const int64_t b = c * kChunk + (lane & 7);
+      float* to = scales + buf * kScaleBuf;
+      if (b < a.rb) {
+        // a row's eight scales are one sector: four rows to an instruction
+        const int row0 = t / tiles_n * kBM + quad * 32 + (lane >> 3);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          copy4_async(to + (i + (lane >> 3)) * kScalePitch + (lane & 7),
+                      a.xs + static_cast<int64_t>(min(row0 + i, a.M - 1)) * a.rb + b);
+        if (lane < kChunk)
+          copy4_async(to + 32 * kScalePitch + lane,
+                      kTrans ? a.ws + b * ncb + nb : a.ws + static_cast<int64_t>(nb) * a.rb + b);
+      }
+    };
+    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+    const int chunks = (a.rb + kChunk - 1) / kChunk;
+    int sbuf = 0;
+    if (static_cast<int>(blockIdx.x) < num_tiles) prefetch(blockIdx.x, 0, 0);
+    commit();
     uint32_t it = 0;
     for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
       const int m0 = t / tiles_n * kBM, n0 = t % tiles_n * kBN + group * kHalfN;
       const int row = m0 + quad * 32 + lane;
-      const int nb = min(n0 / 128, ncb - 1);  // (a group past NO stores nothing)
-      const float* xsr = a.xs + static_cast<int64_t>(min(row, a.M - 1)) * a.rb;
-      const float* wsr = kTrans ? a.ws + nb : a.ws + static_cast<int64_t>(nb) * a.rb;
-      const int wstep = kTrans ? ncb : 1;
       float acc[kHalfN];
 #pragma unroll
       for (int e = 0; e < kHalfN; ++e) acc[e] = 0.f;
-      // the next block's scales are loaded a block ahead, multiplied at use
-      float xs_next = xsr[0], ws_next = wsr[0];
       bool ok = true;
       for (int b = 0; b < a.rb; ++b, ++it) {
-        const int buf = it & 1;
-        const float xs_now = xs_next, ws_now = ws_next;
-        if (b + 1 < a.rb) {
-          xs_next = xsr[b + 1];
-          ws_next = wsr[static_cast<int64_t>(b + 1) * wstep];
+        const int buf = it % kBufs;
+        if (b % kChunk == 0) {
+          const int c = b / kChunk;
+          if (b) sbuf ^= 1;
+          __syncwarp();  // the other buffer's readers are done
+          if (c + 1 < chunks) prefetch(t, c + 1, sbuf ^ 1);
+          else if (t + static_cast<int>(gridDim.x) < num_tiles) prefetch(t + gridDim.x, 0, sbuf ^ 1);
+          commit();
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+          __syncwarp();
         }
-        if (!mbar_wait(&ss->tfull[buf], (it >> 1) & 1, a.err, kDevTimeoutMma)) {
+        const float* sc = scales + sbuf * kScaleBuf;
+        const float s =
+            sc[lane * kScalePitch + b % kChunk] * sc[32 * kScalePitch + b % kChunk];
+        if (!mbar_wait(&ss->tfull[buf], (it / kBufs) & 1, a.err, kDevTimeoutMma)) {
           *abort_flag = 1;
           ok = false;
           break;
@@ -235,7 +281,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         // 16 columns are added up while the next 16 come from TMEM
         uint32_t r[2][16];
         tmem_ld16(taddr, r[0]);
-        const float s = xs_now * ws_now;
 #pragma unroll
         for (int c = 0; c < kHalfN; c += 16) {
           uint32_t(&cur)[16] = r[(c / 16) & 1];
@@ -254,6 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!ok) break;
+      sbuf ^= 1;  // the next tile's first scales
       const TO* bias = static_cast<const TO*>(a.bias);
       const bool bias_vec = (reinterpret_cast<uintptr_t>(bias) & 15) == 0;
       TO* y = static_cast<TO*>(a.y);
@@ -317,6 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (lane == 0) bulk_wait_all();
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();

@@ -118,25 +118,6 @@ __device__ __forceinline__ float4 cluster_sum4(uint32_t at, int ranks) {
   return s;
 }
 
-__device__ __forceinline__ float cluster_sum1(uint32_t at, int ranks) {
-  float v[8];
-#pragma unroll
-  for (int q = 0; q < 8; ++q)
-    if (q < ranks)
-      asm volatile(
-          "{\n\t.reg .b32 ra;\n\t"
-          "mapa.shared::cluster.u32 ra, %1, %2;\n\t"
-          "ld.shared::cluster.f32 %0, [ra];\n\t}\n"
-          : "=f"(v[q])
-          : "r"(at), "r"(q)
-          : "memory");
-  float s = v[0];
-#pragma unroll
-  for (int q = 1; q < 8; ++q)
-    if (q < ranks) s += v[q];
-  return s;
-}
-
 // Two bf16 (low half first) of two codes in bytes 0 and 1 (sel 0x1404 of the
 // word) or 2 and 3 (0x3424), times f.  A code's seven exponent and mantissa
 // bits, moved to bf16's places, read as value * 2^-120 (the biases are 7 and
@@ -168,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sR = sB + kStages * kBBytes;
   float* sBias = reinterpret_cast<float*>(sR + kStages * kRawBytes);  // [kTN]
   Bars* ss = reinterpret_cast<Bars*>(sBias + kTN);
-  const int warp = warp_id(), lane = lane_id();
+  const int warp = static_cast<int>(uniform(threadIdx.x >> 5)), lane = lane_id();
   const int tiles_k = (a.K + kTK - 1) / kTK;
   const int tile = static_cast<int>(blockIdx.x) / a.split;
   const int rank = static_cast<int>(blockIdx.x) % a.split;
@@ -199,60 +180,62 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ss->tmem_base;
+  const uint32_t tmem = uniform(ss->tmem_base);
   volatile int* abort_flag = &ss->abort;
   pdl_launch_dependents();
   pdl_wait();
 
   if (warp == 0) {
-    // ---------------------------------------------------------- producer
-    if (lane == 0) {
-      int i = 0;
-      for (; i < steps && !*abort_flag; ++i) {
-        const int s = i % kStages;
-        if (!mbar_wait_hot(&ss->empty[s], ((i / kStages) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
-          *abort_flag = 1;
-          break;
-        }
+    // ---------------------------------------------------- producer of dy
+    int i = 0;
+    for (; i < steps && !*abort_flag; ++i) {
+      const int s = i % kStages;
+      if (!warp_mbar_wait_hot(&ss->empty[s], ((i / kStages) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
+        *abort_flag = 1;
+        break;
+      }
+      if (elect_one()) {
         mbar_arrive_expect_tx(&ss->full[s], kBBytes);
 #pragma unroll
         for (int j = 0; j < kTN / 64; ++j)
           tma_load_2d(sB + s * kBBytes + j * kBlk, &map_dy, &ss->full[s], n0 + j * 64,
                       (st0 + i) * kTok);
       }
-      if (*abort_flag)  // the copies in flight land before the CTA goes
-        for (int j = i > kStages ? i - kStages : 0; j < i; ++j)
-          mbar_wait_hot(&ss->full[j % kStages], (j / kStages) & 1, nullptr, 0);
+      __syncwarp();
     }
+    if (*abort_flag && lane == 0)  // the copies in flight land before the CTA goes
+      for (int j = i > kStages ? i - kStages : 0; j < i; ++j)
+        mbar_wait(&ss->full[j % kStages], (j / kStages) & 1, nullptr, 0);
   } else if (warp == 2) {
-    // ------------------------------------------- producer of the codes
-    if (lane == 0) {
-      int i = 0;
-      for (; i < steps && !*abort_flag; ++i) {
-        const int s = i % kStages;
-        if (!mbar_wait_hot(&ss->rempty[s], ((i / kStages) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
-          *abort_flag = 1;
-          break;
-        }
+    // ------------------------------------------------- producer of the codes
+    int i = 0;
+    for (; i < steps && !*abort_flag; ++i) {
+      const int s = i % kStages;
+      if (!warp_mbar_wait_hot(&ss->rempty[s], ((i / kStages) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
+        *abort_flag = 1;
+        break;
+      }
+      if (elect_one()) {
         mbar_arrive_expect_tx(&ss->rfull[s], kRawBytes);
         tma_load_2d(sR + s * kRawBytes, &map_xq, &ss->rfull[s], k0, (st0 + i) * kTok);
       }
-      if (*abort_flag)
-        for (int j = i > kStages ? i - kStages : 0; j < i; ++j)
-          mbar_wait_hot(&ss->rfull[j % kStages], (j / kStages) & 1, nullptr, 0);
+      __syncwarp();
     }
+    if (*abort_flag && lane == 0)
+      for (int j = i > kStages ? i - kStages : 0; j < i; ++j)
+        mbar_wait(&ss->rfull[j % kStages], (j / kStages) & 1, nullptr, 0);
   } else if (warp == 1) {
     // -------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_bf16_f32(kTK, kTN, 1, 1);
-      for (int i = 0; i < steps; ++i) {
-        const int s = i % kStages;
-        if (*abort_flag || !mbar_wait_hot(&ss->full[s], (i / kStages) & 1, a.err, kDevTimeoutLoad) ||
-            !mbar_wait_hot(&ss->deq[s], (i / kStages) & 1, a.err, kDevTimeoutLoad)) {
-          *abort_flag = 1;
-          break;
-        }
-        tc_fence_after();
+    constexpr uint32_t idesc = idesc_bf16_f32(kTK, kTN, 1, 1);
+    for (int i = 0; i < steps; ++i) {
+      const int s = i % kStages;
+      if (*abort_flag || !warp_mbar_wait_hot(&ss->full[s], (i / kStages) & 1, a.err, kDevTimeoutLoad) ||
+          !warp_mbar_wait_hot(&ss->deq[s], (i / kStages) & 1, a.err, kDevTimeoutLoad)) {
+        *abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      if (elect_one()) {
         const uint32_t a0 = smem_u32(sA + s * kABytes), b0 = smem_u32(sB + s * kBBytes);
 #pragma unroll
         for (int k = 0; k < kTok / 16; ++k)
@@ -260,8 +243,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                   sdesc_sw128(b0 + k * 2048, kBlk, 1024), idesc, (i | k) != 0);
         umma_commit(&ss->empty[s]);
       }
-      umma_commit(&ss->done);
+      __syncwarp();
     }
+    if (elect_one()) umma_commit(&ss->done);
+    __syncwarp();
   } else if (warp >= kBiasWarp0 && warp < kDeqWarp0) {
     // ----------------------------------------------------------- bias sums
     // the tile's 8-column chunks kt, kt + tiles_k, ...: four to a round over

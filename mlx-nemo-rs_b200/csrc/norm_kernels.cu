@@ -244,28 +244,6 @@ __device__ __forceinline__ float warp_sums(const float (&v)[kN], int lane) {
   return a[0];
 }
 
-// The sum of one float at the same shared-memory offset over the cluster's
-// CTAs (at most 8), in rank order; all loads in flight together.
-__device__ __forceinline__ float cluster_column(const float* p, int ranks) {
-  const uint32_t at = smem_u32(p);
-  float v[8];
-#pragma unroll
-  for (int q = 0; q < 8; ++q)
-    if (q < ranks)
-      asm volatile(
-          "{\n\t.reg .b32 ra;\n\t"
-          "mapa.shared::cluster.u32 ra, %1, %2;\n\t"
-          "ld.shared::cluster.f32 %0, [ra];\n\t}\n"
-          : "=f"(v[q])
-          : "r"(at), "r"(q)
-          : "memory");
-  float s = v[0];
-#pragma unroll
-  for (int q = 1; q < 8; ++q)
-    if (q < ranks) s += v[q];
-  return s;
-}
-
 // A lane's eight elements of a row as they lie in memory, and as f32.
 template <typename T, bool kVec>
 struct Strip {
@@ -463,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
     cluster_sync();
     const int ranks = gridDim.x;
     for (int c = blockIdx.x * blockDim.x + threadIdx.x; c < 2 * cols; c += ranks * blockDim.x) {
-      const float s = cluster_column(col_sums + c, ranks);
+      const float s = cluster_sum1(smem_u32(col_sums + c), ranks);
       if (c < cols) dgamma[c] = s;
       else dbeta[c - cols] = s;
     }

@@ -115,6 +115,14 @@ __device__ __forceinline__ bool mbar_wait_hot(uint64_t* bar, uint32_t parity, in
   }
 }
 
+// Waits of a whole warp, whose lanes all see the same outcome.
+__device__ __forceinline__ bool warp_mbar_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+}
+__device__ __forceinline__ bool warp_mbar_wait_hot(uint64_t* bar, uint32_t parity, int* err, int code) {
+  return __all_sync(0xffffffffu, mbar_wait_hot(bar, parity, err, code));
+}
+
 // bytes (a multiple of 16, both addresses 16-byte aligned) from global to
 // this CTA's shared memory, completing on `bar` (an untiled bulk copy)
 __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes,
@@ -152,6 +160,27 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint64_t* bar, uint32_t rank
       "mbarrier.arrive.shared::cluster.b64 _, [ra];\n\t}\n" ::"r"(smem_u32(bar)),
       "r"(rank)
       : "memory");
+}
+
+// The sum of the float at one shared-memory offset over the cluster's first
+// `ranks` (at most 8) CTAs, in rank order; all loads in flight together.
+__device__ __forceinline__ float cluster_sum1(uint32_t at, int ranks) {
+  float v[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    if (q < ranks)
+      asm volatile(
+          "{\n\t.reg .b32 ra;\n\t"
+          "mapa.shared::cluster.u32 ra, %1, %2;\n\t"
+          "ld.shared::cluster.f32 %0, [ra];\n\t}\n"
+          : "=f"(v[q])
+          : "r"(at), "r"(q)
+          : "memory");
+  float s = v[0];
+#pragma unroll
+  for (int q = 1; q < 8; ++q)
+    if (q < ranks) s += v[q];
+  return s;
 }
 
 // ------------------------------------------------------------------ TMA
@@ -501,6 +530,25 @@ __device__ __forceinline__ float sigmoid_approx(float x) {
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// One lane of a converged warp, chosen by the hardware.  Code under
+// `if (elect_one())` in a warp that runs its loop as a whole can keep
+// descriptors and addresses in uniform registers, which tcgen05.mma, its commit
+// and the TMA copies read (four 8-bit MMAs and two commits: 400 cycles of the
+// issuing thread, 560 under `if (lane == 0)`).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p));
+  return p != 0;
+}
+// A value that all lanes hold, in a form the compiler knows to be uniform.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) {
+  return __shfl_sync(0xffffffffu, v, 0);
 }
 
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 31; }

@@ -10,7 +10,7 @@ const CUDA_SOURCES: &[&str] = &[
     "gemm_sm100.cu", "gemm_tf32.cu", "attn_sm100.cu", "attn_simt.cu", "attn_stream.cu",
     "kernels_misc.cu",
     "noalloc.cu", "block_kernels.cu", "subsampling_kernels.cu",
-    "fp8_quant.cu", "gemm_fp8.cu", "gemm_fp8_wgrad.cu", "norm_kernels.cu",
+    "fp8_quant.cu", "gemm_fp8.cu", "gemm_fp8_small.cu", "gemm_fp8_wgrad.cu", "norm_kernels.cu",
 ];
 const CPP_SOURCES: &[&str] = &["api.cpp", "halo.cpp", "block.cpp", "subsampling.cpp", "fp8_api.cpp"];
 
