@@ -10,11 +10,8 @@
 // backward pass takes x as it was or as the e4m3 checkpoint (codes and one
 // scale per 128 columns), with the saved mean and rstd of the exact row.
 //
-// Bound by HBM.  Forward, up to 2048 columns: a warp holds a row in registers,
-// 8 consecutive elements per lane and 256-column chunk (16-byte loads), or
-// one element per lane and 32-column chunk where the columns or pointers do
-// not allow those.  Backward: strips of 256 columns, see there; the sums over
-// rows are added up in registers, over the CTA's groups in shared memory, and
+// Bound by HBM.  Up to 2048 columns, both passes take strips of 256 columns.  The
+// backward's sums over rows are added up in registers, over the CTA's groups in shared memory, and
 // over CTAs through distributed shared memory (few rows: one cluster) or a
 // second kernel over partial rows in the caller's workspace: fixed order, no
 // atomics.  Wider rows take a CTA each and read their inputs again from L1/L2.
@@ -103,147 +100,6 @@ __device__ __forceinline__ void store_v(__nv_bfloat16* p, const float* v) {
     *p = __float2bfloat16_rn(v[0]);
 }
 
-// ------------------------------------------------------------- forward
-// One warp per row of at most kCh * 32 * kV columns.
-template <typename T, int kV, int kCh>
-__global__ void __launch_bounds__(256)
-    norm_fwd_kernel(const T* x, int64_t rows, int cols, const float* __restrict__ gamma,
-                    const float* __restrict__ beta, float eps, T* y, float* __restrict__ mean_out,
-                    float* __restrict__ rstd_out) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  pdl_launch_dependents();
-  if (row >= rows) return;
-  pdl_wait();
-  const T* xr = x + row * cols;
-  float v[kCh][kV];
-  float s = 0.f;
-#pragma unroll
-  for (int c = 0; c < kCh; ++c) {
-    const int col = (c * 32 + lane) * kV;
-    if (col < cols) {
-      load_v<kV>(xr + col, v[c]);
-#pragma unroll
-      for (int e = 0; e < kV; ++e) s += v[c][e];
-    }
-  }
-  const float mean = warp_sum(s) / static_cast<float>(cols);
-  float q = 0.f;
-#pragma unroll
-  for (int c = 0; c < kCh; ++c)
-    if ((c * 32 + lane) * kV < cols) {
-#pragma unroll
-      for (int e = 0; e < kV; ++e) {
-        v[c][e] -= mean;
-        q = fmaf(v[c][e], v[c][e], q);
-      }
-    }
-  const float rstd = 1.f / sqrtf(warp_sum(q) / static_cast<float>(cols) + eps);
-  T* yr = y + row * cols;
-#pragma unroll
-  for (int c = 0; c < kCh; ++c) {
-    const int col = (c * 32 + lane) * kV;
-    if (col < cols) {
-      float g[kV], b[kV], o[kV];
-      load_v<kV>(gamma + col, g);
-      load_v<kV>(beta + col, b);
-#pragma unroll
-      for (int e = 0; e < kV; ++e) o[e] = fmaf(v[c][e] * rstd, g[e], b[e]);
-      store_v<kV>(yr + col, o);
-    }
-  }
-  if (lane == 0 && mean_out) {
-    mean_out[row] = mean;
-    rstd_out[row] = rstd;
-  }
-}
-
-// Sum of one value per thread over the CTA's 8 warps, to every thread.
-__device__ __forceinline__ float block_sum(float v, float* part) {
-  v = warp_sum(v);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) s += part[w];
-  __syncthreads();
-  return s;
-}
-
-// Any width: one CTA per row, x read three times.
-template <typename T>
-__global__ void __launch_bounds__(256)
-    norm_fwd_wide_kernel(const T* x, int64_t rows, int cols, const float* __restrict__ gamma,
-                         const float* __restrict__ beta, float eps, T* y,
-                         float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-  __shared__ float part[8];
-  pdl_launch_dependents();
-  pdl_wait();
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const T* xr = x + row * cols;
-    float s = 0.f;
-    for (int c = threadIdx.x; c < cols; c += 256) s += get(xr + c);
-    const float mean = block_sum(s, part) / static_cast<float>(cols);
-    float q = 0.f;
-    for (int c = threadIdx.x; c < cols; c += 256) {
-      const float d = get(xr + c) - mean;
-      q = fmaf(d, d, q);
-    }
-    const float rstd = 1.f / sqrtf(block_sum(q, part) / static_cast<float>(cols) + eps);
-    for (int c = threadIdx.x; c < cols; c += 256)
-      put(y + row * cols + c, fmaf((get(xr + c) - mean) * rstd, gamma[c], beta[c]));
-    if (threadIdx.x == 0 && mean_out) {
-      mean_out[row] = mean;
-      rstd_out[row] = rstd;
-    }
-  }
-}
-
-// ------------------------------------------------------------ backward
-// A group of W = ceil(cols / 256) warps takes kRows rows at a time, each warp
-// a strip of 256 columns, a lane eight of them (consecutive, 16-byte loads,
-// or 32 apart where the columns or pointers do not allow those).  dgamma and
-// dbeta then cost a lane 16 registers whatever the width, and a warp has
-// kRows rows' loads in flight.  The rows' two sums cross the warps of a group
-// through shared memory (double buffered: one barrier per batch of rows).
-constexpr int kRows = 4;
-constexpr int kStripWarps = 8;         // W at most: 2048 columns
-constexpr int kStripCols = 256 * kStripWarps;
-constexpr int kFewRows = 1024;         // up to here one cluster takes all rows
-constexpr int kFewThreads = 512;       // threads of its CTAs
-constexpr int kManyThreads = 256;
-constexpr int kManyParts = 2 * 148;    // CTAs of the persistent grid at most
-
-int strip_warps(int cols) { return (cols + 255) / 256; }
-int strip_groups(int cols, int threads) { return std::max(1, threads / 32 / strip_warps(cols)); }
-
-// Partial rows of dgamma | dbeta that go through the workspace (0: none).
-int norm_parts(int64_t rows, int cols) {
-  if (cols > kStripCols) return static_cast<int>(std::min<int64_t>((rows + 7) / 8, 296));
-  if (rows <= kFewRows) return 0;
-  const int per = strip_groups(cols, kManyThreads) * kRows;
-  return static_cast<int>(std::min<int64_t>((rows + per - 1) / per, kManyParts));
-}
-
-// The sums over the warp of kN = 4 or 8 values per lane, halving the values
-// and the lanes that hold each: lane l ends with the sum of value l / (32 / kN).
-template <int kN>
-__device__ __forceinline__ float warp_sums(const float (&v)[kN], int lane) {
-  float a[kN];
-#pragma unroll
-  for (int i = 0; i < kN; ++i) a[i] = v[i];
-#pragma unroll
-  for (int n = kN / 2, o = 16; n >= 1; n /= 2, o /= 2)
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const bool hi = lane & o;
-      a[i] = (hi ? a[i + n] : a[i]) + __shfl_xor_sync(0xffffffffu, hi ? a[i] : a[i + n], o);
-    }
-#pragma unroll
-  for (int o = 16 / kN; o >= 1; o /= 2) a[0] += __shfl_xor_sync(0xffffffffu, a[0], o);
-  return a[0];
-}
-
 // A lane's eight elements of a row as they lie in memory, and as f32.
 template <typename T, bool kVec>
 struct Strip {
@@ -305,6 +161,325 @@ __device__ __forceinline__ void store_strip(T* p, int col, int cols, const float
   }
 }
 
+// Packed pairs of f32 (one instruction for two elements).
+struct F2 {
+  float a, b;
+};
+__device__ __forceinline__ F2 mul2(F2 x, F2 y) {
+  F2 r;
+  asm("{\n .reg .b64 rx, ry;\n mov.b64 rx, {%2, %3};\n mov.b64 ry, {%4, %5};\n"
+      " mul.rn.f32x2 rx, rx, ry;\n mov.b64 {%0, %1}, rx;\n}"
+      : "=f"(r.a), "=f"(r.b)
+      : "f"(x.a), "f"(x.b), "f"(y.a), "f"(y.b));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 x, F2 y) {
+  F2 r;
+  add_f32x2(r.a, r.b, x.a, x.b, y.a, y.b);
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 x, F2 y, F2 z) {
+  F2 r;
+  asm("{\n .reg .b64 rx, ry, rz;\n mov.b64 rx, {%2, %3};\n mov.b64 ry, {%4, %5};\n"
+      " mov.b64 rz, {%6, %7};\n fma.rn.f32x2 rx, rx, ry, rz;\n mov.b64 {%0, %1}, rx;\n}"
+      : "=f"(r.a), "=f"(r.b)
+      : "f"(x.a), "f"(x.b), "f"(y.a), "f"(y.b), "f"(z.a), "f"(z.b));
+  return r;
+}
+__device__ __forceinline__ F2 both(float v) { return {v, v}; }
+
+// ------------------------------------------------------------- forward
+// A group of W = ceil(cols / 256) warps takes kR rows at a time, each warp a
+// strip of 256 columns, a lane eight of them, with the next rows' loads in
+// flight.  gamma and beta then stay in 16 registers of a lane: a
+// warp that takes whole rows reads 8 bytes of them from L1 for every element
+// (50000 x 1024 bf16: 44 us at best).  A strip's mean and sum of squares about
+// it are joined through shared memory, one barrier per batch (double
+// buffered): with n_w columns each,
+//   mean = sum n_w mean_w / C,  M2 = sum M2_w + n_w (mean_w - mean)^2.
+constexpr int kStripWarps = 8;  // W at most: 2048 columns
+constexpr int kStripCols = 256 * kStripWarps;
+int strip_warps(int cols) { return (cols + 255) / 256; }
+int strip_groups(int cols, int threads) { return std::max(1, threads / 32 / strip_warps(cols)); }
+
+// W rounded up to a power of two (lanes of a row when the strips are joined).
+__device__ __forceinline__ int strips_pow2(int W) { return W <= 1 ? 1 : 1 << (32 - __clz(W - 1)); }
+
+// The sums over the warp of kN = 2, 4 or 8 values per lane, halving the values
+// and the lanes that hold each: lane l ends with the sum of value l / (32 / kN).
+template <int kN>
+__device__ __forceinline__ float warp_sums(const float (&v)[kN], int lane) {
+  float a[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) a[i] = v[i];
+#pragma unroll
+  for (int n = kN / 2, o = 16; n >= 1; n /= 2, o /= 2)
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const bool hi = lane & o;
+      a[i] = (hi ? a[i + n] : a[i]) + __shfl_xor_sync(0xffffffffu, hi ? a[i] : a[i + n], o);
+    }
+#pragma unroll
+  for (int o = 16 / kN; o >= 1; o /= 2) a[0] += __shfl_xor_sync(0xffffffffu, a[0], o);
+  return a[0];
+}
+
+constexpr int kFwdThreads = 256;
+// CTAs per SM of a kernel that takes kR rows at a time (kR kStripWarps <= 32).
+template <int kR>
+constexpr int kFwdCtas = kR == 4 ? 2 : 3;
+
+template <typename T, int kR>
+__global__ void __launch_bounds__(kFwdThreads, kFwdCtas<kR>)
+    norm_fwd_kernel(const T* x, int64_t rows, int cols, int W, const float* __restrict__ gamma,
+                    const float* __restrict__ beta, float eps, T* y, float* __restrict__ mean_out,
+                    float* __restrict__ rstd_out) {
+  __shared__ float2 red[2][kFwdThreads / 32][kR];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int strip = warp % W, grp = warp / W, groups = static_cast<int>(blockDim.x) / 32 / W;
+  const int col = strip * 256 + lane * 8;
+  pdl_launch_dependents();
+  pdl_wait();
+  const float inv_n = 1.f / static_cast<float>(min(256, cols - strip * 256));
+  const int Wp = strips_pow2(W), at_w = lane % Wp, at_r = lane / Wp;
+  const float at_n = at_w < W ? static_cast<float>(min(256, cols - at_w * 256)) : 0.f;
+  const float inv_c = 1.f / static_cast<float>(cols);
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * groups * kR;
+  int64_t row0 = (static_cast<int64_t>(blockIdx.x) * groups + grp) * kR;
+  Strip<T, true> next[kR];
+  auto load = [&](int64_t r0) {
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      if (r0 + r < rows) next[r].load(x + (r0 + r) * cols, col, cols);
+      else next[r].zero();
+    }
+  };
+  load(row0);
+  const bool in = col < cols;  // (cols % 8 == 0: all of the lane's columns or none)
+  F2 gm[4], bt[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    gm[e] = in ? F2{gamma[col + 2 * e], gamma[col + 2 * e + 1]} : both(0.f);
+    bt[e] = in ? F2{beta[col + 2 * e], beta[col + 2 * e + 1]} : both(0.f);
+  }
+  int buf = 0;
+  for (; row0 < rows; row0 += stride, buf ^= 1) {
+    F2 v[kR][4];
+    float part[kR];
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      F2 s = both(0.f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[r][e] = {next[r].get(2 * e), next[r].get(2 * e + 1)};
+        s = add2(s, v[r][e]);  // columns past the end are zeros
+      }
+      part[r] = s.a + s.b;
+    }
+    // (y may be x: these rows are in registers, and the next are others)
+    load(row0 + stride);
+    constexpr int kHold = 32 / kR;  // lanes that hold each sum
+    // lane l: the strip's mean of row l / kHold, then its sum of squares
+    const float mean_w = warp_sums(part, lane) * inv_n;
+    float mean[kR], rstd[kR];
+#pragma unroll
+    for (int r = 0; r < kR; ++r) mean[r] = __shfl_sync(0xffffffffu, mean_w, kHold * r);
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      F2 q = both(0.f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const F2 d = add2(v[r][e], both(-mean[r]));
+        q = fma2(d, d, q);
+      }
+      part[r] = in ? q.a + q.b : 0.f;  // (the others hold -mean)
+    }
+    const float m2_w = warp_sums(part, lane);
+    if (W == 1) {
+      const float rs = 1.f / sqrtf(m2_w * inv_c + eps);
+#pragma unroll
+      for (int r = 0; r < kR; ++r) rstd[r] = __shfl_sync(0xffffffffu, rs, kHold * r);
+    } else {
+      if (lane % kHold == 0) red[buf][warp][lane / kHold] = make_float2(mean_w, m2_w);
+      named_bar_sync(1 + grp, 32 * W);
+      // lane (r, w) takes strip w's share of row r
+      const bool mine = at_w < W && at_r < kR;
+      const float2 p = mine ? red[buf][grp * W + at_w][at_r] : make_float2(0.f, 0.f);
+      float m = p.x * at_n * inv_c;
+      for (int o = Wp / 2; o; o /= 2) m += __shfl_xor_sync(0xffffffffu, m, o);
+      const float d = p.x - m;
+      float t = fmaf(d * d, at_n, p.y);
+      for (int o = Wp / 2; o; o /= 2) t += __shfl_xor_sync(0xffffffffu, t, o);
+      const float rs = 1.f / sqrtf(t * inv_c + eps);
+#pragma unroll
+      for (int r = 0; r < kR; ++r) {
+        mean[r] = __shfl_sync(0xffffffffu, m, Wp * r);
+        rstd[r] = __shfl_sync(0xffffffffu, rs, Wp * r);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      if (row0 + r >= rows) break;
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const F2 u = mul2(add2(v[r][e], both(-mean[r])), both(rstd[r]));
+        const F2 f = fma2(u, gm[e], bt[e]);
+        o[2 * e] = f.a;
+        o[2 * e + 1] = f.b;
+      }
+      store_strip<T, true>(y + (row0 + r) * cols, col, cols, o);
+      if (mean_out && strip == 0 && lane == 0) {
+        mean_out[row0 + r] = mean[r];
+        rstd_out[row0 + r] = rstd[r];
+      }
+    }
+  }
+}
+
+// Columns or pointers that do not allow 16-byte loads: a warp's whole row, of at
+// most kCh strips, a lane's elements 32 apart.
+constexpr int kRowThreads = 128;
+template <typename T, int kCh>
+__global__ void __launch_bounds__(kRowThreads)
+    norm_fwd_rows_kernel(const T* x, int64_t rows, int cols, const float* __restrict__ gamma,
+                         const float* __restrict__ beta, float eps, T* y,
+                         float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row =
+      static_cast<int64_t>(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5);
+  pdl_launch_dependents();
+  if (row >= rows) return;
+  pdl_wait();
+  const float inv_c = 1.f / static_cast<float>(cols);
+  // column of the lane's element e of strip c
+  auto col_of = [&](int c, int e) { return c * 256 + lane + 32 * e; };
+  Strip<T, false> v[kCh];
+#pragma unroll
+  for (int c = 0; c < kCh; ++c) v[c].load(x + row * cols, col_of(c, 0), cols);
+  float s = 0.f;
+#pragma unroll
+  for (int c = 0; c < kCh; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += v[c].get(e);  // columns past the end are zeros
+  const float mean = warp_sum(s) * inv_c;
+  float q = 0.f;
+#pragma unroll
+  for (int c = 0; c < kCh; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float d = v[c].get(e) - mean;
+      if (col_of(c, e) < cols) q = fmaf(d, d, q);
+    }
+  const float rstd = 1.f / sqrtf(warp_sum(q) * inv_c + eps);
+#pragma unroll
+  for (int c = 0; c < kCh; ++c) {
+    float o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = col_of(c, e);
+      o[e] = i < cols ? fmaf((v[c].get(e) - mean) * rstd, gamma[i], beta[i]) : 0.f;
+    }
+    store_strip<T, false>(y + row * cols, col_of(c, 0), cols, o);
+  }
+  if (lane == 0 && mean_out) {
+    mean_out[row] = mean;
+    rstd_out[row] = rstd;
+  }
+}
+
+// Sum of one value per thread over the CTA's 8 warps, to every thread.
+__device__ __forceinline__ float block_sum(float v, float* part) {
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) s += part[w];
+  __syncthreads();
+  return s;
+}
+
+// Any width: one CTA per row, x read three times.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    norm_fwd_wide_kernel(const T* x, int64_t rows, int cols, const float* __restrict__ gamma,
+                         const float* __restrict__ beta, float eps, T* y,
+                         float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+  __shared__ float part[8];
+  pdl_launch_dependents();
+  pdl_wait();
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T* xr = x + row * cols;
+    float s = 0.f;
+    for (int c = threadIdx.x; c < cols; c += 256) s += get(xr + c);
+    const float mean = block_sum(s, part) / static_cast<float>(cols);
+    float q = 0.f;
+    for (int c = threadIdx.x; c < cols; c += 256) {
+      const float d = get(xr + c) - mean;
+      q = fmaf(d, d, q);
+    }
+    const float rstd = 1.f / sqrtf(block_sum(q, part) / static_cast<float>(cols) + eps);
+    for (int c = threadIdx.x; c < cols; c += 256)
+      put(y + row * cols + c, fmaf((get(xr + c) - mean) * rstd, gamma[c], beta[c]));
+    if (threadIdx.x == 0 && mean_out) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+  }
+}
+
+// ------------------------------------------------------------ backward
+// Groups of W warps and strips of columns as in the forward pass: dgamma and
+// dbeta cost a lane 16 registers whatever the width.  The rows' two sums cross
+// the warps of a group through shared memory.
+constexpr int kRows = 2;  // 2 kRows kStripWarps <= 32 lanes
+constexpr int kFewRows = 256;          // up to here one cluster takes all rows
+constexpr int kFewThreads = 512;       // threads of its CTAs
+constexpr int kManyThreads = 256;
+constexpr int kManyParts = 2 * 148;    // CTAs of the persistent grid at most
+
+// Partial rows of dgamma | dbeta that go through the workspace (0: none).
+int norm_parts(int64_t rows, int cols) {
+  if (cols > kStripCols) return static_cast<int>(std::min<int64_t>((rows + 7) / 8, 296));
+  if (rows <= kFewRows) return 0;
+  const int per = strip_groups(cols, kManyThreads) * kRows;
+  return static_cast<int>(std::min<int64_t>((rows + per - 1) / per, kManyParts));
+}
+
+// kRows rows of a lane's strip on their way.
+template <typename T, typename TX, bool kVec>
+struct Batch {
+  static constexpr int kScales = sizeof(TX) == 1 ? (kVec ? 1 : 2) : 0;
+  Strip<TX, kVec> x[kRows];
+  Strip<T, kVec> dy[kRows];
+  float mu[kRows], rs[kRows], sx[kRows][kScales ? kScales : 1];
+  __device__ __forceinline__ void load(const TX* px, const float* xs, const T* pdy,
+                                       const float* mean, const float* rstd, int64_t row0,
+                                       int64_t rows, int cols, int cb, int col) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const int64_t row = row0 + r;
+      mu[r] = rs[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kScales; ++i) sx[r][i] = 0.f;
+      if (row < rows) {
+        x[r].load(px + row * cols, col, cols);
+        dy[r].load(pdy + row * cols, col, cols);
+        mu[r] = mean[row];
+        rs[r] = rstd[row];
+        // a lane's columns lie in one block (kVec), or in two
+#pragma unroll
+        for (int i = 0; i < kScales; ++i)
+          if (col + 128 * i < cols) sx[r][i] = xs[row * cb + (col >> 7) + i];
+      } else {
+        x[r].zero();
+        dy[r].zero();
+      }
+    }
+  }
+};
+
 // blockDim.x = 32 * W * groups.  partials [gridDim.x][2][cols], or null: the
 // grid is one cluster, and dgamma and dbeta (null: not wanted) are written.
 template <typename T, typename TX, bool kVec, int kThreads>
@@ -316,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
                     float* __restrict__ dgamma, float* __restrict__ dbeta) {
   constexpr bool kCodes = sizeof(TX) == 1;
   extern __shared__ float col_sums[];  // [groups][2][cols]
-  __shared__ __align__(16) float red[2][kThreads / 32][2 * kRows];
+  __shared__ float red[2][kThreads / 32][2 * kRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int strip = warp % W, grp = warp / W, groups = static_cast<int>(blockDim.x) / 32 / W;
   const int col = strip * 256 + (kVec ? lane * 8 : lane);
@@ -324,106 +499,87 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
   pdl_wait();
   const int cb = (cols + kQBlock - 1) / kQBlock;
   const float inv_c = 1.f / static_cast<float>(cols);
-  float ag[8], ab[8], gm[8];
+  const int Wp = strips_pow2(W), at_w = lane % Wp, at_i = lane / Wp;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * groups * kRows;
+  int64_t row0 = (static_cast<int64_t>(blockIdx.x) * groups + grp) * kRows;
+  Batch<T, TX, kVec> next;
+  next.load(x, xs, dy, mean, rstd, row0, rows, cols, cb, col);
+  F2 ag[4], ab[4], gm[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    ag[e] = ab[e] = 0.f;
-    const int c = col + (kVec ? e : 32 * e);
-    gm[e] = c < cols ? gamma[c] : 0.f;
+  for (int e = 0; e < 4; ++e) {
+    ag[e] = ab[e] = both(0.f);
+    const int c0 = col + (kVec ? 2 * e : 64 * e), c1 = c0 + (kVec ? 1 : 32);
+    gm[e] = {c0 < cols ? gamma[c0] : 0.f, c1 < cols ? gamma[c1] : 0.f};
   }
   int buf = 0;
-  for (int64_t row0 = (static_cast<int64_t>(blockIdx.x) * groups + grp) * kRows; row0 < rows;
-       row0 += static_cast<int64_t>(gridDim.x) * groups * kRows, buf ^= 1) {
-    Strip<TX, kVec> rx[kRows];
-    Strip<T, kVec> ry[kRows];
-    float mu[kRows], rs[kRows], sx[kRows][kCodes && !kVec ? 2 : 1];
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const int64_t row = row0 + r;
-      mu[r] = rs[r] = sx[r][0] = 0.f;
-      if (kCodes && !kVec) sx[r][kCodes && !kVec ? 1 : 0] = 0.f;
-      if (row < rows) {
-        rx[r].load(x + row * cols, col, cols);
-        ry[r].load(dy + row * cols, col, cols);
-        mu[r] = mean[row];
-        rs[r] = rstd[row];
-        if (kCodes) {
-          // a lane's columns lie in one block (kVec), or in two
-          if (col < cols) sx[r][0] = xs[row * cb + (col >> 7)];
-          if (!kVec && col + 128 < cols) sx[r][kVec ? 0 : 1] = xs[row * cb + (col >> 7) + 1];
-        }
-      } else {
-        rx[r].zero();
-        ry[r].zero();
-      }
-    }
-    auto u_of = [&](int r, int e) {
-      const float v = rx[r].get(e);
-      return (kCodes ? fmaf(v, sx[r][kVec ? 0 : e >> 2], -mu[r]) : v - mu[r]) * rs[r];
-    };
+  for (; row0 < rows; row0 += stride, buf ^= 1) {
+    const Batch<T, TX, kVec> now = next;
+    next.load(x, xs, dy, mean, rstd, row0 + stride, rows, cols, cb, col);
+    F2 u[kRows][4], g[kRows][4];
     float part[2 * kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      float c1 = 0.f, c2 = 0.f;
+      F2 c1 = both(0.f), c2 = both(0.f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float u = u_of(r, e), d = ry[r].get(e), g = d * gm[e];
-        ag[e] = fmaf(d, u, ag[e]);
-        ab[e] += d;
-        c1 += g;
-        c2 = fmaf(g, u, c2);
+      for (int e = 0; e < 4; ++e) {
+        const F2 xv = {now.x[r].get(2 * e), now.x[r].get(2 * e + 1)};
+        const F2 d = {now.dy[r].get(2 * e), now.dy[r].get(2 * e + 1)};
+        if constexpr (kCodes) {
+          // (code * scale - mean) * rstd with the constants multiplied first: a
+          // mean so large that its rounding shows here leaves eight bits nothing
+          const float k = now.sx[r][kVec ? 0 : e >> 1] * now.rs[r];
+          u[r][e] = fma2(xv, both(k), both(-now.mu[r] * now.rs[r]));
+        } else {
+          u[r][e] = mul2(add2(xv, both(-now.mu[r])), both(now.rs[r]));
+        }
+        ag[e] = fma2(d, u[r][e], ag[e]);
+        ab[e] = add2(ab[e], d);
+        g[r][e] = mul2(d, gm[e]);
+        c1 = add2(c1, g[r][e]);
+        c2 = fma2(g[r][e], u[r][e], c2);
       }
-      part[r] = c1;
-      part[kRows + r] = c2;
+      part[r] = c1.a + c1.b;
+      part[kRows + r] = c2.a + c2.b;
     }
     // lanes past the columns hold x = 0 and dy = 0: nothing but zeros added
     const float mine = warp_sums(part, lane);
     constexpr int kHold = 16 / kRows;  // lanes that hold each sum
-    float c1[kRows], c2[kRows];
+    float s[2 * kRows];
     if (W == 1) {
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        c1[r] = __shfl_sync(0xffffffffu, mine, kHold * r) * inv_c;
-        c2[r] = __shfl_sync(0xffffffffu, mine, kHold * (kRows + r)) * inv_c;
-      }
+      for (int i = 0; i < 2 * kRows; ++i) s[i] = __shfl_sync(0xffffffffu, mine, kHold * i);
     } else {
       if (lane % kHold == 0) red[buf][warp][lane / kHold] = mine;
       named_bar_sync(1 + grp, 32 * W);
-      float s[2 * kRows];
+      // lane (i, w) takes strip w's share of sum i
+      float t = at_w < W && at_i < 2 * kRows ? red[buf][grp * W + at_w][at_i] : 0.f;
+      for (int o = Wp / 2; o; o /= 2) t += __shfl_xor_sync(0xffffffffu, t, o);
 #pragma unroll
-      for (int i = 0; i < 2 * kRows; ++i) s[i] = 0.f;
-      for (int w = 0; w < W; ++w) {
-        const float4* q = reinterpret_cast<const float4*>(red[buf][grp * W + w]);
-#pragma unroll
-        for (int i = 0; i < kRows / 2; ++i) {
-          const float4 v = q[i];
-          s[4 * i] += v.x, s[4 * i + 1] += v.y, s[4 * i + 2] += v.z, s[4 * i + 3] += v.w;
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        c1[r] = s[r] * inv_c;
-        c2[r] = s[kRows + r] * inv_c;
-      }
+      for (int i = 0; i < 2 * kRows; ++i) s[i] = __shfl_sync(0xffffffffu, t, Wp * i);
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       if (row0 + r >= rows) break;
+      // dx = rstd g - rstd mean(g) - u rstd mean(g u)
+      const float rs = now.rs[r];
+      const F2 k0 = both(-rs * (s[r] * inv_c)), k2 = both(-rs * (s[kRows + r] * inv_c));
       float o[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        o[e] = rs[r] * (ry[r].get(e) * gm[e] - c1[r] - u_of(r, e) * c2[r]);
+      for (int e = 0; e < 4; ++e) {
+        const F2 v = fma2(u[r][e], k2, fma2(g[r][e], both(rs), k0));
+        o[2 * e] = v.a;
+        o[2 * e + 1] = v.b;
+      }
       store_strip<T, kVec>(dx + (row0 + r) * cols, col, cols, o);
     }
   }
   if (!partials && !dgamma) return;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int c = col + (kVec ? e : 32 * e);
-    if (c < cols) {
-      col_sums[2 * grp * cols + c] = ag[e];
-      col_sums[(2 * grp + 1) * cols + c] = ab[e];
-    }
+  for (int e = 0; e < 4; ++e) {
+    const int c0 = col + (kVec ? 2 * e : 64 * e), c1 = c0 + (kVec ? 1 : 32);
+    float* to = col_sums + 2 * grp * cols;
+    if (c0 < cols) to[c0] = ag[e].a, to[cols + c0] = ab[e].a;
+    if (c1 < cols) to[c1] = ag[e].b, to[cols + c1] = ab[e].b;
   }
   __syncthreads();
   if (groups > 1) {
@@ -554,24 +710,37 @@ struct FwdArgs {
   float *mean, *rstd;
 };
 
-template <typename T, int kV, int kCh>
+template <typename T, int kR>
+cudaError_t fwd_strips(const T* x, T* y, const FwdArgs& a, int num_sms, cudaStream_t stream) {
+  const int W = strip_warps(a.cols), groups = strip_groups(a.cols, kFwdThreads);
+  const int per = groups * kR;
+  const int64_t grid = std::min<int64_t>((a.rows + per - 1) / per, kFwdCtas<kR> * num_sms);
+  return launch_pdl(norm_fwd_kernel<T, kR>, dim3(static_cast<unsigned>(grid)),
+                    dim3(32 * W * groups), 0, stream, x, a.rows, a.cols, W, a.gamma, a.beta, a.eps,
+                    y, a.mean, a.rstd);
+}
+
+template <typename T, int kCh>
 cudaError_t fwd_rows(const T* x, T* y, const FwdArgs& a, cudaStream_t stream) {
-  const int64_t grid = (a.rows + 7) / 8;
+  const int64_t grid = (a.rows + kRowThreads / 32 - 1) / (kRowThreads / 32);
   if (grid > 0x7fffffff) return cudaErrorInvalidValue;
-  return launch_pdl(norm_fwd_kernel<T, kV, kCh>, dim3(static_cast<unsigned>(grid)), dim3(256), 0,
-                    stream, x, a.rows, a.cols, a.gamma, a.beta, a.eps, y, a.mean, a.rstd);
+  return launch_pdl(norm_fwd_rows_kernel<T, kCh>, dim3(static_cast<unsigned>(grid)),
+                    dim3(kRowThreads), 0, stream, x, a.rows, a.cols, a.gamma, a.beta, a.eps, y,
+                    a.mean, a.rstd);
 }
 
 template <typename T>
 cudaError_t fwd(const T* x, T* y, const FwdArgs& a, int num_sms, cudaStream_t stream) {
-  const bool vec = a.cols % 8 == 0 && aligned16(x) && aligned16(y) && aligned16(a.gamma) &&
-                   aligned16(a.beta);
-  if (vec && a.cols <= 256) return fwd_rows<T, 8, 1>(x, y, a, stream);
-  if (vec && a.cols <= 512) return fwd_rows<T, 8, 2>(x, y, a, stream);
-  if (vec && a.cols <= 1024) return fwd_rows<T, 8, 4>(x, y, a, stream);
-  if (vec && a.cols <= 2048) return fwd_rows<T, 8, 8>(x, y, a, stream);
-  if (!vec && a.cols <= 256) return fwd_rows<T, 1, 8>(x, y, a, stream);
-  if (!vec && a.cols <= 1024) return fwd_rows<T, 1, 32>(x, y, a, stream);
+  const bool vec = a.cols % 8 == 0 && aligned16(x) && aligned16(y);
+  // f32 strips of several warps are faster with two rows and three CTAs per SM
+  // (50000 x 1024: 67 us, 77 with four and two), the others with four and two
+  if (vec && a.cols <= kStripCols)
+    return sizeof(T) == 4 && a.cols > 256 ? fwd_strips<T, 2>(x, y, a, num_sms, stream)
+                                          : fwd_strips<T, 4>(x, y, a, num_sms, stream);
+  if (a.cols <= 256) return fwd_rows<T, 1>(x, y, a, stream);
+  if (a.cols <= 512) return fwd_rows<T, 2>(x, y, a, stream);
+  if (a.cols <= 1024) return fwd_rows<T, 4>(x, y, a, stream);
+  if (a.cols <= 2048) return fwd_rows<T, 8>(x, y, a, stream);
   const int grid = static_cast<int>(std::min<int64_t>(a.rows, 8 * num_sms));
   return launch_pdl(norm_fwd_wide_kernel<T>, dim3(grid), dim3(256), 0, stream, x, a.rows, a.cols,
                     a.gamma, a.beta, a.eps, y, a.mean, a.rstd);
