@@ -51,7 +51,7 @@ cudaError_t launch_fp8_small(bool bf16, const void* x, uint8_t* xq, float* xs, i
 // type (db may be null).  dy bf16 [M, N], N % 8 == 0, K % 16 == 0.
 cudaError_t launch_fp8_weight_grad(bool bf16_out, const void* dy, const uint8_t* xq,
                                    const float* xs, int M, int N, int K, void* dw, void* db,
-                                   int* err, cudaStream_t stream);
+                                   int num_sms, int* err, cudaStream_t stream);
 
 // y = (x - mean) * rstd * gamma + beta over rows of cols; mean and rstd
 // (f32 [rows]) written when non-null.  y may be x.

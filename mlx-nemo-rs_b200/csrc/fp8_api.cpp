@@ -146,7 +146,7 @@ int nrp_fp8_linear_weight_grad(nrp_context* ctx, void* stream, const void* dy, c
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   ProfScope ps(ctx, NRP_KERNEL_FP8_WGRAD, st);
   return status(nrp::launch_fp8_weight_grad(dtype == NRP_DTYPE_BF16, dy, xq, xs, M, N, K, dw,
-                                            dbias, ctx->d_err, st),
+                                            dbias, ctx->num_sms, ctx->d_err, st),
                 "fp8 weight gradient");
 }
 

@@ -16,17 +16,19 @@
 // The bf16 checkpoint never exists in HBM, and the codes are half its bytes.
 // The kernel is bound by the bf16 tensor rate.
 //
-// Tiles are 128 k x 256 n, one per CTA.  Where they do not fill the SMs, a
-// cluster of 2, 4 or 8 CTAs splits the tokens of one tile; the partial tiles
-// are summed in rank order through distributed shared memory, so the result
-// does not depend on timing and needs no workspace.  The bias' gradient is
+// Tiles are 128 k x 256 n, one per CTA, or narrower for few tokens.  Where they do
+// not fill the SMs, a cluster of 2, 4 or 8 CTAs splits the tokens of one tile;
+// the partial tiles are summed in rank order through distributed shared memory,
+// so the result does not depend on timing and needs no workspace.  That sum costs
+// about 4 us for four partial 256-wide tiles, which narrower ones save at the
+// price of more conversion.  The bias' gradient is
 // summed from the dy tiles in shared memory, which all of a column's tiles
 // hold: each takes every tiles_k-th 8 columns, so that no CTA is the slowest.
 //
 // Shared-memory traffic costs most: per 64 tokens 48 KB of MMA operands, 40 KB
 // of TMA writes and 24 KB of conversion, 896 cycles at 128 bytes each against
-// the tensor cores' 512.  Tried and slower at 16000 x 4096 x 1024 (133 us
-// here): CTA pairs with 256 x 256 tiles (165, the hand-off of both CTAs'
+// the tensor cores' 512.  Measured at 16000 x 4096 x 1024 with bias: 128 us, 1.05
+// PFLOP/s.  Tried and slower: CTA pairs with 256 x 256 tiles (165, the hand-off of both CTAs'
 // conversions to one issuer), 512-wide tiles (145), the k0 = 0 tiles summing
 // all of the bias (170 to 195), CTAs of its own for the bias (133, but a
 // second wave of clusters at 1024 x 1024).
@@ -46,7 +48,6 @@ namespace nrp {
 namespace {
 
 constexpr int kTK = 128;    // k columns of a CTA: one scale block
-constexpr int kTN = 256;    // n columns of a tile: MMA N
 constexpr int kTok = 64;    // tokens per stage
 constexpr int kStages = 4;
 constexpr int kSets = 4;    // dequantising sets of four warps
@@ -56,11 +57,16 @@ constexpr int kThreads = 32 * (kDeqWarp0 + 4 * kSets);
 constexpr int kStoreThreads = 512;
 constexpr uint32_t kBlk = kTok * 128;         // bytes of a 64-column bf16 block
 constexpr uint32_t kABytes = kTK / 64 * kBlk;
-constexpr uint32_t kBBytes = kTN / 64 * kBlk;
 constexpr uint32_t kRawBytes = kTok * kTK;
-constexpr size_t kSmem = 1024 + kStages * (kABytes + kBBytes + kRawBytes) + kTN * 4 + 256;
-static_assert(kSmem <= 232448, "shared memory budget");
-static_assert(kTN * kTK * 4 <= kStages * (kABytes + kBBytes), "a partial tile fits the stages");
+
+// kTN: n columns of a tile (MMA N)
+template <int kTN>
+struct Cfg {
+  static constexpr uint32_t kBBytes = kTN / 64 * kBlk;
+  static constexpr size_t kSmem = 1024 + kStages * (kABytes + kBBytes + kRawBytes) + kTN * 4 + 256;
+  static_assert(kSmem <= 232448, "shared memory budget");
+  static_assert(kTN * kTK * 4 <= kStages * (kABytes + kBBytes), "a partial tile fits the stages");
+};
 
 struct Bars {
   uint64_t full[kStages];   // dy by TMA
@@ -131,16 +137,38 @@ __device__ __forceinline__ uint32_t codes_to_bf16(uint32_t w, uint32_t f) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(f));
   return d;
 }
+// Before a barrier arrival that hands shared memory back to TMA: the thread's
+// reads of it are complete, and ordered before the copy that overwrites it.  The
+// arrival alone is not enough (generic reads against writes of the async
+// proxy): without this, stages that come round again were overwritten under
+// their readers.
+__device__ __forceinline__ void reads_done() { fence_proxy_async_smem(); }
 // Whether a byte of w is the NaN code.
 __device__ __forceinline__ bool has_nan_code(uint32_t w) {
   return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
 }
 
+// Four consecutive elements; wide: 16 (or 8) bytes at once.
 template <typename TO>
+__device__ __forceinline__ void store_four(TO* p, float4 v, bool wide) {
+  if (!wide) {
+    store_one(p, v.x);
+    store_one(p + 1, v.y);
+    store_one(p + 2, v.z);
+    store_one(p + 3, v.w);
+  } else if constexpr (sizeof(TO) == 4) {
+    *reinterpret_cast<float4*>(p) = v;
+  } else {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+  }
+}
+
+template <int kTN, typename TO>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy,  // bf16 [M, N], box (64, 64)
                      const __grid_constant__ CUtensorMap map_xq,  // u8 [M, K], box (128, 64)
                      const Args a) {
+  constexpr uint32_t kBBytes = Cfg<kTN>::kBBytes;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* base = smem_raw + (((raw + 1023u) & ~1023u) - raw);
@@ -281,6 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
+        reads_done();
         __syncwarp();
         if (lane == 0) mbar_arrive(&ss->empty[s]);
       }
@@ -336,6 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int h = 0; h < kRowsT; ++h)
         q[h] = *reinterpret_cast<const uint4*>(sR + s * kRawBytes + (row + 16 * h) * 128 + c * 16);
+      reads_done();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ss->rempty[s]);
       uint32_t out[kRowsT][8];
@@ -394,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!fine) *abort_flag = 1;
   tc_fence_after();
   __syncthreads();
-  const int quad = warp & 3, grp = warp >> 2;  // a quarter of n each
+  const int quad = warp & 3, grp = warp >> 2;  // 32 columns of n at a time
   const bool storer = threadIdx.x < kStoreThreads;
   const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16);
   TO* dw = static_cast<TO*>(a.dw);
@@ -405,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!*abort_flag && storer) {
       const int k = k0 + quad * 32 + lane;
 #pragma unroll 1
-      for (int c = grp * 64; c < grp * 64 + 64; c += 32) {
+      for (int c = grp * 32; c < kTN; c += 128) {
         uint32_t r[32];
         tmem_ld32(taddr + c, r);
         tmem_ld_wait();
@@ -420,11 +450,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         store_one(db + n0 + threadIdx.x, sBias[threadIdx.x]);
     }
   } else {
-    // partial sums [256 n][128 k] f32 over the (drained) stages
+    // partial sums [kTN n][128 k] f32 over the (drained) stages
     float* part = reinterpret_cast<float*>(base);
     if (storer) {
 #pragma unroll 1
-      for (int c = grp * 64; c < grp * 64 + 64; c += 32) {
+      for (int c = grp * 32; c < kTN; c += 128) {
         uint32_t r[32];
         tmem_ld32(taddr + c, r);
         tmem_ld_wait();
@@ -436,16 +466,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     cluster_sync();
     // this rank's columns, four k at a time, the ranks' tiles in order
     const int cols = kTN / a.split;
-    for (int u = threadIdx.x; u < cols * (kTK / 4); u += kThreads) {
-      const int nn = rank * cols + u / (kTK / 4), kk = (u % (kTK / 4)) * 4;
-      const float4 sum = cluster_sum4(smem_u32(part + nn * kTK + kk), a.split);
-      const int n = n0 + nn, k = k0 + kk;
-      if (n < a.N && k < a.K) {  // K % 16 == 0: the four are inside together
-        TO* o = dw + static_cast<int64_t>(n) * a.K + k;
-        store_one(o, sum.x);
-        store_one(o + 1, sum.y);
-        store_one(o + 2, sum.z);
-        store_one(o + 3, sum.w);
+    const bool wide = reinterpret_cast<uintptr_t>(dw) % 16 == 0;
+    constexpr int kFly = 3;  // units whose loads are in flight together
+    for (int u0 = threadIdx.x; u0 < cols * (kTK / 4); u0 += kFly * kThreads) {
+      float4 sum[kFly];
+#pragma unroll
+      for (int i = 0; i < kFly; ++i) {
+        const int u = min(u0 + i * kThreads, cols * (kTK / 4) - 1);
+        const int nn = rank * cols + u / (kTK / 4), kk = (u % (kTK / 4)) * 4;
+        sum[i] = cluster_sum4(smem_u32(part + nn * kTK + kk), a.split);
+      }
+#pragma unroll
+      for (int i = 0; i < kFly; ++i) {
+        const int u = u0 + i * kThreads;
+        const int n = n0 + rank * cols + u / (kTK / 4), k = k0 + (u % (kTK / 4)) * 4;
+        if (u < cols * (kTK / 4) && n < a.N && k < a.K)  // K % 16 == 0: all four are inside
+          store_four(dw + static_cast<int64_t>(n) * a.K + k, sum[i], wide);
       }
     }
     for (int c = threadIdx.x; c < cols; c += kThreads) {
@@ -484,10 +520,11 @@ int max_clusters(F* kernel, int size, size_t smem) {
   return n;
 }
 
-template <typename TO>
+template <int kTN, typename TO>
 cudaError_t launch(const void* dy, const uint8_t* xq, Args a, cudaStream_t stream) {
+  constexpr size_t kSmem = Cfg<kTN>::kSmem;
   static std::atomic<uint64_t> attr{0};
-  auto* kernel = fp8_wgrad_kernel<TO>;
+  auto* kernel = fp8_wgrad_kernel<kTN, TO>;
   if (cudaError_t e = smem_attr_once(kernel, static_cast<int>(kSmem), attr)) return e;
   CUtensorMap mdy, mxq;
   if (!make_tmap_2d(&mdy, dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.N, a.M,
@@ -528,11 +565,25 @@ cudaError_t launch(const void* dy, const uint8_t* xq, Args a, cudaStream_t strea
   return cudaLaunchKernelEx(&cfg, kernel, mdy, mxq, a);
 }
 
+template <typename TO>
+cudaError_t pick(const void* dy, const uint8_t* xq, const Args& a, int num_sms,
+                 cudaStream_t stream) {
+  // Few tokens and no full wave of wide tiles: narrower ones, whose partial sums
+  // are smaller, down to 64 columns where those need no split at all (1024 x
+  // 1024, 256 / 128 / 64 columns: 100 tokens 10.0 / 7.5 / 5.5 us, 749 tokens
+  // 12.0 / 9.7 / 9.4, 1500 tokens 15.1 / 12.2 / 13.8, 5000 tokens 21.8 / 23.7 / 33.8).
+  const int64_t kb = qblocks(a.K);
+  if (a.M <= 768 && kb * ((a.N + 63) / 64) <= num_sms) return launch<64, TO>(dy, xq, a, stream);
+  if (a.M <= 2816 && 2 * kb * ((a.N + 255) / 256) <= num_sms)
+    return launch<128, TO>(dy, xq, a, stream);
+  return launch<256, TO>(dy, xq, a, stream);
+}
+
 }  // namespace
 
 cudaError_t launch_fp8_weight_grad(bool bf16_out, const void* dy, const uint8_t* xq,
                                    const float* xs, int M, int N, int K, void* dw, void* db,
-                                   int* err, cudaStream_t stream) {
+                                   int num_sms, int* err, cudaStream_t stream) {
   if (M <= 0) {  // no tokens: the sums are empty
     const size_t es = bf16_out ? 2 : 4;
     if (cudaError_t e = cudaMemsetAsync(dw, 0, static_cast<size_t>(N) * K * es, stream)) return e;
@@ -547,8 +598,8 @@ cudaError_t launch_fp8_weight_grad(bool bf16_out, const void* dy, const uint8_t*
   a.K = K;
   a.kb = static_cast<int>(qblocks(K));
   a.err = err;
-  return bf16_out ? launch<__nv_bfloat16>(dy, xq, a, stream)
-                  : launch<float>(dy, xq, a, stream);
+  return bf16_out ? pick<__nv_bfloat16>(dy, xq, a, num_sms, stream)
+                  : pick<float>(dy, xq, a, num_sms, stream);
 }
 
 }  // namespace nrp

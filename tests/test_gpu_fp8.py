@@ -311,6 +311,49 @@ def test_weight_grad_is_a_derivative(nrp):
     assert abs(float((dx.double().cpu() * v).sum() - diff)) <= float(size)
 
 
+def device_values(q):
+    """float64 values of an Fp8Tensor on the device."""
+    s = q.scales.double().repeat_interleave(q.block_rows, 0)[:q.codes.shape[0]]
+    return q.codes.double() * s.repeat_interleave(128, 1)[:, :q.codes.shape[1]]
+
+
+@pytest.mark.parametrize("m,k,n", [(16000, 1024, 4096), (5000, 1024, 1024), (3000, 2048, 1040),
+                                   (16000, 144, 256), (12500, 512, 1024)])
+def test_long_sums_and_repeats(nrp, m, k, n):
+    """Many turns of the kernels' stage rings and many waves of tiles: each
+    direction against 64 bits on the device, and twenty times the same bits
+    (a stage handed back too early shows in some of them only)."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x = torch.randn(m, k, device="cuda", generator=g).mul_(
+        torch.exp2(torch.randn(m, 1, device="cuda", generator=g) * 3)).bfloat16()
+    dy = torch.randn(m, n, device="cuda", generator=g).mul_(1e-3).bfloat16()
+    w = nrp.fp8_quantize(torch.randn(n, k, device="cuda", generator=g) / math.sqrt(k), 128)
+    xq, gq = nrp.fp8_quantize(x), nrp.fp8_quantize(dy)
+    runs = {
+        "linear": lambda: [nrp.fp8_linear(xq, w, dtype=torch.float32)],
+        "input_grad": lambda: [nrp.fp8_linear_input_grad(gq, w, dtype=torch.float32)],
+        "weight_grad": lambda: list(nrp.fp8_linear_weight_grad(dy, xq, bias=True)),
+    }
+    first = {name: f() for name, f in runs.items()}
+    for _ in range(20):
+        for name, f in runs.items():
+            assert all(torch.equal(a, b) for a, b in zip(f(), first[name])), name
+    nrp.Context.default().check()
+    xv, wv, gv, d = device_values(xq), device_values(w), device_values(gq), dy.double()
+
+    def check(got, a, b, chain):
+        ref, size = a @ b, a.abs() @ b.abs()
+        off = (got.double() - ref).abs()
+        assert (off <= size * chain + ref.abs() * U).all(), float((off / size).max())
+
+    check(first["linear"][0], xv, wv.t(), 132 * 2.0 ** -23 + (k // 128 + 4) * U)
+    check(first["input_grad"][0], gv, wv, 132 * 2.0 ** -23 + (n // 128 + 4) * U)
+    check(first["weight_grad"][0], d.t(), xv, (m + m / 16 + 16) * 2.0 ** -23)
+    off = (first["weight_grad"][1].double() - d.sum(0)).abs()
+    assert (off <= d.abs().sum(0) * (m + 16) * U).all()
+
+
 def test_repeatable(nrp):
     """Two calls on the same inputs give the same bits."""
     import torch
