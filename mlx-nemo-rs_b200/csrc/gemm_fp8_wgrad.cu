@@ -27,8 +27,8 @@
 //
 // Shared-memory traffic costs most: per 64 tokens 48 KB of MMA operands, 40 KB
 // of TMA writes and 24 KB of conversion, 896 cycles at 128 bytes each against
-// the tensor cores' 512.  Measured at 16000 x 4096 x 1024 with bias: 128 us, 1.05
-// PFLOP/s.  Tried and slower: CTA pairs with 256 x 256 tiles (165, the hand-off of both CTAs'
+// the tensor cores' 512.  Measured at 16000 x 4096 x 1024 with bias: 141 us, 0.95
+// PFLOP/s.  Tried and slower (then against 126 to 135): CTA pairs with 256 x 256 tiles (165, the hand-off of both CTAs'
 // conversions to one issuer), 512-wide tiles (145), the k0 = 0 tiles summing
 // all of the bias (170 to 195), CTAs of its own for the bias (133, but a
 // second wave of clusters at 1024 x 1024).
@@ -55,6 +55,15 @@ constexpr int kBiasWarp0 = 3, kBiasWarps = 4;
 constexpr int kDeqWarp0 = kBiasWarp0 + kBiasWarps;
 constexpr int kThreads = 32 * (kDeqWarp0 + 4 * kSets);
 constexpr int kStoreThreads = 512;
+// Steps between two additions of the accumulator to the running sum.  The
+// tensor cores cut each addition to the accumulator off instead of rounding it,
+// an error that grows with their number: 8e-6 of the result's norm after 1000 (16000
+// tokens of 16000 x 4096 x 1024, an f32 product being off by 6e-7).  After 64
+// additions the accumulator is added to a second one in f32, rounded to
+// nearest, and starts again from zero: 3e-7, for 141 us against 131 (every 32
+// steps 6e-7 and 137 us, every 64 1.4e-6 and 135 us).
+constexpr int kSeg = 16;
+static_assert(kSeg % kSets == 0 && kSeg > kSets, "every set starts every segment");
 constexpr uint32_t kBlk = kTok * 128;         // bytes of a 64-column bf16 block
 constexpr uint32_t kABytes = kTK / 64 * kBlk;
 constexpr uint32_t kRawBytes = kTok * kTK;
@@ -74,6 +83,7 @@ struct Bars {
   uint64_t empty[kStages];
   uint64_t rfull[kStages];   // codes by TMA
   uint64_t rempty[kStages];
+  uint64_t seg_full, seg_empty;  // a segment's sums are complete; are taken
   uint64_t done;
   uint32_t tmem_base;
   int abort;
@@ -163,6 +173,35 @@ __device__ __forceinline__ void store_four(TO* p, float4 v, bool wide) {
   }
 }
 
+// Adds a segment's sums to the running sums kTN columns further on (`more`: there
+// are some) in a quarter of the tile's columns, once full completes the phase
+// `parity`, and arrives on empty.  Out of line: its registers would spill the
+// conversion's.
+template <int kTN>
+__device__ __noinline__ bool add_segment(uint32_t at, bool more, uint64_t* full, uint64_t* empty,
+                                         uint32_t parity, int* err) {
+  if (!warp_mbar_wait_hot(full, parity, err, kDevTimeoutMma)) return false;
+  tc_fence_after();
+#pragma unroll 1
+  for (int c = 0; c < kTN / kSets; c += 16) {
+    uint32_t r[16], t[16];
+    tmem_ld16(at + c, r);
+    if (more) tmem_ld16(at + kTN + c, t);
+    tmem_ld_wait();
+    if (more) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        r[e] = __float_as_uint(__uint_as_float(r[e]) + __uint_as_float(t[e]));
+    }
+    tmem_st16(at + kTN + c, r);
+  }
+  tmem_st_wait();
+  tc_fence_before();
+  __syncwarp();
+  if (lane_id() == 0) mbar_arrive(empty);
+  return true;
+}
+
 template <int kTN, typename TO>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy,  // bf16 [M, N], box (64, 64)
@@ -195,6 +234,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&ss->rempty[s], 4);
       mbar_init(&ss->empty[s], a.db ? 1 + kBiasWarps : 1);  // the MMAs, the bias warps
     }
+    mbar_init(&ss->seg_full, 1);
+    mbar_init(&ss->seg_empty, 4 * kSets);
     mbar_init(&ss->done, 1);
     ss->abort = 0;
     fence_mbar_init();
@@ -202,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tensormap(&map_xq);
   }
   if (warp == 1) {
-    tmem_alloc(&ss->tmem_base, kTN);
+    tmem_alloc(&ss->tmem_base, 2 * kTN);  // a segment's sums, the sum of the segments
     tmem_relinquish();
   }
   tc_fence_before();
@@ -262,14 +303,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         *abort_flag = 1;
         break;
       }
+      if (i > 0 && i % kSeg == 0 &&
+          !warp_mbar_wait_hot(&ss->seg_empty, (i / kSeg - 1) & 1, a.err, kDevTimeoutEpi)) {
+        *abort_flag = 1;
+        break;
+      }
       tc_fence_after();
       if (elect_one()) {
         const uint32_t a0 = smem_u32(sA + s * kABytes), b0 = smem_u32(sB + s * kBBytes);
 #pragma unroll
         for (int k = 0; k < kTok / 16; ++k)
           umma_ss(tmem, sdesc_sw128(a0 + k * 2048, kBlk, 1024),
-                  sdesc_sw128(b0 + k * 2048, kBlk, 1024), idesc, (i | k) != 0);
+                  sdesc_sw128(b0 + k * 2048, kBlk, 1024), idesc, (i % kSeg | k) != 0);
         umma_commit(&ss->empty[s]);
+        if ((i + 1) % kSeg == 0 && i + 1 < steps) umma_commit(&ss->seg_full);
       }
       __syncwarp();
     }
@@ -350,6 +397,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     scales(set);
+    const uint32_t quarter =
+        tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + set * (kTN / kSets);
+    // Behind its first step of a segment, which the MMAs then find ready, a set
+    // takes its quarter of the segment before.
+    auto take_segment = [&](int b) -> bool {
+      if (!*abort_flag &&
+          add_segment<kTN>(quarter, b > 1, &ss->seg_full, &ss->seg_empty, (b - 1) & 1, a.err))
+        return true;
+      *abort_flag = 1;
+      return false;
+    };
+    int taken = 0;
     for (int i = set; i < steps; i += kSets) {
       const int s = i % kStages;
       const uint32_t round = i / kStages;
@@ -415,7 +474,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ss->deq[s]);
+      if (i >= kSeg && i % kSeg < kSets) {
+        if (!take_segment(i / kSeg)) break;
+        ++taken;
+      }
     }
+    // a last segment too short for this set to have a step in it
+    if (taken < (steps - 1) / kSeg && !*abort_flag) take_segment((steps - 1) / kSeg);
   }
 
   // ------------------------------------------------------------- the result
@@ -427,6 +492,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int quad = warp & 3, grp = warp >> 2;  // 32 columns of n at a time
   const bool storer = threadIdx.x < kStoreThreads;
   const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+  // 32 columns of the result: the last segment's, and the sum of those before
+  auto sums = [&](int c, float (&v)[32]) {
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      uint32_t r[16], t[16];
+      tmem_ld16(taddr + c + h, r);
+      if (steps > kSeg) tmem_ld16(taddr + kTN + c + h, t);
+      tmem_ld_wait();
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        v[h + e] = __uint_as_float(r[e]) + (steps > kSeg ? __uint_as_float(t[e]) : 0.f);
+    }
+  };
   TO* dw = static_cast<TO*>(a.dw);
   TO* db = static_cast<TO*>(a.db);
   // bias columns this CTA summed (this rank writes its share of them)
@@ -436,14 +514,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int k = k0 + quad * 32 + lane;
 #pragma unroll 1
       for (int c = grp * 32; c < kTN; c += 128) {
-        uint32_t r[32];
-        tmem_ld32(taddr + c, r);
-        tmem_ld_wait();
+        float v[32];
+        sums(c, v);
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           const int n = n0 + c + e;
           if (n < a.N && k < a.K)
-            store_one(dw + static_cast<int64_t>(n) * a.K + k, __uint_as_float(r[e]));
+            store_one(dw + static_cast<int64_t>(n) * a.K + k, v[e]);
         }
       }
       if (threadIdx.x < kTN && bias_here(threadIdx.x))
@@ -455,12 +532,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (storer) {
 #pragma unroll 1
       for (int c = grp * 32; c < kTN; c += 128) {
-        uint32_t r[32];
-        tmem_ld32(taddr + c, r);
-        tmem_ld_wait();
+        float v[32];
+        sums(c, v);
 #pragma unroll
         for (int e = 0; e < 32; ++e)
-          part[(c + e) * kTK + quad * 32 + lane] = __uint_as_float(r[e]);
+          part[(c + e) * kTK + quad * 32 + lane] = v[e];
       }
     }
     cluster_sync();
@@ -494,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, kTN);
+    tmem_dealloc(tmem, 2 * kTN);
   }
 }
 
