@@ -45,6 +45,28 @@ cudaError_t smem_attr_once(F* func, int bytes, std::atomic<uint64_t>& done) {
   return e;
 }
 
+// The clusters of `size` CTAs of the kernel that fit the device at once.
+template <typename F>
+inline int max_clusters(F* kernel, int size, int threads, size_t smem) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(size));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute la[1];
+  la[0].id = cudaLaunchAttributeClusterDimension;
+  la[0].val.clusterDim.x = static_cast<unsigned>(size);
+  la[0].val.clusterDim.y = 1;
+  la[0].val.clusterDim.z = 1;
+  cfg.attrs = la;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return n;
+}
+
 // ---- TMA descriptors (driver entry point resolved through the runtime) ----
 // Row-major 2-D tensor [outer, inner] of `elem_bytes` elements, row stride in
 // bytes; box (box_inner, box_outer); 128-byte swizzle when box_inner *

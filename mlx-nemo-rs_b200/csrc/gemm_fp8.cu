@@ -18,7 +18,8 @@
 //
 // Warp roles (10 warps): 0 TMA producer, 1 TMEM allocator and MMA issuer,
 // 2..9 epilogue (two groups of four, each half of the tile's columns).  The
-// grid is persistent, one CTA per SM.  An epilogue thread keeps 128 sums and
+// grid is persistent, one CTA per SM; where the tiles are few and the
+// reduction is long, a cluster shares a tile's reduction (launch).  An epilogue thread keeps 128 sums and
 // two 16-column reads of TMEM in its 168 registers.
 #include <algorithm>
 
@@ -42,6 +43,12 @@ constexpr int kChunk = 8, kScalePitch = kChunk + 1;
 constexpr int kScaleBuf = 32 * kScalePitch + kChunk;
 constexpr int kScaleFloats = 2 * kScaleBuf;
 
+// A split tile's partial sums: four more floats to a row, for the banks.
+constexpr int kPartPitch = 128 + 4;
+// A split spares each CTA at least this many blocks of the reduction: a cluster
+// starts and joins in 1.7 us, a block takes 0.33 us.
+constexpr int kSplitSaves = 6;
+
 template <int kBN>
 struct Cfg {
   static constexpr int kStages = kBN == 256 ? 3 : 5;
@@ -52,6 +59,8 @@ struct Cfg {
 };
 static_assert(Cfg<256>::kSmem <= 232448 && Cfg<128>::kSmem <= 232448,
               "shared memory budget");
+static_assert(kBM * kPartPitch * 4 <= Cfg<128>::kStages * (kABytes + Cfg<128>::kBBytes),
+              "a split tile's sums fit the ring");
 
 struct Bars {
   uint64_t full[kMaxStages];
@@ -91,6 +100,7 @@ struct Args {
   void* y;           // [M, NO]
   int M, NO, rb;     // rb: reduction blocks
   int tma_out;       // y's rows are 16-byte multiples: stored through map_y
+  int split;         // CTAs to a tile (a cluster), each with blocks of the reduction
   int* err;
 };
 
@@ -100,7 +110,8 @@ __device__ __forceinline__ float to_f32(TO v) {
   else return __bfloat162float(v);
 }
 
-template <int kBN, bool kTrans, typename TO>
+// kSplit: a cluster of a.split CTAs shares one tile's reduction.
+template <int kBN, bool kTrans, typename TO, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_x,
                     const __grid_constant__ CUtensorMap map_w,
@@ -117,11 +128,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sB = sA + kStages * kABytes;
   uint8_t* sE = sB + kStages * kBBytes;
   float* sS = reinterpret_cast<float*>(sE + 8 * kSlabBytes);
+  [[maybe_unused]] float* part = reinterpret_cast<float*>(sA);  // kSplit: [128][kPartPitch]
   Bars* ss = reinterpret_cast<Bars*>(sS + 8 * kScaleFloats);
   const int warp = static_cast<int>(uniform(threadIdx.x >> 5)), lane = lane_id();
   const int tiles_m = (a.M + kBM - 1) / kBM;
   const int tiles_n = (a.NO + kBN - 1) / kBN;
   const int num_tiles = tiles_m * tiles_n;
+  // this CTA's tiles and blocks of the reduction
+  const int first = kSplit ? blockIdx.x / a.split : blockIdx.x;
+  const int step = kSplit ? num_tiles : gridDim.x;
+  const int share = kSplit ? (a.rb + a.split - 1) / a.split : a.rb;
+  const int lo = kSplit ? min(static_cast<int>(cluster_ctarank()) * share, a.rb) : 0;
+  const int blocks = kSplit ? min(share, a.rb - lo) : a.rb;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -153,9 +171,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     // ---------------------------------------------------------- producer
     uint32_t it = 0;
-    for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
+    for (int t = first; t < num_tiles && !*abort_flag; t += step) {
       const int m0 = t / tiles_n * kBM, n0 = t % tiles_n * kBN;
-      for (int b = 0; b < a.rb; ++b, ++it) {
+      for (int b = 0; b < blocks; ++b, ++it) {
         const int s = it % kStages;
         if (!warp_mbar_wait(&ss->empty[s], ((it / kStages) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
           *abort_flag = 1;
@@ -164,14 +182,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (elect_one()) {
           uint8_t *A = sA + s * kABytes, *B = sB + s * kBBytes;
           mbar_arrive_expect_tx(&ss->full[s], kABytes + kBBytes);
-          tma_load_2d(A, &map_x, &ss->full[s], b * kBR, m0);
+          tma_load_2d(A, &map_x, &ss->full[s], (lo + b) * kBR, m0);
           if constexpr (!kTrans) {
-            tma_load_2d(B, &map_w, &ss->full[s], b * kBR, n0);  // [n][128 r]
+            tma_load_2d(B, &map_w, &ss->full[s], (lo + b) * kBR, n0);  // [n][128 r]
           } else {
             // [r][128 n]: one box per 128 columns
 #pragma unroll
             for (int j = 0; j < kBN; j += 128)
-              tma_load_2d(B + j * kBR, &map_w, &ss->full[s], n0 + j, b * kBR);
+              tma_load_2d(B + j * kBR, &map_w, &ss->full[s], n0 + j, (lo + b) * kBR);
           }
         }
         __syncwarp();
@@ -185,8 +203,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // -------------------------------------------------------- MMA issuer
     constexpr uint32_t idesc = idesc_e4m3_f32(kBM, kBN, kTrans ? 1 : 0);
     uint32_t it = 0;
-    for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
-      for (int b = 0; b < a.rb; ++b, ++it) {
+    for (int t = first; t < num_tiles && !*abort_flag; t += step) {
+      for (int b = 0; b < blocks; ++b, ++it) {
         const int s = it % kStages, buf = it % kBufs;
         if (!warp_mbar_wait(&ss->tempty[buf], ((it / kBufs) & 1) ^ 1, a.err, kDevTimeoutEpi) ||
             !warp_mbar_wait(&ss->full[s], (it / kStages) & 1, a.err, kDevTimeoutLoad)) {
@@ -228,9 +246,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     // with it, 68 with these.)
     auto prefetch = [&](int t, int c, int buf) {
       const int nb = min((t % tiles_n * kBN + group * kHalfN) / 128, ncb - 1);
-      const int64_t b = c * kChunk + (lane & 7);
+      const int64_t b = lo + c * kChunk + (lane & 7);
       float* to = scales + buf * kScaleBuf;
-      if (b < a.rb) {
+      if (b < lo + blocks) {
         // a row's eight scales are one sector: four rows to an instruction
         const int row0 = t / tiles_n * kBM + quad * 32 + (lane >> 3);
 #pragma unroll
@@ -243,26 +261,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-    const int chunks = (a.rb + kChunk - 1) / kChunk;
+    const int chunks = (blocks + kChunk - 1) / kChunk;
     int sbuf = 0;
-    if (static_cast<int>(blockIdx.x) < num_tiles) prefetch(blockIdx.x, 0, 0);
+    if (first < num_tiles) prefetch(first, 0, 0);
     commit();
     uint32_t it = 0;
-    for (int t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
+    for (int t = first; t < num_tiles && !*abort_flag; t += step) {
       const int m0 = t / tiles_n * kBM, n0 = t % tiles_n * kBN + group * kHalfN;
       const int row = m0 + quad * 32 + lane;
       float acc[kHalfN];
 #pragma unroll
       for (int e = 0; e < kHalfN; ++e) acc[e] = 0.f;
       bool ok = true;
-      for (int b = 0; b < a.rb; ++b, ++it) {
+      for (int b = 0; b < blocks; ++b, ++it) {
         const int buf = it % kBufs;
         if (b % kChunk == 0) {
           const int c = b / kChunk;
           if (b) sbuf ^= 1;
           __syncwarp();  // the other buffer's readers are done
           if (c + 1 < chunks) prefetch(t, c + 1, sbuf ^ 1);
-          else if (t + static_cast<int>(gridDim.x) < num_tiles) prefetch(t + gridDim.x, 0, sbuf ^ 1);
+          else if (t + step < num_tiles) prefetch(t + step, 0, sbuf ^ 1);
           commit();
           asm volatile("cp.async.wait_group 1;" ::: "memory");
           __syncwarp();
@@ -299,6 +317,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!ok) break;
+      if constexpr (kSplit) {
+        // the ring's loads and MMAs are done: this CTA's sums take its place
+        float* to = part + (quad * 32 + lane) * kPartPitch + group * kHalfN;
+#pragma unroll
+        for (int e = 0; e < kHalfN; e += 4)
+          *reinterpret_cast<float4*>(to + e) =
+              make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+        break;
+      }
       sbuf ^= 1;  // the next tile's first scales
       const TO* bias = static_cast<const TO*>(a.bias);
       const bool bias_vec = (reinterpret_cast<uintptr_t>(bias) & 15) == 0;
@@ -365,6 +392,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) bulk_wait_all();
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
+  if constexpr (kSplit) {
+    // Each CTA adds up and stores every split-th row, the cluster's sums in
+    // the order of their ranks.
+    __syncwarp();
+    cluster_sync();
+    const int m0 = first / tiles_n * kBM, n0 = first % tiles_n * kBN;
+    const int rows = min(kBM, a.M - m0), cols = min(kBN, a.NO - n0);
+    const TO* bias = static_cast<const TO*>(a.bias);
+    TO* y = static_cast<TO*>(a.y);
+    for (int i = warp * a.split + static_cast<int>(cluster_ctarank()); i < rows;
+         i += kThreads / 32 * a.split) {
+      const int c = lane * 4;
+      if (c >= cols) continue;
+      const float4 q = cluster_sum4(smem_u32(part + i * kPartPitch + c), a.split);
+      float v[4] = {q.x, q.y, q.z, q.w};
+      TO* o = y + static_cast<int64_t>(m0 + i) * a.NO + n0 + c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (bias && c + e < cols) v[e] += to_f32(bias[n0 + c + e]);
+      if (a.tma_out) {  // whole groups of four, 16 (8) byte aligned
+        if constexpr (sizeof(TO) == 4)
+          *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+          *reinterpret_cast<uint2*>(o) =
+              make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < cols) {
+            if constexpr (sizeof(TO) == 4) o[e] = v[e];
+            else o[e] = __float2bfloat16_rn(v[e]);
+          }
+      }
+    }
+    cluster_sync();  // no CTA leaves while another reads its sums
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -373,12 +436,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int kBN, bool kTrans, typename TO>
+template <int kBN, bool kTrans, typename TO, bool kSplit>
 cudaError_t launch(const uint8_t* xq, int R, const uint8_t* wq, Args a, int num_sms,
                    cudaStream_t stream) {
   static std::atomic<uint64_t> attr{0};
   constexpr int kSmem = static_cast<int>(Cfg<kBN>::kSmem);
-  auto* kernel = gemm_fp8_kernel<kBN, kTrans, TO>;
+  auto* kernel = gemm_fp8_kernel<kBN, kTrans, TO, kSplit>;
   if (cudaError_t e = smem_attr_once(kernel, kSmem, attr)) return e;
   constexpr int es = sizeof(TO);
   CUtensorMap mx, mw, my;
@@ -398,6 +461,43 @@ cudaError_t launch(const uint8_t* xq, int R, const uint8_t* wq, Args a, int num_
   const int64_t tiles =
       ((a.M + kBM - 1) / kBM) * static_cast<int64_t>((a.NO + kBN - 1) / kBN);
   if (tiles > 0x7fffffff) return cudaErrorInvalidValue;
+  if constexpr (kSplit) {
+    // The largest split whose clusters all run at once (on a B200 33 of four
+    // CTAs, 15 of eight) and that leaves a CTA two blocks.  Split against one
+    // CTA to a tile, bf16 output: 64 rows, 1024 to 1024 5.1 against 5.9 us, 4096
+    // to 1024 6.4 against 13.8; 896 rows, 4096 to 1024 12.2 against 15.1, 2048
+    // to 1024 9.2 against 9.3, and 1024 to 1024 (a split of two would spare four
+    // blocks) 7.8 against 6.5.
+    static std::atomic<int> fit[64][4];
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return e;
+    a.split = 1;
+    for (int l = 1; l <= 3 && a.rb >> l >= 2; ++l) {
+      if (a.rb - (a.rb >> l) < kSplitSaves) continue;
+      int f = fit[dev & 63][l].load(std::memory_order_relaxed);
+      if (f == 0) {
+        f = max_clusters(kernel, 1 << l, kThreads, kSmem);
+        fit[dev & 63][l].store(f > 0 ? f : -1, std::memory_order_relaxed);
+      }
+      if (tiles <= f) a.split = 1 << l;
+    }
+    if (a.split == 1) return launch<kBN, kTrans, TO, false>(xq, R, wq, a, num_sms, stream);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * a.split));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute la[2];
+    la[0].id = cudaLaunchAttributeClusterDimension;
+    la[0].val.clusterDim.x = static_cast<unsigned>(a.split);
+    la[0].val.clusterDim.y = 1;
+    la[0].val.clusterDim.z = 1;
+    la[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    la[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = la;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, mx, mw, my, a);
+  }
   const int grid = static_cast<int>(std::min<int64_t>(tiles, num_sms));
   return launch_pdl(kernel, dim3(grid), dim3(kThreads), static_cast<size_t>(kSmem), stream, mx, mw,
                     my, a);
@@ -412,8 +512,10 @@ cudaError_t pick(const uint8_t* xq, int R, const uint8_t* wq, const Args& a, int
   // against 8.0; 2432 x 1024 (152) 9.5 against 8.2, 896 x 4096 (224) 10.4
   // against 8.4, 16000 x 4096 88 against 80.
   const int64_t narrow = static_cast<int64_t>((a.M + kBM - 1) / kBM) * ((a.NO + 127) / 128);
-  if (narrow <= num_sms) return launch<128, kTrans, TO>(xq, R, wq, a, num_sms, stream);
-  return launch<256, kTrans, TO>(xq, R, wq, a, num_sms, stream);
+  if (narrow > num_sms) return launch<256, kTrans, TO, false>(xq, R, wq, a, num_sms, stream);
+  if (a.rb >= kSplitSaves + 2 && 2 * narrow <= num_sms)
+    return launch<128, kTrans, TO, true>(xq, R, wq, a, num_sms, stream);
+  return launch<128, kTrans, TO, false>(xq, R, wq, a, num_sms, stream);
 }
 
 }  // namespace

@@ -103,37 +103,6 @@ __device__ __forceinline__ void store_one(TO* p, float v) {
   else *p = __float2bfloat16_rn(v);
 }
 
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
-  float4 v;
-  asm volatile(
-      "{\n\t.reg .b32 ra;\n\t"
-      "mapa.shared::cluster.u32 ra, %4, %5;\n\t"
-      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [ra];\n\t}\n"
-      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-      : "r"(addr), "r"(rank)
-      : "memory");
-  return v;
-}
-
-// The sum of four floats at one shared-memory offset over the cluster's first
-// `ranks` (2, 4 or 8) CTAs, in rank order, all loads in flight together.
-__device__ __forceinline__ float4 cluster_sum4(uint32_t at, int ranks) {
-  float4 v[8];
-#pragma unroll
-  for (int q = 0; q < 8; ++q)
-    if (q < ranks) v[q] = ld_cluster_f4(at, q);
-  float4 s = v[0];
-#pragma unroll
-  for (int q = 1; q < 8; ++q)
-    if (q < ranks) {
-      s.x += v[q].x;
-      s.y += v[q].y;
-      s.z += v[q].z;
-      s.w += v[q].w;
-    }
-  return s;
-}
-
 // Two bf16 (low half first) of two codes in bytes 0 and 1 (sel 0x1404 of the
 // word) or 2 and 3 (0x3424), times f.  A code's seven exponent and mantissa
 // bits, moved to bf16's places, read as value * 2^-120 (the biases are 7 and
@@ -574,28 +543,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// The clusters of `size` CTAs of the kernel that fit the device at once.
-template <typename F>
-int max_clusters(F* kernel, int size, size_t smem) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(size));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cudaLaunchAttribute la[1];
-  la[0].id = cudaLaunchAttributeClusterDimension;
-  la[0].val.clusterDim.x = static_cast<unsigned>(size);
-  la[0].val.clusterDim.y = 1;
-  la[0].val.clusterDim.z = 1;
-  cfg.attrs = la;
-  cfg.numAttrs = 1;
-  int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
-    cudaGetLastError();
-    return 0;
-  }
-  return n;
-}
-
 template <int kTN, typename TO>
 cudaError_t launch(const void* dy, const uint8_t* xq, Args a, cudaStream_t stream) {
   constexpr size_t kSmem = Cfg<kTN>::kSmem;
@@ -618,7 +565,7 @@ cudaError_t launch(const void* dy, const uint8_t* xq, Args a, cudaStream_t strea
   for (int l = 1; l <= 3 && (1 << l) <= steps; ++l) {
     int f = fit[dev & 63][l].load(std::memory_order_relaxed);
     if (f == 0) {
-      f = max_clusters(kernel, 1 << l, kSmem);
+      f = max_clusters(kernel, 1 << l, kThreads, kSmem);
       fit[dev & 63][l].store(f > 0 ? f : -1, std::memory_order_relaxed);
     }
     if (tiles <= f) a.split = 1 << l;

@@ -182,6 +182,36 @@ __device__ __forceinline__ float cluster_sum1(uint32_t at, int ranks) {
     if (q < ranks) s += v[q];
   return s;
 }
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\t"
+      "mapa.shared::cluster.u32 ra, %4, %5;\n\t"
+      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [ra];\n\t}\n"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(addr), "r"(rank)
+      : "memory");
+  return v;
+}
+
+// The sum of four floats at one shared-memory offset over the cluster's first
+// `ranks` (2, 4 or 8) CTAs, in rank order, all loads in flight together.
+__device__ __forceinline__ float4 cluster_sum4(uint32_t at, int ranks) {
+  float4 v[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    if (q < ranks) v[q] = ld_cluster_f4(at, q);
+  float4 s = v[0];
+#pragma unroll
+  for (int q = 1; q < 8; ++q)
+    if (q < ranks) {
+      s.x += v[q].x;
+      s.y += v[q].y;
+      s.z += v[q].z;
+      s.w += v[q].w;
+    }
+  return s;
+}
 
 // ------------------------------------------------------------------ TMA
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar,

@@ -354,6 +354,40 @@ def test_long_sums_and_repeats(nrp, m, k, n):
     assert (off <= d.abs().sum(0) * (m + 16) * U).all()
 
 
+@pytest.mark.parametrize("m,k,n", [(33, 1024, 1024), (64, 4096, 1024), (100, 1040, 200),
+                                   (129, 2176, 1040), (200, 4224, 136), (600, 4096, 1024),
+                                   (896, 2064, 1000), (1100, 4096, 1024)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_shared_reductions(nrp, m, k, n, dtype):
+    """Few tiles and a long reduction, which several CTAs share: the rows,
+    columns and blocks at the ends, the bias added once, the same bits in every
+    run, and nothing written behind the last row."""
+    import torch
+    dt = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    u = 2.0 ** -8 if dt == torch.bfloat16 else U
+    g = torch.Generator(device="cuda").manual_seed(m + k)
+    x = nrp.fp8_quantize(torch.randn(m, k, device="cuda", generator=g))
+    w = nrp.fp8_quantize(torch.randn(n, k, device="cuda", generator=g) / math.sqrt(k), 128)
+    bias = torch.randn(n, device="cuda", generator=g).to(dt)
+    # the same reduction for the input's gradient: w [k, n] there
+    n16 = n // 16 * 16
+    wt = nrp.fp8_quantize(torch.randn(k, n16, device="cuda", generator=g) / math.sqrt(k), 128)
+    held = torch.full((m + 1, n), 7.0, device="cuda", dtype=dt)
+    y = nrp.fp8_linear(x, w, bias, dtype=dt, out=held[:m])
+    dx = nrp.fp8_linear_input_grad(x, wt, dtype=dt)
+    for _ in range(5):
+        assert torch.equal(nrp.fp8_linear(x, w, bias, dtype=dt), y)
+        assert torch.equal(nrp.fp8_linear_input_grad(x, wt, dtype=dt), dx)
+    assert (held[m] == 7).all()
+    xv = device_values(x)
+    for got, b, add in ((y, device_values(w).t(), bias.double()), (dx, device_values(wt), None)):
+        ref, size = xv @ b, xv.abs() @ b.abs()
+        if add is not None:
+            ref, size = ref + add, size + add.abs()
+        off = (got.double() - ref).abs()
+        assert (off <= size * (132 * 2.0 ** -23 + (k // 128 + 5) * U) + ref.abs() * u).all()
+
+
 def test_repeatable(nrp):
     """Two calls on the same inputs give the same bits."""
     import torch
