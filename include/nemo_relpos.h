@@ -598,6 +598,8 @@ int nrp_qlinear(nrp_context* ctx, void* stream, const void* x, int M, int K, con
  * codes 16-byte aligned.  All matrices are contiguous.  `dtype` is the type
  * of the unquantised operands and outputs (NRP_DTYPE_F32 or _BF16); sums are
  * f32.  A matrix without rows is allowed; its pointers are not looked at.
+ * Every pointer is aligned to its elements (to 16 bytes where a call says so);
+ * no output overlaps another argument, unless a call says so.
  * These calls allocate nothing and use no buffers but their arguments,
  * so calls and captured graphs on different streams do not share state. */
 
@@ -649,8 +651,7 @@ int nrp_layer_norm_backward_workspace(int64_t rows, int cols, int64_t* bytes);
  * their values stand in for it, with the mean and rstd given.  workspace:
  * device memory of at least nrp_layer_norm_backward_workspace bytes, 16-byte
  * aligned, not shared with work that may run at the same time; unused
- * without dgamma.  dx must not overlap x or dy.  rows == 0 gives zero dgamma
- * and dbeta. */
+ * without dgamma.  rows == 0 gives zero dgamma and dbeta. */
 int nrp_layer_norm_backward(nrp_context* ctx, void* stream, int dtype, const void* x,
                             const float* x_scales, const void* dy, const float* mean,
                             const float* rstd, const float* gamma, int64_t rows, int cols,

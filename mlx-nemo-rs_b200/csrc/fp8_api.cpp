@@ -2,6 +2,8 @@
 // and the LayerNorm's forward and backward pass (include/nemo_relpos.h).
 #include <cuda_runtime.h>
 
+#include <initializer_list>
+
 #include "../../include/nemo_relpos.h"
 #include "fp8.h"
 #include "handles.h"
@@ -41,6 +43,56 @@ int check_codes(const char* name, const void* codes, const void* scales, int64_t
   return NRP_OK;
 }
 
+int64_t elem(int dtype) { return dtype == NRP_DTYPE_BF16 ? 2 : 4; }
+int64_t scale_bytes(int64_t rows, int64_t cols, int block_rows) {
+  return 4 * (block_rows == 1 ? rows : nrp::qblocks(rows)) * nrp::qblocks(cols);
+}
+
+// An argument's bytes and the alignment that its loads and stores need.
+struct Span {
+  const char* name;
+  const void* p;
+  int64_t bytes;
+  int64_t align;
+};
+// Every argument is aligned, and no output overlaps another argument (the
+// kernels read inputs while they write outputs).
+int check_spans(const char* what, std::initializer_list<Span> outputs,
+                std::initializer_list<Span> inputs) {
+  for (const auto& list : {outputs, inputs})
+    for (const Span& s : list)
+      if (s.bytes > 0 && !aligned(s.p, static_cast<size_t>(s.align)))
+        return failf(NRP_ERR_INVALID, "%s: %s must be %lld-byte aligned", what, s.name,
+                     static_cast<long long>(s.align));
+  auto meet = [](const Span& a, const Span& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return x && y && a.bytes > 0 && b.bytes > 0 && x < y + static_cast<uintptr_t>(b.bytes) &&
+           y < x + static_cast<uintptr_t>(a.bytes);
+  };
+  for (const Span* o = outputs.begin(); o != outputs.end(); ++o) {
+    for (const Span* q = o + 1; q != outputs.end(); ++q)
+      if (meet(*o, *q))
+        return failf(NRP_ERR_INVALID, "%s: %s and %s overlap", what, o->name, q->name);
+    for (const Span& i : inputs)
+      if (meet(*o, i)) return failf(NRP_ERR_INVALID, "%s: %s and %s overlap", what, o->name, i.name);
+  }
+  return NRP_OK;
+}
+
+// The arguments of a product [M, R] x weight [wr, wc].
+int check_product(const char* what, int dtype, const void* x, const uint8_t* xq, const float* xs,
+                  int64_t M, int64_t R, const uint8_t* wq, const float* ws, int64_t wr, int64_t wc,
+                  const void* bias, const void* y, int64_t NO) {
+  const int64_t es = elem(dtype), n = M * R, sb = scale_bytes(M, R, 1);
+  const Span out{"the output", y, M * NO * es, es};
+  const Span w{"the weight's codes", wq, wr * wc, 16};
+  const Span wsc{"the weight's scales", ws, scale_bytes(wr, wc, 128), 4};
+  const Span b{"bias", bias, NO * es, es};
+  if (!x) return check_spans(what, {out}, {{"codes", xq, n, 16}, {"scales", xs, sb, 4}, w, wsc, b});
+  return check_spans(what, {out, {"codes", xq, n, 16}, {"scales", xs, sb, 4}},
+                     {{"the input", x, n * es, 16}, w, wsc, b});
+}
+
 // Quantises x (when given) into xq, xs and multiplies by the weight.
 int product(nrp_context* ctx, cudaStream_t st, bool trans, int dtype, const void* x, uint8_t* xq,
             float* xs, int M, int R, const uint8_t* wq, const float* ws, int NO, const void* bias,
@@ -78,7 +130,11 @@ int nrp_fp8_quantize(nrp_context* ctx, void* stream, int dtype, const void* x, i
   if (block_rows != 1 && block_rows != 128)
     return failf(NRP_ERR_UNSUPPORTED, "block_rows %d (supported: 1, 128)", block_rows);
   if (int rc = check_codes("quantize", codes, scales, cols, rows == 0)) return rc;
-  if (!aligned(x, 16)) return failf(NRP_ERR_INVALID, "the input must be 16-byte aligned");
+  if (int rc = check_spans("quantize",
+                           {{"codes", codes, rows * cols, 16},
+                            {"scales", scales, scale_bytes(rows, cols, block_rows), 4}},
+                           {{"the input", x, rows * cols * elem(dtype), 16}}))
+    return rc;
   if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   ProfScope ps(ctx, NRP_KERNEL_FP8_QUANT, st);
@@ -95,7 +151,10 @@ int nrp_fp8_dequantize(nrp_context* ctx, void* stream, const uint8_t* codes, con
   if (block_rows != 1 && block_rows != 128)
     return failf(NRP_ERR_UNSUPPORTED, "block_rows %d (supported: 1, 128)", block_rows);
   if (int rc = check_codes("dequantize", codes, scales, cols, rows == 0)) return rc;
-  if (!aligned(x, 16)) return failf(NRP_ERR_INVALID, "the output must be 16-byte aligned");
+  if (int rc = check_spans("dequantize", {{"the output", x, rows * cols * elem(dtype), 16}},
+                           {{"codes", codes, rows * cols, 16},
+                            {"scales", scales, scale_bytes(rows, cols, block_rows), 4}}))
+    return rc;
   if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   ProfScope ps(ctx, NRP_KERNEL_FP8_QUANT, st);
@@ -112,7 +171,8 @@ int nrp_fp8_linear(nrp_context* ctx, void* stream, int dtype, const void* x, uin
   if (int rc = check_dtype(dtype)) return rc;
   if (int rc = check_codes("fp8 linear: input", xq, xs, K, M == 0)) return rc;
   if (int rc = check_codes("fp8 linear: weight", wq, ws, K)) return rc;
-  if (!aligned(x, 16)) return failf(NRP_ERR_INVALID, "the input must be 16-byte aligned");
+  if (int rc = check_product("fp8 linear", dtype, x, xq, xs, M, K, wq, ws, N, K, bias, y, N))
+    return rc;
   if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
   return product(ctx, static_cast<cudaStream_t>(stream), false, dtype, x, xq, xs, M, K, wq, ws, N,
                  bias, y);
@@ -126,7 +186,9 @@ int nrp_fp8_linear_input_grad(nrp_context* ctx, void* stream, int dtype, const v
   if (int rc = check_dtype(dtype)) return rc;
   if (int rc = check_codes("fp8 input gradient: output gradient", gq, gs, N, M == 0)) return rc;
   if (int rc = check_codes("fp8 input gradient: weight", wq, ws, K)) return rc;
-  if (!aligned(dy, 16)) return failf(NRP_ERR_INVALID, "the output gradient must be 16-byte aligned");
+  if (int rc = check_product("fp8 input gradient", dtype, dy, gq, gs, M, N, wq, ws, N, K, nullptr,
+                             dx, K))
+    return rc;
   if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
   return product(ctx, static_cast<cudaStream_t>(stream), true, dtype, dy, gq, gs, M, N, wq, ws, K,
                  nullptr, dx);
@@ -141,7 +203,13 @@ int nrp_fp8_linear_weight_grad(nrp_context* ctx, void* stream, const void* dy, c
   if (int rc = check_codes("fp8 weight gradient: input", xq, xs, K, M == 0)) return rc;
   if (N % 8)
     return failf(NRP_ERR_UNSUPPORTED, "fp8 weight gradient: N = %d (needs a multiple of 8)", N);
-  if (!aligned(dy, 16)) return failf(NRP_ERR_INVALID, "the output gradient must be 16-byte aligned");
+  const int64_t es = elem(dtype), n = N, k = K;
+  if (int rc = check_spans("fp8 weight gradient",
+                           {{"dw", dw, n * k * es, es}, {"dbias", dbias, n * es, es}},
+                           {{"dy", dy, M * n * 2, 16},
+                            {"codes", xq, M * k, 16},
+                            {"scales", xs, scale_bytes(M, k, 1), 4}}))
+    return rc;
   if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   ProfScope ps(ctx, NRP_KERNEL_FP8_WGRAD, st);
@@ -158,6 +226,13 @@ int nrp_layer_norm(nrp_context* ctx, void* stream, int dtype, const void* x, int
   if (rows && !mean != !rstd) return failf(NRP_ERR_INVALID, "layer norm: mean and rstd go together");
   if (!(eps >= 0.f)) return failf(NRP_ERR_INVALID, "layer norm: eps must not be negative");
   if (int rc = check_dtype(dtype)) return rc;
+  const int64_t es = elem(dtype), bytes = rows * cols * es, vec = 4 * static_cast<int64_t>(cols);
+  if (int rc = check_spans("layer norm",
+                           {{"the output", y, bytes, es}, {"mean", mean, rows * 4, 4},
+                            {"rstd", rstd, rows * 4, 4}},
+                           {{"the input", x == y ? nullptr : x, bytes, es}, {"gamma", gamma, vec, 4},
+                            {"beta", beta, vec, 4}}))
+    return rc;
   if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   ProfScope ps(ctx, NRP_KERNEL_LAYERNORM, st);
@@ -183,13 +258,23 @@ int nrp_layer_norm_backward(nrp_context* ctx, void* stream, int dtype, const voi
   if (int rc = check_dtype(dtype)) return rc;
   if (x_scales)
     if (int rc = check_codes("layer norm backward: input", x, x_scales, cols)) return rc;
-  if (dgamma) {
-    const int64_t need = 4 * nrp::norm_bwd_partials(rows, cols);
-    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+  const int64_t need = dgamma ? 4 * nrp::norm_bwd_partials(rows, cols) : 0;
+  if (need) {
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
       return failf(NRP_ERR_INVALID,
                    "layer norm backward: workspace of %lld bytes (16-byte aligned) needed, got %lld",
                    static_cast<long long>(need), static_cast<long long>(workspace_bytes));
   }
+  const int64_t es = elem(dtype), n = rows * cols, vec = 4 * static_cast<int64_t>(cols);
+  if (int rc = check_spans(
+          "layer norm backward",
+          {{"dx", dx, n * es, es}, {"dgamma", dgamma, vec, 4}, {"dbeta", dbeta, vec, 4},
+           {"workspace", dgamma ? workspace : nullptr, need, 4}},
+          {{"the input", x, x_scales ? n : n * es, x_scales ? 16 : es},
+           {"scales", x_scales, x_scales ? scale_bytes(rows, cols, 1) : 0, 4},
+           {"dy", dy, n * es, es}, {"mean", mean, rows * 4, 4}, {"rstd", rstd, rows * 4, 4},
+           {"gamma", gamma, vec, 4}}))
+    return rc;
   if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   ProfScope ps(ctx, NRP_KERNEL_LAYERNORM_BWD, st);

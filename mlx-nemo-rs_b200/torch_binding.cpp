@@ -115,7 +115,7 @@ Tensor output(const char* name, PyObject* out, at::IntArrayRef shape, ScalarType
   return t;
 }
 
-bool is_fp8(PyObject* o) { return PyObject_TypeCheck(o, g_fp8); }
+bool is_fp8(PyObject* o) { return PyObject_TypeCheck(o, g_fp8) && PyTuple_GET_SIZE(o) == 3; }
 struct Codes {
   const Tensor* codes;
   uint8_t* q;
@@ -182,15 +182,18 @@ void* stream_of(int dev) {
 // it was (the library makes the context's current).
 template <typename F>
 void call(int dev, F&& f) {
+  struct Unlocked {
+    PyThreadState* save = PyEval_SaveThread();
+    ~Unlocked() { PyEval_RestoreThread(save); }  // also when a CUDA call throws
+  };
   int rc;
   std::string msg;
   {
-    PyThreadState* save = PyEval_SaveThread();
+    Unlocked unlocked;
     const auto current = c10::cuda::current_device();
     rc = f();
     if (rc < 0) msg = nrp_last_error();
     if (current != dev) c10::cuda::set_device(current);
-    PyEval_RestoreThread(save);
   }
   if (rc < 0) fail(msg, rc);
 }

@@ -177,3 +177,66 @@ def test_python_refusals(nrp):
         nrp.layer_norm(x, torch.ones(64), torch.zeros(64))
     with pytest.raises(nrp.NrpError):
         nrp.fp8_linear(x, (x, x, 128))  # not an Fp8Tensor
+
+
+# Arguments far apart, named by their place in the call: (function, arguments,
+# outputs, inputs, element size of each).
+AT = [0x10000000 * i for i in range(1, 12)]
+CALLS = {
+    "quantize": ("nrp_fp8_quantize", lambda a, p: [p, None, BF16, a["x"], 64, 256, 1, a["codes"],
+                                                   a["scales"]],
+                 {"codes": 16, "scales": 4}, {"x": 16}),
+    "dequantize": ("nrp_fp8_dequantize", lambda a, p: [p, None, a["codes"], a["scales"], 64, 256, 1,
+                                                       F32, a["x"]],
+                   {"x": 16}, {"codes": 16, "scales": 4}),
+    "linear": ("nrp_fp8_linear", lambda a, p: [p, None, BF16, a["x"], a["xq"], a["xs"], 64, 256,
+                                               a["wq"], a["ws"], 512, a["bias"], a["y"]],
+               {"y": 2, "xq": 16, "xs": 4}, {"x": 16, "wq": 16, "ws": 4, "bias": 2}),
+    "linear of codes": ("nrp_fp8_linear", lambda a, p: [p, None, F32, None, a["xq"], a["xs"], 64,
+                                                        256, a["wq"], a["ws"], 512, a["bias"],
+                                                        a["y"]],
+                        {"y": 4}, {"xq": 16, "xs": 4, "wq": 16, "ws": 4, "bias": 4}),
+    "input gradient": ("nrp_fp8_linear_input_grad",
+                       lambda a, p: [p, None, BF16, a["x"], a["xq"], a["xs"], 64, 256, a["wq"],
+                                     a["ws"], 512, a["y"]],
+                       {"y": 2, "xq": 16, "xs": 4}, {"x": 16, "wq": 16, "ws": 4}),
+    "weight gradient": ("nrp_fp8_linear_weight_grad",
+                        lambda a, p: [p, None, a["dy"], a["xq"], a["xs"], 64, 256, 512, F32,
+                                      a["dw"], a["db"]],
+                        {"dw": 4, "db": 4}, {"dy": 16, "xq": 16, "xs": 4}),
+    "norm": ("nrp_layer_norm", lambda a, p: [p, None, BF16, a["x"], 64, 256, a["gamma"], a["beta"],
+                                             C.c_float(1e-5), a["y"], a["mean"], a["rstd"]],
+             {"y": 2, "mean": 4, "rstd": 4}, {"x": 2, "gamma": 4, "beta": 4}),
+    "norm backward": ("nrp_layer_norm_backward",
+                      lambda a, p: [p, None, BF16, a["x"], None, a["dy"], a["mean"], a["rstd"],
+                                    a["gamma"], 1000, 256, a["dx"], a["dg"], a["db"], a["ws"],
+                                    1 << 24],
+                      {"dx": 2, "dg": 4, "db": 4, "ws": 16},
+                      {"x": 2, "dy": 2, "mean": 4, "rstd": 4, "gamma": 4}),
+    "norm backward of codes": ("nrp_layer_norm_backward",
+                               lambda a, p: [p, None, F32, a["x"], a["xs"], a["dy"], a["mean"],
+                                             a["rstd"], a["gamma"], 64, 256, a["dx"], a["dg"],
+                                             a["db"], None, 0],
+                               {"dx": 4, "dg": 4, "db": 4},
+                               {"x": 16, "xs": 4, "dy": 4, "mean": 4, "rstd": 4, "gamma": 4}),
+}
+
+
+@pytest.mark.parametrize("name", sorted(CALLS))
+def test_overlaps_and_alignment(nrp, mem, name):
+    """An output at the place of an input or of another output, and any argument off its alignment, is refused."""
+    p, _ = mem
+    fn, call, outs, ins = CALLS[name]
+    place = dict(zip(list(outs) + list(ins), AT))
+    for o in outs:
+        for other in list(outs) + list(ins):
+            if other == o:
+                continue
+            if name == "norm" and (o, other) == ("y", "x"):  # in place, but not shifted
+                refused(nrp, INVALID, fn, *call(dict(place, y=place["x"] + 16), p))
+            else:
+                refused(nrp, INVALID, fn, *call(dict(place, **{o: place[other]}), p))
+                assert "overlap" in nrp.lib().nrp_last_error().decode()
+    for arg, align in {**outs, **ins}.items():
+        refused(nrp, INVALID, fn, *call(dict(place, **{arg: place[arg] + align // 2}), p))
+        assert "aligned" in nrp.lib().nrp_last_error().decode()
