@@ -19,8 +19,8 @@
 //
 // Measured: forward, 50000 x 1024 bf16 36 us (5.7 TB/s; a plain copy of that
 // size runs at 6.2), 14 x 512 f32 2.9 us; backward of 50000 x 1024 from bf16 dy
-// and codes 59 us with its second kernel (4.4 TB/s: two batches of rows in 128
-// registers do not cover the latency fully), 749 x 512 bf16 6.4 us.
+// and codes 49 us with its second kernel (5.2 TB/s; instruction issue, at 60%,
+// comes close to being the bound), 749 x 512 bf16 6.4 us in two launches.
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -390,32 +390,36 @@ __global__ void __launch_bounds__(256)
 // Groups of W warps and strips of columns as in the forward pass: dgamma and
 // dbeta cost a lane 16 registers whatever the width.  The rows' two sums cross
 // the warps of a group through shared memory.
-constexpr int kRows = 2;  // 2 kRows kStripWarps <= 32 lanes
-constexpr int kFewRows = 256;          // up to here one cluster takes all rows
+// A batch is kR rows: 2, or 4 where the rows wait in shared memory (bf16 dy,
+// 16-byte copies, W <= 4: 2 kR W <= 32 lanes when the strips are joined).
+constexpr int kRingWarps = 4;
+// Up to here one cluster takes all rows, in one launch: bf16 64 x 1024 5.6 us
+// (host 5.8) against 5.5 us (host 8.2) in two, 200 x 1024 8.4 against 6.2.
+constexpr int kFewRows = 64;
 constexpr int kFewThreads = 512;       // threads of its CTAs
 constexpr int kManyThreads = 256;
 constexpr int kManyParts = 2 * 148;    // CTAs of the persistent grid at most
 
-// Partial rows of dgamma | dbeta that go through the workspace (0: none).
+// The most partial rows of dgamma | dbeta that go through the workspace (0: none).
 int norm_parts(int64_t rows, int cols) {
   if (cols > kStripCols) return static_cast<int>(std::min<int64_t>((rows + 7) / 8, kManyParts));
   if (rows <= kFewRows) return 0;
-  const int per = strip_groups(cols, kManyThreads) * kRows;
+  const int per = strip_groups(cols, kManyThreads) * 2;
   return static_cast<int>(std::min<int64_t>((rows + per - 1) / per, kManyParts));
 }
 
-// kRows rows of a lane's strip on their way.
-template <typename T, typename TX, bool kVec>
+// kR rows of a lane's strip.
+template <typename T, typename TX, bool kVec, int kR>
 struct Batch {
   static constexpr int kScales = sizeof(TX) == 1 ? (kVec ? 1 : 2) : 0;
-  Strip<TX, kVec> x[kRows];
-  Strip<T, kVec> dy[kRows];
-  float mu[kRows], rs[kRows], sx[kRows][kScales ? kScales : 1];
+  Strip<TX, kVec> x[kR];
+  Strip<T, kVec> dy[kR];
+  float mu[kR], rs[kR], sx[kR][kScales ? kScales : 1];
   __device__ __forceinline__ void load(const TX* px, const float* xs, const T* pdy,
                                        const float* mean, const float* rstd, int64_t row0,
                                        int64_t rows, int cols, int cb, int col) {
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
+    for (int r = 0; r < kR; ++r) {
       const int64_t row = row0 + r;
       mu[r] = rs[r] = 0.f;
 #pragma unroll
@@ -437,18 +441,75 @@ struct Batch {
   }
 };
 
+// The ring of the rows on their way: kDepth batches, each thread its own columns
+// in its own places ([piece][thread], no barrier), a warp the rows' mean, rstd
+// and scales in 16 floats.  It frees the registers that the next batch takes
+// otherwise for four rows at a time, which share the reductions, the barrier and
+// the addresses: those are two thirds of the instructions (50000 x 1024, bf16
+// dy and codes: 59.5 us with two rows in registers and their next on the way, 56.5
+// with two rows and this ring, 49.2 with four; 50.3 three batches deep).  f32 runs
+// at the rate of a copy with two rows in registers (100 us; 161 with this ring).
+template <typename T, typename TX, int kR>
+struct Ring {
+  static constexpr int kDepth = 2;
+  static constexpr int kBytes = kR * 8 * static_cast<int>(sizeof(T) + sizeof(TX));  // per thread
+  static constexpr int kSlot = kManyThreads * kBytes + kManyThreads / 32 * 64;
+};
+template <int kN>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool read) {
+  const int n = read ? kN : 0;  // else zeros
+  if constexpr (kN == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
+                 : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kN),
+                 "r"(n)
+                 : "memory");
+}
+// Eight elements of a row into thread-strided pieces of up to 16 bytes.
+template <typename E>
+__device__ __forceinline__ uint32_t copy_strip(uint32_t at, int threads, const E* p, bool read) {
+  constexpr int kAll = 8 * static_cast<int>(sizeof(E)), kPiece = kAll < 16 ? kAll : 16;
+#pragma unroll
+  for (int i = 0; i < kAll / kPiece; ++i) {
+    copy_async<kPiece>(at + threadIdx.x * kPiece, reinterpret_cast<const uint8_t*>(p) + i * kPiece,
+                       read);
+    at += threads * kPiece;
+  }
+  return at;
+}
+template <typename E>
+__device__ __forceinline__ const uint8_t* take_strip(const uint8_t* at, int threads,
+                                                     Strip<E, true>& s) {
+  constexpr int kAll = 8 * static_cast<int>(sizeof(E)), kPiece = kAll < 16 ? kAll : 16;
+#pragma unroll
+  for (int i = 0; i < kAll / kPiece; ++i) {
+    if constexpr (kPiece == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(at + threadIdx.x * 8);
+      s.w[0] = v.x, s.w[1] = v.y;
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(at + threadIdx.x * 16);
+      s.w[4 * i] = v.x, s.w[4 * i + 1] = v.y, s.w[4 * i + 2] = v.z, s.w[4 * i + 3] = v.w;
+    }
+    at += threads * kPiece;
+  }
+  return at;
+}
+
 // blockDim.x = 32 * W * groups.  partials [gridDim.x][2][cols], or null: the
 // grid is one cluster, and dgamma and dbeta (null: not wanted) are written.
-template <typename T, typename TX, bool kVec, int kThreads>
+template <typename T, typename TX, bool kVec, int kThreads, int kR>
 __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
     norm_bwd_kernel(const TX* __restrict__ x, const float* __restrict__ xs,
                     const T* __restrict__ dy, const float* __restrict__ mean,
                     const float* __restrict__ rstd, const float* __restrict__ gamma, int64_t rows,
                     int cols, int W, T* __restrict__ dx, float* __restrict__ partials,
                     float* __restrict__ dgamma, float* __restrict__ dbeta) {
-  constexpr bool kCodes = sizeof(TX) == 1;
-  extern __shared__ float col_sums[];  // [groups][2][cols]
-  __shared__ float red[2][kThreads / 32][2 * kRows];
+  constexpr bool kCodes = sizeof(TX) == 1, kRing = kR == 4;
+  // the ring of rows, then [groups][2][cols] column sums
+  extern __shared__ __align__(16) uint8_t norm_smem[];
+  float* col_sums = reinterpret_cast<float*>(norm_smem);
+  __shared__ float red[2][kThreads / 32][2 * kR];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int strip = warp % W, grp = warp / W, groups = static_cast<int>(blockDim.x) / 32 / W;
   const int col = strip * 256 + (kVec ? lane * 8 : lane);
@@ -457,10 +518,37 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
   const int cb = (cols + kQBlock - 1) / kQBlock;
   const float inv_c = 1.f / static_cast<float>(cols);
   const int Wp = strips_pow2(W), at_w = lane % Wp, at_i = lane / Wp;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * groups * kRows;
-  int64_t row0 = (static_cast<int64_t>(blockIdx.x) * groups + grp) * kRows;
-  Batch<T, TX, kVec> next;
-  next.load(x, xs, dy, mean, rstd, row0, rows, cols, cb, col);
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * groups * kR;
+  int64_t row0 = (static_cast<int64_t>(blockIdx.x) * groups + grp) * kR;
+  using Rg = Ring<T, TX, kR>;
+  const uint32_t ring = smem_u32(norm_smem);
+  const bool in = col < cols;
+  auto issue = [&](int slot, int64_t r0) {
+    uint32_t at = ring + slot * Rg::kSlot;
+    // lanes 0..3: mean, 4..7: rstd, then the scales of the strip's two blocks
+    const int64_t row = r0 + (lane & 3);
+    const int blk = strip * 2 + ((lane >> 2) & 1);
+    const float* src = lane < 4 ? mean + row : lane < 8 ? rstd + row : xs + row * cb + blk;
+    const bool read = row < rows && (lane < 8 || blk < cb);
+    if (lane < (kCodes ? 16 : 8))
+      copy_async<4>(at + kThreads * Rg::kBytes + warp * 64 + lane * 4, read ? src : mean, read);
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      const bool get = in && r0 + r < rows;
+      const int64_t off = get ? (r0 + r) * cols + col : 0;
+      at = copy_strip(at, kThreads, x + off, get);
+      at = copy_strip(at, kThreads, dy + off, get);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  int slot = 0;
+  [[maybe_unused]] Batch<T, TX, kVec, kR> next;
+  if constexpr (kRing) {
+#pragma unroll
+    for (int d = 0; d < Rg::kDepth - 1; ++d) issue(d, row0 + d * stride);
+  } else {
+    next.load(x, xs, dy, mean, rstd, row0, rows, cols, cb, col);
+  }
   F2 ag[4], ab[4], gm[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -470,12 +558,30 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
   }
   int buf = 0;
   for (; row0 < rows; row0 += stride, buf ^= 1) {
-    const Batch<T, TX, kVec> now = next;
-    next.load(x, xs, dy, mean, rstd, row0 + stride, rows, cols, cb, col);
-    F2 u[kRows][4], g[kRows][4];
-    float part[2 * kRows];
+    Batch<T, TX, kVec, kR> now;
+    if constexpr (kRing) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(Rg::kDepth - 2) : "memory");
+      __syncwarp();  // the warp's floats are there; the slot before has been read
+      issue(slot == 0 ? Rg::kDepth - 1 : slot - 1, row0 + (Rg::kDepth - 1) * stride);
+      const uint8_t* at = norm_smem + slot * Rg::kSlot;
+      const float* of_warp = reinterpret_cast<const float*>(at + kThreads * Rg::kBytes) + warp * 16;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
+      for (int r = 0; r < kR; ++r) {
+        now.mu[r] = of_warp[r];
+        now.rs[r] = of_warp[4 + r];
+        if constexpr (kCodes) now.sx[r][0] = of_warp[8 + r + 4 * (lane >> 4)];
+        at = take_strip(at, kThreads, now.x[r]);
+        at = take_strip(at, kThreads, now.dy[r]);
+      }
+      slot = slot == Rg::kDepth - 1 ? 0 : slot + 1;
+    } else {
+      now = next;
+      next.load(x, xs, dy, mean, rstd, row0 + stride, rows, cols, cb, col);
+    }
+    F2 u[kR][4], g[kR][4];
+    float part[2 * kR];
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
       F2 c1 = both(0.f), c2 = both(0.f);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -496,30 +602,30 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
         c2 = fma2(g[r][e], u[r][e], c2);
       }
       part[r] = c1.a + c1.b;
-      part[kRows + r] = c2.a + c2.b;
+      part[kR + r] = c2.a + c2.b;
     }
     // lanes past the columns hold x = 0 and dy = 0: nothing but zeros added
     const float mine = warp_sums(part, lane);
-    constexpr int kHold = 16 / kRows;  // lanes that hold each sum
-    float s[2 * kRows];
+    constexpr int kHold = 16 / kR;  // lanes that hold each sum
+    float s[2 * kR];
     if (W == 1) {
 #pragma unroll
-      for (int i = 0; i < 2 * kRows; ++i) s[i] = __shfl_sync(0xffffffffu, mine, kHold * i);
+      for (int i = 0; i < 2 * kR; ++i) s[i] = __shfl_sync(0xffffffffu, mine, kHold * i);
     } else {
       if (lane % kHold == 0) red[buf][warp][lane / kHold] = mine;
       named_bar_sync(1 + grp, 32 * W);
       // lane (i, w) takes strip w's share of sum i
-      float t = at_w < W && at_i < 2 * kRows ? red[buf][grp * W + at_w][at_i] : 0.f;
+      float t = at_w < W && at_i < 2 * kR ? red[buf][grp * W + at_w][at_i] : 0.f;
       for (int o = Wp / 2; o; o /= 2) t += __shfl_xor_sync(0xffffffffu, t, o);
 #pragma unroll
-      for (int i = 0; i < 2 * kRows; ++i) s[i] = __shfl_sync(0xffffffffu, t, Wp * i);
+      for (int i = 0; i < 2 * kR; ++i) s[i] = __shfl_sync(0xffffffffu, t, Wp * i);
     }
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
+    for (int r = 0; r < kR; ++r) {
       if (row0 + r >= rows) break;
       // dx = rstd g - rstd mean(g) - u rstd mean(g u)
       const float rs = now.rs[r];
-      const F2 k0 = both(-rs * (s[r] * inv_c)), k2 = both(-rs * (s[kRows + r] * inv_c));
+      const F2 k0 = both(-rs * (s[r] * inv_c)), k2 = both(-rs * (s[kR + r] * inv_c));
       float o[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -530,7 +636,9 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
       store_strip<T, kVec>(dx + (row0 + r) * cols, col, cols, o);
     }
   }
+  if constexpr (kRing) asm volatile("cp.async.wait_all;" ::: "memory");
   if (!partials && !dgamma) return;
+  if constexpr (kRing) __syncthreads();  // the sums take its place
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const int c0 = col + (kVec ? 2 * e : 64 * e), c1 = c0 + (kVec ? 1 : 32);
@@ -708,10 +816,12 @@ struct BwdArgs {
   float *dgamma, *dbeta, *partials;
 };
 
-template <typename T, typename TX, bool kVec, int kThreads>
-cudaError_t bwd_strips(const TX* x, const T* dy, T* dx, const BwdArgs& a, cudaStream_t stream) {
+// parts: the CTAs, which is the partial rows written.
+template <typename T, typename TX, bool kVec, int kThreads, int kR>
+cudaError_t bwd_strips(const TX* x, const T* dy, T* dx, const BwdArgs& a, int& parts,
+                       cudaStream_t stream) {
   const int W = strip_warps(a.cols), groups = strip_groups(a.cols, kThreads);
-  const int per = groups * kRows;
+  const int per = groups * kR;
   const int64_t batches = (a.rows + per - 1) / per;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute la[2];
@@ -731,26 +841,41 @@ cudaError_t bwd_strips(const TX* x, const T* dy, T* dx, const BwdArgs& a, cudaSt
     cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(batches, kManyParts)));
   }
   cfg.blockDim = dim3(32 * W * groups);
-  // groups * W <= 16 warps of 256 columns: 32 KB at most
-  cfg.dynamicSmemBytes = a.dgamma ? 8 * static_cast<size_t>(groups) * a.cols : 0;
+  parts = static_cast<int>(cfg.gridDim.x);
+  // groups * W <= 16 warps of 256 columns: 32 KB of sums at most
+  auto* kernel = norm_bwd_kernel<T, TX, kVec, kThreads, kR>;
+  const size_t sums = a.dgamma ? 8 * static_cast<size_t>(groups) * a.cols : 0;
+  cfg.dynamicSmemBytes = sums;
+  if constexpr (kR == 4) {
+    static std::atomic<uint64_t> attr{0};
+    constexpr int kSmem = std::max(Ring<T, TX, kR>::kDepth * Ring<T, TX, kR>::kSlot, 16384);
+    if (cudaError_t e = smem_attr_once(kernel, kSmem, attr)) return e;
+    cfg.dynamicSmemBytes = kSmem;
+  }
   cfg.stream = stream;
   cfg.attrs = la;
   float* partials = kThreads == kFewThreads ? nullptr : a.partials;
-  return cudaLaunchKernelEx(&cfg, norm_bwd_kernel<T, TX, kVec, kThreads>, x, a.xs, dy, a.mean,
+  return cudaLaunchKernelEx(&cfg, kernel, x, a.xs, dy, a.mean,
                             a.rstd, a.gamma, a.rows, a.cols, W, dx, partials, a.dgamma, a.dbeta);
 }
 
 template <typename T, typename TX>
 cudaError_t bwd(const TX* x, const T* dy, T* dx, const BwdArgs& a, cudaStream_t stream) {
   const bool vec = a.cols % 8 == 0 && aligned16(x) && aligned16(dy) && aligned16(dx);
-  const int parts = norm_parts(a.rows, a.cols);
+  int parts = norm_parts(a.rows, a.cols);
   cudaError_t e;
   if (a.cols <= kStripCols) {
     if (parts == 0)
-      return vec ? bwd_strips<T, TX, true, kFewThreads>(x, dy, dx, a, stream)
-                 : bwd_strips<T, TX, false, kFewThreads>(x, dy, dx, a, stream);
-    e = vec ? bwd_strips<T, TX, true, kManyThreads>(x, dy, dx, a, stream)
-            : bwd_strips<T, TX, false, kManyThreads>(x, dy, dx, a, stream);
+      return vec ? bwd_strips<T, TX, true, kFewThreads, 2>(x, dy, dx, a, parts, stream)
+                 : bwd_strips<T, TX, false, kFewThreads, 2>(x, dy, dx, a, parts, stream);
+    bool four = false;
+    if constexpr (sizeof(T) == 2) {
+      four = vec && strip_warps(a.cols) <= kRingWarps;
+      if (four) e = bwd_strips<T, TX, true, kManyThreads, 4>(x, dy, dx, a, parts, stream);
+    }
+    if (!four)
+      e = vec ? bwd_strips<T, TX, true, kManyThreads, 2>(x, dy, dx, a, parts, stream)
+              : bwd_strips<T, TX, false, kManyThreads, 2>(x, dy, dx, a, parts, stream);
   } else {
     const int grid = static_cast<int>(std::min<int64_t>(a.rows, 4 * kManyParts));
     e = launch_pdl(norm_bwd_wide_kernel<T, TX>, dim3(grid), dim3(256), 0, stream, x, a.xs, dy,
