@@ -34,7 +34,8 @@ int check_dtype(int dtype) {
 // One without rows may have null pointers (an empty tensor's).
 int check_codes(const char* name, const void* codes, const void* scales, int64_t cols,
                 bool empty = false) {
-  if (!empty && (!codes || !scales)) return failf(NRP_ERR_INVALID, "%s: null codes or scales", name);
+  if (!empty && (!codes || !scales))
+    return failf(NRP_ERR_INVALID, "%s: null codes or scales", name);
   if (cols % 16)
     return failf(NRP_ERR_UNSUPPORTED, "%s: %lld columns (codes need a multiple of 16)", name,
                  static_cast<long long>(cols));
@@ -74,7 +75,8 @@ int check_spans(const char* what, std::initializer_list<Span> outputs,
       if (meet(*o, *q))
         return failf(NRP_ERR_INVALID, "%s: %s and %s overlap", what, o->name, q->name);
     for (const Span& i : inputs)
-      if (meet(*o, i)) return failf(NRP_ERR_INVALID, "%s: %s and %s overlap", what, o->name, i.name);
+      if (meet(*o, i))
+        return failf(NRP_ERR_INVALID, "%s: %s and %s overlap", what, o->name, i.name);
   }
   return NRP_OK;
 }
@@ -223,15 +225,16 @@ int nrp_layer_norm(nrp_context* ctx, void* stream, int dtype, const void* x, int
                    float* mean, float* rstd) {
   if (!ctx || !gamma || !beta || (rows && (!x || !y)) || rows < 0 || cols <= 0)
     return failf(NRP_ERR_INVALID, "invalid layer norm arguments");
-  if (rows && !mean != !rstd) return failf(NRP_ERR_INVALID, "layer norm: mean and rstd go together");
+  if (rows && !mean != !rstd)
+    return failf(NRP_ERR_INVALID, "layer norm: mean and rstd go together");
   if (!(eps >= 0.f)) return failf(NRP_ERR_INVALID, "layer norm: eps must not be negative");
   if (int rc = check_dtype(dtype)) return rc;
   const int64_t es = elem(dtype), bytes = rows * cols * es, vec = 4 * static_cast<int64_t>(cols);
   if (int rc = check_spans("layer norm",
                            {{"the output", y, bytes, es}, {"mean", mean, rows * 4, 4},
                             {"rstd", rstd, rows * 4, 4}},
-                           {{"the input", x == y ? nullptr : x, bytes, es}, {"gamma", gamma, vec, 4},
-                            {"beta", beta, vec, 4}}))
+                           {{"the input", x == y ? nullptr : x, bytes, es},
+                            {"gamma", gamma, vec, 4}, {"beta", beta, vec, 4}}))
     return rc;
   if (nrp::select_device(ctx)) return NRP_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

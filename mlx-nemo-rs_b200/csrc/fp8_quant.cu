@@ -11,7 +11,10 @@
 // 119 keeps 448 * s finite).  NaN and infinities become the NaN code: e4m3
 // has no infinity, and a saturated one would hide an overflow.
 //
-// Both kernels are bound by HBM: they read and write each element once.
+// All are bound by HBM: they read and write each element once.  Measured: 16000
+// x 4096 bf16 by rows 32 us (6.2 TB/s, a plain copy's rate), 4096 x 1024 f32 by
+// 128 x 128 blocks 4.3 us (4.9 TB/s with the launch in it: 256 CTAs hold a block
+// each in registers between its maximum and its codes).
 #include "fp8.h"
 #include "fp8_quant.cuh"
 

@@ -7,11 +7,15 @@
 // where that gives more SMs work; its eight warps take every eighth 128-block.
 // A warp asks for its first block's codes, then the CTA quantises its part of x
 // (as every other CTA of that part: 14 x 1024 values, from L2) into shared
-// memory while they come, four blocks' loads in flight per lane.  mma.sync m16n8k32 takes the weight rows as the
-// 16-row operand and up to 8 tokens as the other; 64 consecutive codes of a row
-// are four lanes' 16-byte loads, the same permutation of k on both sides.  A
-// block's sum is scaled by its two scales and added in f32; the warps' partial
-// results meet in shared memory, the CTAs' in the cluster's.
+// memory while they come, four blocks' loads in flight per lane.  mma.sync
+// m16n8k32 takes the weight rows as the 16-row operand and up to 8 tokens as the
+// other (a tcgen05 tile has 128 rows, of which 14 would be used); 64 consecutive
+// codes of a row are four lanes' 16-byte loads, the same permutation of k on both
+// sides.  A block's sum is scaled by its two scales and added in f32; the warps'
+// partial results meet in shared memory, the CTAs' in the cluster's.
+//
+// Measured: 14 rows, 1024 to 4096, bf16 with bias 5.0 us (an empty kernel takes
+// 2.2), 0.8 TB/s of weight.
 #include <algorithm>
 
 #include "fp8.h"

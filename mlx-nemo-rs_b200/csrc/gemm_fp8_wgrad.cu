@@ -14,24 +14,26 @@
 // one column n is 32 consecutive k.
 //
 // The bf16 checkpoint never exists in HBM, and the codes are half its bytes.
-// The kernel is bound by the bf16 tensor rate.
 //
-// Tiles are 128 k x 256 n, one per CTA, or narrower for few tokens.  Where they do
-// not fill the SMs, a cluster of 2, 4 or 8 CTAs splits the tokens of one tile;
-// the partial tiles are summed in rank order through distributed shared memory,
-// so the result does not depend on timing and needs no workspace.  That sum costs
-// about 4 us for four partial 256-wide tiles, which narrower ones save at the
-// price of more conversion.  The bias' gradient is
-// summed from the dy tiles in shared memory, which all of a column's tiles
-// hold: each takes every tiles_k-th 8 columns, so that no CTA is the slowest.
+// Tiles are 128 k x 256 n, one per CTA, or narrower for few tokens.  Where they
+// do not fill the SMs, a cluster of 2, 4 or 8 CTAs splits the tokens of one
+// tile; the partial tiles are summed in rank order through distributed shared
+// memory, so the result does not depend on timing and needs no workspace.  That
+// sum costs about 4 us for four partial 256-wide tiles, which narrower ones save
+// at the price of more conversion.  The bias' gradient is summed from the dy
+// tiles in shared memory, which all of a column's tiles hold: each takes every
+// tiles_k-th 8 columns, so that no CTA is the slowest.
 //
-// Shared-memory traffic costs most: per 64 tokens 48 KB of MMA operands, 40 KB
-// of TMA writes and 24 KB of conversion, 896 cycles at 128 bytes each against
-// the tensor cores' 512.  Measured at 16000 x 4096 x 1024 with bias: 141 us, 0.95
-// PFLOP/s.  Tried and slower (then against 126 to 135): CTA pairs with 256 x 256 tiles (165, the hand-off of both CTAs'
-// conversions to one issuer), 512-wide tiles (145), the k0 = 0 tiles summing
-// all of the bias (170 to 195), CTAs of its own for the bias (133, but a
-// second wave of clusters at 1024 x 1024).
+// Bound by shared-memory traffic: per 64 tokens 48 KB of MMA operands, 40 KB of
+// TMA writes and 24 KB of conversion, 896 cycles at 128 bytes each against the
+// tensor cores' 512, which makes 121 us at 16000 x 4096 x 1024.  Measured there
+// with bias: 141 us, 0.95 PFLOP/s; 749 x 1024 x 1024 10.0 us.  TMEM holds a
+// segment's sums and the running ones (below), which leaves no room in it for
+// the converted operand.  Tried and slower (then against 126 to 135): CTA pairs
+// with 256 x 256 tiles (165, the hand-off of both CTAs' conversions to one
+// issuer), 512-wide tiles (145), the k0 = 0 tiles summing all of the bias (170 to
+// 195), CTAs of its own for the bias (133, but a second wave of clusters at 1024
+// x 1024).
 //
 // Warp roles (23 warps): 0 TMA producer of dy, 1 TMEM allocator and MMA
 // issuer, 2 TMA producer of the codes, 3..6 the bias, 7..22 dequantisation:
@@ -267,8 +269,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t idesc = idesc_bf16_f32(kTK, kTN, 1, 1);
     for (int i = 0; i < steps; ++i) {
       const int s = i % kStages;
-      if (*abort_flag || !warp_mbar_wait_hot(&ss->full[s], (i / kStages) & 1, a.err, kDevTimeoutLoad) ||
-          !warp_mbar_wait_hot(&ss->deq[s], (i / kStages) & 1, a.err, kDevTimeoutLoad)) {
+      const uint32_t parity = (i / kStages) & 1;
+      if (*abort_flag || !warp_mbar_wait_hot(&ss->full[s], parity, a.err, kDevTimeoutLoad) ||
+          !warp_mbar_wait_hot(&ss->deq[s], parity, a.err, kDevTimeoutLoad)) {
         *abort_flag = 1;
         break;
       }
@@ -305,7 +308,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < 8; ++e) sum[j][e] = 0.f;
       for (int i = 0; i < steps; ++i) {
         const int s = i % kStages;
-        if (*abort_flag || !mbar_wait_hot(&ss->full[s], (i / kStages) & 1, a.err, kDevTimeoutLoad)) {
+        if (*abort_flag ||
+            !mbar_wait_hot(&ss->full[s], (i / kStages) & 1, a.err, kDevTimeoutLoad)) {
           *abort_flag = 1;
           break;
         }

@@ -123,7 +123,8 @@ struct Codes {
   Size size;
 };
 // A valid Fp8Tensor with the given block rows (0: any).
-Codes codes_of(const char* name, PyObject* o, int64_t block_rows, int dev, int64_t* block = nullptr) {
+Codes codes_of(const char* name, PyObject* o, int64_t block_rows, int dev,
+               int64_t* block = nullptr) {
   if (!is_fp8(o)) fail(std::string(name) + ": an Fp8Tensor is needed");
   PyObject* b = PyTuple_GET_ITEM(o, 2);
   const int64_t br = PyLong_Check(b) ? PyLong_AsLongLong(b) : -1;
