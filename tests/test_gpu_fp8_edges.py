@@ -262,3 +262,27 @@ def test_offsets_past_32_bits(nrp):
     assert torch.equal(wide[-tail:], nrp.fp8_linear_input_grad(few, w))
     del wide
     torch.cuda.empty_cache()
+
+
+def test_statistics_and_sums_are_tensors_of_their_own(nrp):
+    """mean and rstd, dgamma and dbeta: their values stay when the other of the
+    pair is written or goes away, also for no rows, and autograd takes them."""
+    import torch
+    o = operands(nrp, 33, 256, 256, seed=2)
+    y, mean, rstd = nrp.layer_norm(o["x"].view(3, 11, 256), o["gamma"], o["beta"])
+    assert mean.shape == rstd.shape == (3, 11) and mean.is_contiguous() and rstd.is_contiguous()
+    keep = rstd.clone()
+    mean.zero_()
+    del mean
+    torch.full((4096,), 5.0, device="cuda")
+    assert torch.equal(rstd, keep)
+    dx, dg, db = nrp.layer_norm_backward(y, o["x"].view(3, 11, 256), rstd * 0, rstd, o["gamma"])
+    assert dg.shape == db.shape == (256,)
+    keep = db.clone()
+    dg.add_(1)
+    assert torch.equal(db, keep)
+    p = torch.ones(256, device="cuda", requires_grad=True)
+    (p * db).sum().backward()
+    assert torch.equal(p.grad, db)
+    e, mean, rstd = nrp.layer_norm(o["x"][:0], o["gamma"], o["beta"])
+    assert mean.shape == rstd.shape == (0,) and e.shape == (0, 256)
