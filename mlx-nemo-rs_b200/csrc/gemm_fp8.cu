@@ -26,8 +26,8 @@
 // into shared memory and 48 KB out of it for 256 cycles of MMA (768 at 128
 // bytes a cycle; measured 930), and the chip takes them from L2 at 11 TB/s.
 // Measured from codes to bf16: 16000 x 4096 to 1024 68 us (1.97 PFLOP/s; 3.4 waves
-// of tiles take four), 16000 x 1024 to 4096 80 us (the output is 131 MB of
-// it), 896 x 1024 to 1024 6.4 us.  Tried and slower: CTA pairs (256 x 256 tiles,
+// of tiles take four), 16000 x 1024 to 4096 with bias 78 us (9 of
+// them the output, 131 MB), 896 x 1024 to 1024 6.3 us.  Tried and slower: CTA pairs (256 x 256 tiles,
 // 76 us against 71: the hand-off over the cluster), sixteen epilogue warps (80
 // against 71), the last wave's tiles in halves (68.3 against 68.2).
 #include <algorithm>
@@ -52,6 +52,9 @@ constexpr int kChunk = 8, kScalePitch = kChunk + 1;
 constexpr int kScaleBuf = 32 * kScalePitch + kChunk;
 constexpr int kScaleFloats = 2 * kScaleBuf;
 
+// ... and its part of the bias, for the tile at hand and the next.
+constexpr uint32_t kBiasBytes = 128 * 4;
+
 // A split tile's partial sums: four more floats to a row, for the banks.
 constexpr int kPartPitch = 128 + 4;
 // A split spares each CTA at least this many blocks of the reduction: a cluster
@@ -64,7 +67,7 @@ struct Cfg {
   static constexpr int kBufs = 512 / kBN;  // accumulators in TMEM
   static constexpr uint32_t kBBytes = kBN * kBR;
   static constexpr size_t kSmem =
-      1024 + kStages * (kABytes + kBBytes) + 8 * (kSlabBytes + 4 * kScaleFloats) + 256;
+      1024 + kStages * (kABytes + kBBytes) + 8 * (kSlabBytes + 4 * kScaleFloats + 2 * kBiasBytes) + 256;
 };
 static_assert(Cfg<256>::kSmem <= 232448 && Cfg<128>::kSmem <= 232448,
               "shared memory budget");
@@ -138,7 +141,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sE = sB + kStages * kBBytes;
   float* sS = reinterpret_cast<float*>(sE + 8 * kSlabBytes);
   [[maybe_unused]] float* part = reinterpret_cast<float*>(sA);  // kSplit: [128][kPartPitch]
-  Bars* ss = reinterpret_cast<Bars*>(sS + 8 * kScaleFloats);
+  uint8_t* sBias = reinterpret_cast<uint8_t*>(sS + 8 * kScaleFloats);
+  Bars* ss = reinterpret_cast<Bars*>(sBias + 8 * 2 * kBiasBytes);
   const int warp = static_cast<int>(uniform(threadIdx.x >> 5)), lane = lane_id();
   const int tiles_m = (a.M + kBM - 1) / kBM;
   const int tiles_n = (a.NO + kBN - 1) / kBN;
@@ -253,8 +257,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     // before them are used.  (A load of each lane's own row per block, one block
     // ahead, touches 32 sectors an instruction: 16000 x 1024 x 4096 took 77 us
     // with it, 68 with these.)
-    auto prefetch = [&](int t, int c, int buf) {
+    // With a tile's first scales comes its bias, in 4-byte words where it lies so
+    // (loaded where it is added: 896 x 1024 to 4096 9.0 against 8.0 us, 16000 rows
+    // 78.9 against 77.7).
+    uint8_t* my_bias = sBias + (warp - kEpiWarp0) * 2 * kBiasBytes;
+    constexpr int kWordCols = 4 / static_cast<int>(sizeof(TO));
+    const bool bias_words = a.bias && reinterpret_cast<uintptr_t>(a.bias) % 4 == 0;
+    auto prefetch = [&](int t, int c, int buf, int bias_buf) {
       const int nb = min((t % tiles_n * kBN + group * kHalfN) / 128, ncb - 1);
+      if (!kSplit && c == 0 && bias_words) {
+        const int n0 = t % tiles_n * kBN + group * kHalfN;
+#pragma unroll
+        for (int w = 0; w < kHalfN / kWordCols; w += 32) {
+          const int n = n0 + (w + lane) * kWordCols;
+          if (n + kWordCols <= a.NO)
+            copy4_async(reinterpret_cast<float*>(my_bias + bias_buf * kBiasBytes) + w + lane,
+                        reinterpret_cast<const float*>(static_cast<const TO*>(a.bias) + n));
+        }
+      }
       const int64_t b = lo + c * kChunk + (lane & 7);
       float* to = scales + buf * kScaleBuf;
       if (b < lo + blocks) {
@@ -271,8 +291,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
     const int chunks = (blocks + kChunk - 1) / kChunk;
-    int sbuf = 0;
-    if (first < num_tiles) prefetch(first, 0, 0);
+    int sbuf = 0, tbuf = 0;  // the buffers of the scales and the tile's bias
+    if (first < num_tiles) prefetch(first, 0, 0, 0);
     commit();
     uint32_t it = 0;
     for (int t = first; t < num_tiles && !*abort_flag; t += step) {
@@ -288,8 +308,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int c = b / kChunk;
           if (b) sbuf ^= 1;
           __syncwarp();  // the other buffer's readers are done
-          if (c + 1 < chunks) prefetch(t, c + 1, sbuf ^ 1);
-          else if (t + step < num_tiles) prefetch(t + step, 0, sbuf ^ 1);
+          if (c + 1 < chunks) prefetch(t, c + 1, sbuf ^ 1, 0);
+          else if (t + step < num_tiles) prefetch(t + step, 0, sbuf ^ 1, tbuf ^ 1);
           commit();
           asm volatile("cp.async.wait_group 1;" ::: "memory");
           __syncwarp();
@@ -337,16 +357,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       sbuf ^= 1;  // the next tile's first scales
       const TO* bias = static_cast<const TO*>(a.bias);
-      const bool bias_vec = (reinterpret_cast<uintptr_t>(bias) & 15) == 0;
+      const uint8_t* tile_bias = my_bias + tbuf * kBiasBytes;
+      tbuf ^= 1;
       TO* y = static_cast<TO*>(a.y);
 #pragma unroll
       for (int c = 0; c < kHalfN; c += kSlabCols) {
         if (n0 + c >= a.NO) break;  // warp-uniform
         if (bias) {
-          if (bias_vec && n0 + c + kSlabCols <= a.NO) {
+          if (bias_words && n0 + c + kSlabCols <= a.NO) {
 #pragma unroll
             for (int e = 0; e < kSlabCols; e += 16 / static_cast<int>(sizeof(TO))) {
-              const uint4 q = *reinterpret_cast<const uint4*>(bias + n0 + c + e);
+              const uint4 q =
+                  *reinterpret_cast<const uint4*>(tile_bias + (c + e) * sizeof(TO));
               const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
