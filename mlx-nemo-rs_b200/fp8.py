@@ -13,7 +13,8 @@ A pre-norm linear's training step, with its activations kept in 8 bits:
     dx, dgamma, dbeta = layer_norm_backward(dh, xq, mean, rstd, gamma)
 
 Tensors are contiguous and on one device; the work is queued on that device's
-current torch stream.  The checks, the outputs' allocation and the calls are
+current torch stream, and autograd does not record it: the gradients are the
+calls above.  The checks, the outputs' allocation and the calls are
 native (torch_binding.cpp); what they refuse raises NrpError.
 """
 from __future__ import annotations

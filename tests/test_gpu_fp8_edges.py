@@ -286,3 +286,9 @@ def test_statistics_and_sums_are_tensors_of_their_own(nrp):
     assert torch.equal(p.grad, db)
     e, mean, rstd = nrp.layer_norm(o["x"][:0], o["gamma"], o["beta"])
     assert mean.shape == rstd.shape == (0,) and e.shape == (0, 256)
+    q = nrp.fp8_quantize(o["x"].view(3, 11, 256)[:, :, :80].contiguous())
+    assert q.codes.shape == (3, 11, 80) and q.scales.shape == (33, 1)
+    codes = q.codes.float()
+    q.scales.mul_(2)
+    assert torch.equal(q.codes.float(), codes) and q.codes.is_contiguous()
+    assert nrp.fp8_quantize(o["x"][:0], 128).scales.shape == (0, 2)
