@@ -393,9 +393,11 @@ __global__ void __launch_bounds__(256)
 // A batch is kR rows: 2, or 4 where the rows wait in shared memory (bf16 dy,
 // 16-byte copies, W <= 4: 2 kR W <= 32 lanes when the strips are joined).
 constexpr int kRingWarps = 4;
-// Up to here one cluster takes all rows, in one launch: bf16 64 x 1024 5.6 us
-// (host 5.8) against 5.5 us (host 8.2) in two, 200 x 1024 8.4 against 6.2.
-constexpr int kFewRows = 64;
+// Up to this many elements (of whole strips) one cluster takes all rows, in one
+// launch: the same time on the device, 2.3 us less on the host (bf16 128 x 512
+// 5.3 us and 4.7 against 5.2 and 7.0 in two launches, 256 x 512 6.3 against 5.7,
+// 64 x 2048 7.2 against 5.3; f32 64 x 512 6.6 against 5.3).
+constexpr int64_t kFewElements = 1 << 16;
 constexpr int kFewThreads = 512;       // threads of its CTAs
 constexpr int kManyThreads = 256;
 constexpr int kManyParts = 2 * 148;    // CTAs of the persistent grid at most
@@ -403,7 +405,7 @@ constexpr int kManyParts = 2 * 148;    // CTAs of the persistent grid at most
 // The most partial rows of dgamma | dbeta that go through the workspace (0: none).
 int norm_parts(int64_t rows, int cols) {
   if (cols > kStripCols) return static_cast<int>(std::min<int64_t>((rows + 7) / 8, kManyParts));
-  if (rows <= kFewRows) return 0;
+  if (rows <= kFewElements / (256 * strip_warps(cols))) return 0;
   const int per = strip_groups(cols, kManyThreads) * 2;
   return static_cast<int>(std::min<int64_t>((rows + per - 1) / per, kManyParts));
 }

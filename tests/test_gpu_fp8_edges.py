@@ -292,3 +292,29 @@ def test_statistics_and_sums_are_tensors_of_their_own(nrp):
     q.scales.mul_(2)
     assert torch.equal(q.codes.float(), codes) and q.codes.is_contiguous()
     assert nrp.fp8_quantize(o["x"][:0], 128).scales.shape == (0, 2)
+
+
+@pytest.mark.parametrize("rows,cols", [(128, 512), (129, 512), (32, 2048), (33, 2048), (256, 200),
+                                       (257, 200), (86, 768), (4097, 8), (3, 2056)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_norm_gradient_on_both_sides_of_one_launch(nrp, rows, cols, dtype):
+    """Where one cluster takes all rows and where two launches do, with the
+    workspace that the size asks for: dgamma and dbeta against 64 bits."""
+    import ctypes as C
+    import torch
+    dt = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn(rows, cols, device="cuda", generator=g).to(dt)
+    dy = torch.randn(rows, cols, device="cuda", generator=g).to(dt)
+    gamma = torch.randn(cols, device="cuda", generator=g)
+    _, mean, rstd = nrp.layer_norm(x, gamma, gamma)
+    size = C.c_int64()
+    assert nrp.lib().nrp_layer_norm_backward_workspace(rows, cols, C.byref(size)) == 0
+    assert (size.value == 0) == (cols <= 2048 and rows * (-(-cols // 256) * 256) <= 65536)
+    dx, dg, db = nrp.layer_norm_backward(dy, x, mean, rstd, gamma)
+    u = (x.double() - mean.double()[:, None]) * rstd.double()[:, None]
+    d = dy.double()
+    # u takes two roundings, dy u one, a column's chain rows + 16
+    assert ((dg.double() - (d * u).sum(0)).abs()
+            <= (rows + 20) * 2.0 ** -24 * (d * u).abs().sum(0) + 2.0 ** -30).all()
+    assert ((db.double() - d.sum(0)).abs() <= (rows + 16) * 2.0 ** -24 * d.abs().sum(0)).all()
