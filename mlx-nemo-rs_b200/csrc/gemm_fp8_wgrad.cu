@@ -547,17 +547,29 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// How a tile width would run: the CTAs that share a tile's tokens, and about how
+// long it takes.
+struct Plan {
+  int split;
+  float us;
+};
+// kStart: a launch whose tiles are not shared, with the result's store; kJoin: the
+// partial tiles' sum over a cluster; kStep: a step of 64 tokens.  From 1024 x
+// 1024 (64 / 128 / 256 columns: 100 tokens 5.5 / 7.5 / 10.0 us, 749 tokens 9.4 / 9.7 /
+// 12.0, 1500 tokens 13.8 / 12.2 / 15.1, 5000 tokens 33.8 / 23.7 / 21.8; these are
+// tiles of 1, 2 and 4 CTAs).
+template <int kTN>
+constexpr float kStep = kTN == 256 ? 0.56f : kTN == 128 ? 0.41f : 0.36f;
+constexpr float kStart = 5.f;
+template <int kTN>
+constexpr float kJoin = kTN == 256 ? 5.f : kTN == 128 ? 2.2f : 1.2f;
+
 template <int kTN, typename TO>
-cudaError_t launch(const void* dy, const uint8_t* xq, Args a, cudaStream_t stream) {
+cudaError_t plan(const Args& a, int num_sms, Plan& best, int& width) {
   constexpr size_t kSmem = Cfg<kTN>::kSmem;
   static std::atomic<uint64_t> attr{0};
   auto* kernel = fp8_wgrad_kernel<kTN, TO>;
   if (cudaError_t e = smem_attr_once(kernel, static_cast<int>(kSmem), attr)) return e;
-  CUtensorMap mdy, mxq;
-  if (!make_tmap_2d(&mdy, dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.N, a.M,
-                    static_cast<uint64_t>(a.N) * 2, 64, kTok, true) ||
-      !make_tmap_2d(&mxq, xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.M, a.K, kTK, kTok, false))
-    return cudaErrorInvalidValue;
   const int64_t tiles = qblocks(a.K) * ((a.N + kTN - 1) / kTN);
   // the largest split whose clusters all run at once, and that leaves every
   // CTA a step (on a B200 33 clusters of four fit, but only 15 of eight)
@@ -565,20 +577,38 @@ cudaError_t launch(const void* dy, const uint8_t* xq, Args a, cudaStream_t strea
   int dev = 0;
   if (cudaError_t e = cudaGetDevice(&dev)) return e;
   const int steps = (a.M + kTok - 1) / kTok;
-  a.split = 1;
+  int split = 1;
   for (int l = 1; l <= 3 && (1 << l) <= steps; ++l) {
     int f = fit[dev & 63][l].load(std::memory_order_relaxed);
     if (f == 0) {
       f = max_clusters(kernel, 1 << l, kThreads, kSmem);
       fit[dev & 63][l].store(f > 0 ? f : -1, std::memory_order_relaxed);
     }
-    if (tiles <= f) a.split = 1 << l;
+    if (tiles <= f) split = 1 << l;
   }
+  const float waves = split > 1 ? 1.f : static_cast<float>((tiles + num_sms - 1) / num_sms);
+  const float us = kStart + (split > 1 ? kJoin<kTN> : 0.f) +
+                   kStep<kTN> * waves * static_cast<float>((steps + split - 1) / split);
+  if (width == 0 || us < best.us) {
+    best = {split, us};
+    width = kTN;
+  }
+  return cudaSuccess;
+}
+
+template <int kTN, typename TO>
+cudaError_t launch(const void* dy, const uint8_t* xq, const Args& a, cudaStream_t stream) {
+  CUtensorMap mdy, mxq;
+  if (!make_tmap_2d(&mdy, dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.N, a.M,
+                    static_cast<uint64_t>(a.N) * 2, 64, kTok, true) ||
+      !make_tmap_2d(&mxq, xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.M, a.K, kTK, kTok, false))
+    return cudaErrorInvalidValue;
+  const int64_t tiles = qblocks(a.K) * ((a.N + kTN - 1) / kTN);
   if (tiles * a.split > 0x7fffffff) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * a.split));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmem;
+  cfg.dynamicSmemBytes = Cfg<kTN>::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute la[2];
   la[0].id = cudaLaunchAttributeClusterDimension;
@@ -589,20 +619,19 @@ cudaError_t launch(const void* dy, const uint8_t* xq, Args a, cudaStream_t strea
   la[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = la;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kernel, mdy, mxq, a);
+  return cudaLaunchKernelEx(&cfg, fp8_wgrad_kernel<kTN, TO>, mdy, mxq, a);
 }
 
 template <typename TO>
-cudaError_t pick(const void* dy, const uint8_t* xq, const Args& a, int num_sms,
-                 cudaStream_t stream) {
-  // Few tokens and no full wave of wide tiles: narrower ones, whose partial sums
-  // are smaller, down to 64 columns where those need no split at all (1024 x
-  // 1024, 256 / 128 / 64 columns: 100 tokens 10.0 / 7.5 / 5.5 us, 749 tokens
-  // 12.0 / 9.7 / 9.4, 1500 tokens 15.1 / 12.2 / 13.8, 5000 tokens 21.8 / 23.7 / 33.8).
-  const int64_t kb = qblocks(a.K);
-  if (a.M <= 768 && kb * ((a.N + 63) / 64) <= num_sms) return launch<64, TO>(dy, xq, a, stream);
-  if (a.M <= 2816 && 2 * kb * ((a.N + 255) / 256) <= num_sms)
-    return launch<128, TO>(dy, xq, a, stream);
+cudaError_t pick(const void* dy, const uint8_t* xq, Args a, int num_sms, cudaStream_t stream) {
+  Plan best{};
+  int width = 0;
+  if (cudaError_t e = plan<64, TO>(a, num_sms, best, width)) return e;
+  if (cudaError_t e = plan<128, TO>(a, num_sms, best, width)) return e;
+  if (cudaError_t e = plan<256, TO>(a, num_sms, best, width)) return e;
+  a.split = best.split;
+  if (width == 64) return launch<64, TO>(dy, xq, a, stream);
+  if (width == 128) return launch<128, TO>(dy, xq, a, stream);
   return launch<256, TO>(dy, xq, a, stream);
 }
 
