@@ -57,9 +57,6 @@ constexpr uint32_t kBiasBytes = 128 * 4;
 
 // A split tile's partial sums: four more floats to a row, for the banks.
 constexpr int kPartPitch = 128 + 4;
-// A split spares each CTA at least this many blocks of the reduction: a cluster
-// starts and joins in 1.7 us, a block takes 0.33 us.
-constexpr int kSplitSaves = 6;
 
 template <int kBN>
 struct Cfg {
@@ -513,24 +510,31 @@ cudaError_t launch(const uint8_t* xq, int R, const uint8_t* wq, Args a, int num_
       ((a.M + kBM - 1) / kBM) * static_cast<int64_t>((a.NO + kBN - 1) / kBN);
   if (tiles > 0x7fffffff) return cudaErrorInvalidValue;
   if constexpr (kSplit) {
-    // The largest split whose clusters all run at once (on a B200 33 of four
-    // CTAs, 15 of eight) and that leaves a CTA two blocks.  Split against one
-    // CTA to a tile, bf16 output: 64 rows, 1024 to 1024 5.1 against 5.9 us, 4096
-    // to 1024 6.4 against 13.8; 896 rows, 4096 to 1024 12.2 against 15.1, 2048
-    // to 1024 9.2 against 9.3, and 1024 to 1024 (a split of two would spare four
-    // blocks) 7.8 against 6.5.
-    static std::atomic<int> fit[64][4];
+    // The split with the least estimate, in us: 0.33 a block of the reduction, 1.1
+    // for a cluster and 0.2 for each of its CTAs; all clusters have to run at once
+    // (on a B200 33 of four CTAs, 15 of eight).  Split against one CTA to a tile,
+    // bf16 output: 64 rows, 1024 to 1024 5.1 against 5.9 us, 4096 to 1024 6.4 against
+    // 13.8; 600 rows, 4096 to 1024 9.8 (three CTAs; two 11.8) against 15.0; 896 rows
+    // 12.2 against 15.1; and two CTAs where none are taken, 896 rows, 1024 to 1024
+    // 7.8 against 6.5.
+    static std::atomic<int> fit[64][9];
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev)) return e;
     a.split = 1;
-    for (int l = 1; l <= 3 && a.rb >> l >= 2; ++l) {
-      if (a.rb - (a.rb >> l) < kSplitSaves) continue;
-      int f = fit[dev & 63][l].load(std::memory_order_relaxed);
+    float best = 0.33f * static_cast<float>(a.rb);
+    for (int s = 2; s <= 8 && a.rb / s >= 2 && tiles * s <= num_sms; ++s) {
+      const float us = 1.1f + 0.2f * static_cast<float>(s) +
+                       0.33f * static_cast<float>((a.rb + s - 1) / s);
+      if (us >= best) continue;
+      int f = fit[dev & 63][s].load(std::memory_order_relaxed);
       if (f == 0) {
-        f = max_clusters(kernel, 1 << l, kThreads, kSmem);
-        fit[dev & 63][l].store(f > 0 ? f : -1, std::memory_order_relaxed);
+        f = max_clusters(kernel, s, kThreads, kSmem);
+        fit[dev & 63][s].store(f > 0 ? f : -1, std::memory_order_relaxed);
       }
-      if (tiles <= f) a.split = 1 << l;
+      if (tiles <= f) {
+        a.split = s;
+        best = us;
+      }
     }
     if (a.split == 1) return launch<kBN, kTrans, TO, false>(xq, R, wq, a, num_sms, stream);
     cudaLaunchConfig_t cfg = {};
@@ -564,7 +568,7 @@ cudaError_t pick(const uint8_t* xq, int R, const uint8_t* wq, const Args& a, int
   // against 8.4, 16000 x 4096 88 against 80.
   const int64_t narrow = static_cast<int64_t>((a.M + kBM - 1) / kBM) * ((a.NO + 127) / 128);
   if (narrow > num_sms) return launch<256, kTrans, TO, false>(xq, R, wq, a, num_sms, stream);
-  if (a.rb >= kSplitSaves + 2 && 2 * narrow <= num_sms)
+  if (a.rb >= 8 && 2 * narrow <= num_sms)  // (fewer blocks: no split pays)
     return launch<128, kTrans, TO, true>(xq, R, wq, a, num_sms, stream);
   return launch<128, kTrans, TO, false>(xq, R, wq, a, num_sms, stream);
 }

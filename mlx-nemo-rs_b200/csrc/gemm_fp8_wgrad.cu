@@ -16,7 +16,7 @@
 // The bf16 checkpoint never exists in HBM, and the codes are half its bytes.
 //
 // Tiles are 128 k x 256 n, one per CTA, or narrower for few tokens.  Where they
-// do not fill the SMs, a cluster of 2, 4 or 8 CTAs splits the tokens of one
+// do not fill the SMs, a cluster of 2 to 8 CTAs splits the tokens of one
 // tile; the partial tiles are summed in rank order through distributed shared
 // memory, so the result does not depend on timing and needs no workspace.  That
 // sum costs about 4 us for four partial 256-wide tiles, which narrower ones save
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     cluster_sync();
     // this rank's columns, four k at a time, the ranks' tiles in order
-    const int cols = kTN / a.split;
+    const int c0 = kTN * rank / a.split, cols = kTN * (rank + 1) / a.split - c0;
     const bool wide = reinterpret_cast<uintptr_t>(dw) % 16 == 0;
     constexpr int kFly = 3;  // units whose loads are in flight together
     for (int u0 = threadIdx.x; u0 < cols * (kTK / 4); u0 += kFly * kThreads) {
@@ -522,19 +522,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < kFly; ++i) {
         const int u = min(u0 + i * kThreads, cols * (kTK / 4) - 1);
-        const int nn = rank * cols + u / (kTK / 4), kk = (u % (kTK / 4)) * 4;
+        const int nn = c0 + u / (kTK / 4), kk = (u % (kTK / 4)) * 4;
         sum[i] = cluster_sum4(smem_u32(part + nn * kTK + kk), a.split);
       }
 #pragma unroll
       for (int i = 0; i < kFly; ++i) {
         const int u = u0 + i * kThreads;
-        const int n = n0 + rank * cols + u / (kTK / 4), k = k0 + (u % (kTK / 4)) * 4;
+        const int n = n0 + c0 + u / (kTK / 4), k = k0 + (u % (kTK / 4)) * 4;
         if (u < cols * (kTK / 4) && n < a.N && k < a.K)  // K % 16 == 0: all four are inside
           store_four(dw + static_cast<int64_t>(n) * a.K + k, sum[i], wide);
       }
     }
     for (int c = threadIdx.x; c < cols; c += kThreads) {
-      const int nn = rank * cols + c;
+      const int nn = c0 + c;
       if (bias_here(nn)) store_one(db + n0 + nn, cluster_sum1(smem_u32(sBias + nn), a.split));
     }
     cluster_sync();  // no CTA leaves while another reads its tile
@@ -554,44 +554,47 @@ struct Plan {
   float us;
 };
 // kStart: a launch whose tiles are not shared, with the result's store; kJoin: the
-// partial tiles' sum over a cluster; kStep: a step of 64 tokens.  From 1024 x
-// 1024 (64 / 128 / 256 columns: 100 tokens 5.5 / 7.5 / 10.0 us, 749 tokens 9.4 / 9.7 /
-// 12.0, 1500 tokens 13.8 / 12.2 / 15.1, 5000 tokens 33.8 / 23.7 / 21.8; these are
-// tiles of 1, 2 and 4 CTAs).
+// partial tiles' sum over a cluster, and kRank for each of its CTAs; kStep: a
+// step of 64 tokens.  From 1024 x 1024 (64 / 128 / 256 columns: 100 tokens 5.7 / 7.9 /
+// 9.3 us, 749 tokens 10.1 / 10.1 / 12.6, 1500 tokens 15.2 / 12.8 / 14.2, 5000 tokens
+// 38 / 25 / 21.7; these are tiles of 1, 2 and 4 CTAs).  With them 5000 x 560 x 120
+// takes 64 columns and eight CTAs to a tile (11.6 us, 18.0 with 256), 12000 x 768 x
+// 768 256 and seven (30.8, 38.7 with four).
 template <int kTN>
 constexpr float kStep = kTN == 256 ? 0.56f : kTN == 128 ? 0.41f : 0.36f;
-constexpr float kStart = 5.f;
 template <int kTN>
-constexpr float kJoin = kTN == 256 ? 5.f : kTN == 128 ? 2.2f : 1.2f;
+constexpr float kJoin = kTN == 256 ? 4.2f : kTN == 128 ? 1.8f : 1.f;
+constexpr float kStart = 5.f, kRank = 0.2f;
 
+// Puts width kTN in place of `best` if it runs faster.
 template <int kTN, typename TO>
 cudaError_t plan(const Args& a, int num_sms, Plan& best, int& width) {
   constexpr size_t kSmem = Cfg<kTN>::kSmem;
   static std::atomic<uint64_t> attr{0};
   auto* kernel = fp8_wgrad_kernel<kTN, TO>;
   if (cudaError_t e = smem_attr_once(kernel, static_cast<int>(kSmem), attr)) return e;
-  const int64_t tiles = qblocks(a.K) * ((a.N + kTN - 1) / kTN);
-  // the largest split whose clusters all run at once, and that leaves every
-  // CTA a step (on a B200 33 clusters of four fit, but only 15 of eight)
-  static std::atomic<int> fit[64][4];
+  static std::atomic<int> fit[64][9];  // clusters that run at once, by size
   int dev = 0;
   if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  const int64_t tiles = qblocks(a.K) * ((a.N + kTN - 1) / kTN);
   const int steps = (a.M + kTok - 1) / kTok;
-  int split = 1;
-  for (int l = 1; l <= 3 && (1 << l) <= steps; ++l) {
-    int f = fit[dev & 63][l].load(std::memory_order_relaxed);
-    if (f == 0) {
-      f = max_clusters(kernel, 1 << l, kThreads, kSmem);
-      fit[dev & 63][l].store(f > 0 ? f : -1, std::memory_order_relaxed);
-    }
-    if (tiles <= f) split = 1 << l;
-  }
-  const float waves = split > 1 ? 1.f : static_cast<float>((tiles + num_sms - 1) / num_sms);
-  const float us = kStart + (split > 1 ? kJoin<kTN> : 0.f) +
-                   kStep<kTN> * waves * static_cast<float>((steps + split - 1) / split);
-  if (width == 0 || us < best.us) {
+  auto better = [&](int split, float us) {
+    if (width != 0 && us >= best.us) return;
     best = {split, us};
     width = kTN;
+  };
+  better(1, kStart + kStep<kTN> * static_cast<float>(steps) *
+                         static_cast<float>((tiles + num_sms - 1) / num_sms));
+  // all clusters have to run at once (on a B200 33 of four CTAs, 15 of eight)
+  for (int s = 2; s <= 8 && s <= steps && tiles * s <= num_sms; ++s) {
+    int f = fit[dev & 63][s].load(std::memory_order_relaxed);
+    if (f == 0) {
+      f = max_clusters(kernel, s, kThreads, kSmem);
+      fit[dev & 63][s].store(f > 0 ? f : -1, std::memory_order_relaxed);
+    }
+    if (tiles <= f)
+      better(s, kStart + kJoin<kTN> + kRank * static_cast<float>(s) +
+                    kStep<kTN> * static_cast<float>((steps + s - 1) / s));
   }
   return cudaSuccess;
 }

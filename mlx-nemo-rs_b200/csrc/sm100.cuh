@@ -195,7 +195,7 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
 }
 
 // The sum of four floats at one shared-memory offset over the cluster's first
-// `ranks` (2, 4 or 8) CTAs, in rank order, all loads in flight together.
+// `ranks` (2 to 8) CTAs, in rank order, all loads in flight together.
 __device__ __forceinline__ float4 cluster_sum4(uint32_t at, int ranks) {
   float4 v[8];
 #pragma unroll

@@ -356,7 +356,8 @@ def test_long_sums_and_repeats(nrp, m, k, n):
 
 @pytest.mark.parametrize("m,k,n", [(33, 1024, 1024), (64, 4096, 1024), (100, 1040, 200),
                                    (129, 2176, 1040), (200, 4224, 136), (600, 4096, 1024),
-                                   (896, 2064, 1000), (1100, 4096, 1024)])
+                                   (896, 2064, 1000), (1100, 4096, 1024), (1100, 2048, 512),
+                                   (200, 4096, 640)])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_shared_reductions(nrp, m, k, n, dtype):
     """Few tiles and a long reduction, which several CTAs share: the rows,
@@ -386,6 +387,32 @@ def test_shared_reductions(nrp, m, k, n, dtype):
             ref, size = ref + add, size + add.abs()
         off = (got.double() - ref).abs()
         assert (off <= size * (132 * 2.0 ** -23 + (k // 128 + 5) * U) + ref.abs() * u).all()
+
+
+@pytest.mark.parametrize("m,k,n", [(5000, 768, 768), (12000, 208, 488), (1500, 80, 1656),
+                                   (400, 512, 512), (9000, 560, 120), (700, 1536, 1024),
+                                   (450, 144, 64)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_shared_tokens(nrp, m, k, n, dtype):
+    """Weight gradients whose tiles' tokens 2 to 8 CTAs share, odd numbers of
+    them too, in every tile width: against 64 bits, five times the same bits."""
+    import torch
+    dt = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    u = 2.0 ** -8 if dt == torch.bfloat16 else U
+    g = torch.Generator(device="cuda").manual_seed(m)
+    xq = nrp.fp8_quantize(torch.randn(m, k, device="cuda", generator=g))
+    dy = torch.randn(m, n, device="cuda", generator=g).bfloat16()
+    dw, db = nrp.fp8_linear_weight_grad(dy, xq, bias=True, dtype=dt)
+    for _ in range(5):
+        a, b = nrp.fp8_linear_weight_grad(dy, xq, bias=True, dtype=dt)
+        assert torch.equal(a, dw) and torch.equal(b, db)
+    nrp.Context.default().check()
+    xv, d = device_values(xq), dy.double()
+    ref, size = d.t() @ xv, d.t().abs() @ xv.abs()
+    off = (dw.double() - ref).abs()
+    assert (off <= size * (m + m / 16 + 16) * 2.0 ** -23 + ref.abs() * u).all()
+    off = (db.double() - d.sum(0)).abs()
+    assert (off <= d.abs().sum(0) * (m + 16) * U + d.sum(0).abs() * u).all()
 
 
 def test_repeatable(nrp):
