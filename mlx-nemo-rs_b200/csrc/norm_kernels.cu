@@ -42,10 +42,11 @@ __device__ __forceinline__ float get(const __nv_bfloat16* p) { return __bfloat16
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 // a code: the caller multiplies by the block's scale
-__device__ __forceinline__ float get(const uint8_t* p) {
-  const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(*p), __NV_E4M3);
+__device__ __forceinline__ float code_value(uint32_t c) {
+  const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(c), __NV_E4M3);
   return __half2float(*reinterpret_cast<const __half*>(&h));
 }
+__device__ __forceinline__ float get(const uint8_t* p) { return code_value(*p); }
 
 // Eight consecutive elements, 16-byte aligned.
 __device__ __forceinline__ void store8(float* p, const float* v) {
@@ -84,9 +85,15 @@ struct Strip {
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float v = 0.f;
-        if (col + 32 * e < cols) v = ::nrp::get(p + col + 32 * e);
-        w[e] = __float_as_uint(v);
+        // as it is: a conversion here would wait for the load (30000 x 777 bf16
+        // backward: 47 us, 93 with it)
+        w[e] = 0u;
+        if (col + 32 * e < cols) {
+          if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(p[col + 32 * e]);
+          else if constexpr (sizeof(T) == 2)
+            w[e] = reinterpret_cast<const uint16_t*>(p)[col + 32 * e];
+          else w[e] = p[col + 32 * e];
+        }
       }
     }
   }
@@ -95,8 +102,11 @@ struct Strip {
     for (int i = 0; i < static_cast<int>(sizeof(w) / 4); ++i) w[i] = 0u;
   }
   __device__ __forceinline__ float get(int e) const {
-    if constexpr (!kVec || sizeof(T) == 4) return __uint_as_float(w[e]);
-    else if constexpr (sizeof(T) == 2)
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+    else if constexpr (!kVec) {
+      if constexpr (sizeof(T) == 2) return __uint_as_float(w[e] << 16);
+      else return code_value(w[e]);
+    } else if constexpr (sizeof(T) == 2)
       return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
     else {
       const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(

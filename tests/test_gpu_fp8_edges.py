@@ -318,3 +318,40 @@ def test_norm_gradient_on_both_sides_of_one_launch(nrp, rows, cols, dtype):
     assert ((dg.double() - (d * u).sum(0)).abs()
             <= (rows + 20) * 2.0 ** -24 * (d * u).abs().sum(0) + 2.0 ** -30).all()
     assert ((db.double() - d.sum(0)).abs() <= (rows + 16) * 2.0 ** -24 * d.abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(700, 129), (701, 777), (600, 130), (900, 255), (1300, 1023),
+                                       (333, 2047), (2000, 1001)])
+@pytest.mark.parametrize("off", [0, 1, 2])
+def test_norm_gradient_of_odd_rows(nrp, rows, cols, off):
+    """bf16 rows of odd columns and of tensors off a word: all gradients, and
+    nothing written around dx."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(cols)
+
+    def view(fill=None):
+        held = torch.full((rows * cols + off + 8,), 9.0, device="cuda", dtype=torch.bfloat16)
+        v = held[off:off + rows * cols].view(rows, cols)
+        if fill is not None:
+            v.copy_(fill)
+        return held, v
+
+    x = view(torch.randn(rows, cols, device="cuda", generator=g) + 0.5)[1]
+    dy = view(torch.randn(rows, cols, device="cuda", generator=g))[1]
+    gamma = torch.randn(cols, device="cuda", generator=g)
+    _, mean, rstd = nrp.layer_norm(x, gamma, gamma)
+    held, out = view()
+    dx, dg, db = nrp.layer_norm_backward(dy, x, mean, rstd, gamma, out=out)
+    assert (held[:off] == 9).all() and (held[off + rows * cols:] == 9).all()
+    d, u = dy.double(), (x.double() - mean.double()[:, None]) * rstd.double()[:, None]
+    w = d * gamma.double()
+    c1, c2 = w.mean(1, keepdim=True), (w * u).mean(1, keepdim=True)
+    ref = rstd.double()[:, None] * (w - c1 - u * c2)
+    # row sums: chains of cols / 32 + 16 at most in f32, u's two roundings
+    chain = (cols / 32 + 20) * 2.0 ** -24
+    size = rstd.double()[:, None] * (w.abs() + w.abs().mean(1, keepdim=True)
+                                     + u.abs() * (w * u).abs().mean(1, keepdim=True))
+    assert ((dx.double() - ref).abs() <= size * chain + ref.abs() * 2.0 ** -8).all()
+    assert ((dg.double() - (d * u).sum(0)).abs()
+            <= (rows + 20) * 2.0 ** -24 * (d * u).abs().sum(0) + 2.0 ** -30).all()
+    assert ((db.double() - d.sum(0)).abs() <= (rows + 16) * 2.0 ** -24 * d.abs().sum(0)).all()
