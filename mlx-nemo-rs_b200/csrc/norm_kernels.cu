@@ -196,7 +196,7 @@ constexpr int kFwdThreads = 256;
 template <int kR>
 constexpr int kFwdCtas = kR == 4 ? 2 : 3;
 
-template <typename T, int kR>
+template <typename T, bool kVec, int kR>
 __global__ void __launch_bounds__(kFwdThreads, kFwdCtas<kR>)
     norm_fwd_kernel(const T* x, int64_t rows, int cols, int W, const float* __restrict__ gamma,
                     const float* __restrict__ beta, float eps, T* y, float* __restrict__ mean_out,
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas<kR>)
   __shared__ float2 red[2][kFwdThreads / 32][kR];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int strip = warp % W, grp = warp / W, groups = static_cast<int>(blockDim.x) / 32 / W;
-  const int col = strip * 256 + lane * 8;
+  const int col = strip * 256 + (kVec ? lane * 8 : lane);
   pdl_launch_dependents();
   pdl_wait();
   const float inv_n = 1.f / static_cast<float>(min(256, cols - strip * 256));
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas<kR>)
   const float inv_c = 1.f / static_cast<float>(cols);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * groups * kR;
   int64_t row0 = (static_cast<int64_t>(blockIdx.x) * groups + grp) * kR;
-  Strip<T, true> next[kR];
+  Strip<T, kVec> next[kR];
   auto load = [&](int64_t r0) {
 #pragma unroll
     for (int r = 0; r < kR; ++r) {
@@ -222,12 +222,14 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas<kR>)
     }
   };
   load(row0);
-  const bool in = col < cols;  // (cols % 8 == 0: all of the lane's columns or none)
+  // columns of the lane's pair e; kVec: all of a lane's columns are inside or none
+  auto c0 = [&](int e) { return col + (kVec ? 2 * e : 64 * e); };
+  auto c1 = [&](int e) { return c0(e) + (kVec ? 1 : 32); };
   F2 gm[4], bt[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    gm[e] = in ? F2{gamma[col + 2 * e], gamma[col + 2 * e + 1]} : both(0.f);
-    bt[e] = in ? F2{beta[col + 2 * e], beta[col + 2 * e + 1]} : both(0.f);
+    gm[e] = {c0(e) < cols ? gamma[c0(e)] : 0.f, c1(e) < cols ? gamma[c1(e)] : 0.f};
+    bt[e] = {c0(e) < cols ? beta[c0(e)] : 0.f, c1(e) < cols ? beta[c1(e)] : 0.f};
   }
   int buf = 0;
   for (; row0 < rows; row0 += stride, buf ^= 1) {
@@ -256,10 +258,11 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas<kR>)
       F2 q = both(0.f);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const F2 d = add2(v[r][e], both(-mean[r]));
+        F2 d = add2(v[r][e], both(-mean[r]));
+        if (!kVec) d = {c0(e) < cols ? d.a : 0.f, c1(e) < cols ? d.b : 0.f};
         q = fma2(d, d, q);
       }
-      part[r] = in ? q.a + q.b : 0.f;  // (the others hold -mean)
+      part[r] = !kVec || col < cols ? q.a + q.b : 0.f;  // (the others hold -mean)
     }
     const float m2_w = warp_sums(part, lane);
     if (W == 1) {
@@ -295,7 +298,7 @@ __global__ void __launch_bounds__(kFwdThreads, kFwdCtas<kR>)
         o[2 * e] = f.a;
         o[2 * e + 1] = f.b;
       }
-      store_strip<T, true>(y + (row0 + r) * cols, col, cols, o);
+      store_strip<T, kVec>(y + (row0 + r) * cols, col, cols, o);
       if (mean_out && strip == 0 && lane == 0) {
         mean_out[row0 + r] = mean[r];
         rstd_out[row0 + r] = rstd[r];
@@ -785,12 +788,12 @@ struct FwdArgs {
   float *mean, *rstd;
 };
 
-template <typename T, int kR>
+template <typename T, bool kVec, int kR>
 cudaError_t fwd_strips(const T* x, T* y, const FwdArgs& a, int num_sms, cudaStream_t stream) {
   const int W = strip_warps(a.cols), groups = strip_groups(a.cols, kFwdThreads);
   const int per = groups * kR;
   const int64_t grid = std::min<int64_t>((a.rows + per - 1) / per, kFwdCtas<kR> * num_sms);
-  return launch_pdl(norm_fwd_kernel<T, kR>, dim3(static_cast<unsigned>(grid)),
+  return launch_pdl(norm_fwd_kernel<T, kVec, kR>, dim3(static_cast<unsigned>(grid)),
                     dim3(32 * W * groups), 0, stream, x, a.rows, a.cols, W, a.gamma, a.beta, a.eps,
                     y, a.mean, a.rstd);
 }
@@ -810,12 +813,14 @@ cudaError_t fwd(const T* x, T* y, const FwdArgs& a, int num_sms, cudaStream_t st
   // f32 strips of several warps are faster with two rows and three CTAs per SM
   // (50000 x 1024: 67 us, 77 with four and two), the others with four and two
   if (vec && a.cols <= kStripCols)
-    return sizeof(T) == 4 && a.cols > 256 ? fwd_strips<T, 2>(x, y, a, num_sms, stream)
-                                          : fwd_strips<T, 4>(x, y, a, num_sms, stream);
+    return sizeof(T) == 4 && a.cols > 256 ? fwd_strips<T, true, 2>(x, y, a, num_sms, stream)
+                                          : fwd_strips<T, true, 4>(x, y, a, num_sms, stream);
   if (a.cols <= 256) return fwd_rows<T, 1>(x, y, a, stream);
   if (a.cols <= 512) return fwd_rows<T, 2>(x, y, a, stream);
   if (a.cols <= 1024) return fwd_rows<T, 4>(x, y, a, stream);
-  if (a.cols <= 2048) return fwd_rows<T, 8>(x, y, a, stream);
+  // long rows as strips all the same (30000 x 1999 bf16: 65 us, 106 with a warp to a
+  // row, which 30000 x 333 favours: 13.7 against 16.0)
+  if (a.cols <= kStripCols) return fwd_strips<T, false, 4>(x, y, a, num_sms, stream);
   const int grid = static_cast<int>(std::min<int64_t>(a.rows, 8 * num_sms));
   return launch_pdl(norm_fwd_wide_kernel<T>, dim3(grid), dim3(256), 0, stream, x, a.rows, a.cols,
                     a.gamma, a.beta, a.eps, y, a.mean, a.rstd);
