@@ -566,16 +566,16 @@ template <int kTN>
 constexpr float kJoin = kTN == 256 ? 4.2f : kTN == 128 ? 1.8f : 1.f;
 constexpr float kStart = 5.f, kRank = 0.2f;
 
+template <int kTN, typename TO>
+cudaError_t allow_smem() {
+  static std::atomic<uint64_t> attr{0};
+  return smem_attr_once(fp8_wgrad_kernel<kTN, TO>, static_cast<int>(Cfg<kTN>::kSmem), attr);
+}
+
 // Puts width kTN in place of `best` if it runs faster.
 template <int kTN, typename TO>
-cudaError_t plan(const Args& a, int num_sms, Plan& best, int& width) {
-  constexpr size_t kSmem = Cfg<kTN>::kSmem;
-  static std::atomic<uint64_t> attr{0};
-  auto* kernel = fp8_wgrad_kernel<kTN, TO>;
-  if (cudaError_t e = smem_attr_once(kernel, static_cast<int>(kSmem), attr)) return e;
+cudaError_t plan(const Args& a, int num_sms, int dev, Plan& best, int& width) {
   static std::atomic<int> fit[64][9];  // clusters that run at once, by size
-  int dev = 0;
-  if (cudaError_t e = cudaGetDevice(&dev)) return e;
   const int64_t tiles = qblocks(a.K) * ((a.N + kTN - 1) / kTN);
   const int steps = (a.M + kTok - 1) / kTok;
   auto better = [&](int split, float us) {
@@ -589,7 +589,8 @@ cudaError_t plan(const Args& a, int num_sms, Plan& best, int& width) {
   for (int s = 2; s <= 8 && s <= steps && tiles * s <= num_sms; ++s) {
     int f = fit[dev & 63][s].load(std::memory_order_relaxed);
     if (f == 0) {
-      f = max_clusters(kernel, s, kThreads, kSmem);
+      if (cudaError_t e = allow_smem<kTN, TO>()) return e;
+      f = max_clusters(fp8_wgrad_kernel<kTN, TO>, s, kThreads, Cfg<kTN>::kSmem);
       fit[dev & 63][s].store(f > 0 ? f : -1, std::memory_order_relaxed);
     }
     if (tiles <= f)
@@ -601,6 +602,7 @@ cudaError_t plan(const Args& a, int num_sms, Plan& best, int& width) {
 
 template <int kTN, typename TO>
 cudaError_t launch(const void* dy, const uint8_t* xq, const Args& a, cudaStream_t stream) {
+  if (cudaError_t e = allow_smem<kTN, TO>()) return e;
   CUtensorMap mdy, mxq;
   if (!make_tmap_2d(&mdy, dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.N, a.M,
                     static_cast<uint64_t>(a.N) * 2, 64, kTok, true) ||
@@ -628,10 +630,11 @@ cudaError_t launch(const void* dy, const uint8_t* xq, const Args& a, cudaStream_
 template <typename TO>
 cudaError_t pick(const void* dy, const uint8_t* xq, Args a, int num_sms, cudaStream_t stream) {
   Plan best{};
-  int width = 0;
-  if (cudaError_t e = plan<64, TO>(a, num_sms, best, width)) return e;
-  if (cudaError_t e = plan<128, TO>(a, num_sms, best, width)) return e;
-  if (cudaError_t e = plan<256, TO>(a, num_sms, best, width)) return e;
+  int width = 0, dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  if (cudaError_t e = plan<64, TO>(a, num_sms, dev, best, width)) return e;
+  if (cudaError_t e = plan<128, TO>(a, num_sms, dev, best, width)) return e;
+  if (cudaError_t e = plan<256, TO>(a, num_sms, dev, best, width)) return e;
   a.split = best.split;
   if (width == 64) return launch<64, TO>(dy, xq, a, stream);
   if (width == 128) return launch<128, TO>(dy, xq, a, stream);
