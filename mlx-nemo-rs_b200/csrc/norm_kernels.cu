@@ -59,7 +59,7 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float* v) {
 }
 
 // A lane's eight elements of a row as they lie in memory, and as f32.
-template <typename T, bool kVec>
+template <typename T, bool kVec, int kL = 32>
 struct Strip {
   static constexpr int kWords = static_cast<int>(sizeof(T)) * 2;  // 8 elements
   uint32_t w[kVec ? kWords : 8];
@@ -88,11 +88,11 @@ struct Strip {
         // as it is: a conversion here would wait for the load (30000 x 777 bf16
         // backward: 47 us, 93 with it)
         w[e] = 0u;
-        if (col + 32 * e < cols) {
-          if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(p[col + 32 * e]);
+        if (col + kL * e < cols) {
+          if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(p[col + kL * e]);
           else if constexpr (sizeof(T) == 2)
-            w[e] = reinterpret_cast<const uint16_t*>(p)[col + 32 * e];
-          else w[e] = p[col + 32 * e];
+            w[e] = reinterpret_cast<const uint16_t*>(p)[col + kL * e];
+          else w[e] = p[col + kL * e];
         }
       }
     }
@@ -117,14 +117,14 @@ struct Strip {
     }
   }
 };
-template <typename T, bool kVec>
+template <typename T, bool kVec, int kL = 32>
 __device__ __forceinline__ void store_strip(T* p, int col, int cols, const float* v) {
   if constexpr (kVec) {
     if (col < cols) store8(p + col, v);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (col + 32 * e < cols) put(p + col + 32 * e, v[e]);
+      if (col + kL * e < cols) put(p + col + kL * e, v[e]);
   }
 }
 
@@ -172,22 +172,23 @@ int strip_groups(int cols, int threads) { return std::max(1, threads / 32 / stri
 // W rounded up to a power of two (lanes of a row when the strips are joined).
 __device__ __forceinline__ int strips_pow2(int W) { return W <= 1 ? 1 : 1 << (32 - __clz(W - 1)); }
 
-// The sums over the warp of kN = 2, 4 or 8 values per lane, halving the values
-// and the lanes that hold each: lane l ends with the sum of value l / (32 / kN).
-template <int kN>
+// The sums over each kL lanes of kN = 2, 4 or 8 <= kL values per lane, halving the
+// values and the lanes that hold each: lane l of them ends with the sum of value
+// l / (kL / kN).
+template <int kL = 32, int kN>
 __device__ __forceinline__ float warp_sums(const float (&v)[kN], int lane) {
   float a[kN];
 #pragma unroll
   for (int i = 0; i < kN; ++i) a[i] = v[i];
 #pragma unroll
-  for (int n = kN / 2, o = 16; n >= 1; n /= 2, o /= 2)
+  for (int n = kN / 2, o = kL / 2; n >= 1; n /= 2, o /= 2)
 #pragma unroll
     for (int i = 0; i < n; ++i) {
       const bool hi = lane & o;
       a[i] = (hi ? a[i + n] : a[i]) + __shfl_xor_sync(0xffffffffu, hi ? a[i] : a[i + n], o);
     }
 #pragma unroll
-  for (int o = 16 / kN; o >= 1; o /= 2) a[0] += __shfl_xor_sync(0xffffffffu, a[0], o);
+  for (int o = kL / 2 / kN; o >= 1; o /= 2) a[0] += __shfl_xor_sync(0xffffffffu, a[0], o);
   return a[0];
 }
 
@@ -413,6 +414,9 @@ constexpr int kRingWarps = 4;
 constexpr int64_t kFewElements = 1 << 16;
 constexpr int kFewThreads = 512;       // threads of its CTAs
 constexpr int kManyThreads = 256;
+// Rows of up to 128 columns take half a warp each (30000 x 64 bf16: 8.7 us, 12.2 with
+// a warp to a row; x 77 10.5 against 14.4).
+constexpr int kNarrowLanes = 16, kNarrow = 8 * kNarrowLanes;
 constexpr int kManyParts = 2 * 148;    // CTAs of the persistent grid at most
 
 // The most partial rows of dgamma | dbeta that go through the workspace (0: none).
@@ -424,11 +428,11 @@ int norm_parts(int64_t rows, int cols) {
 }
 
 // kR rows of a lane's strip.
-template <typename T, typename TX, bool kVec, int kR>
+template <typename T, typename TX, bool kVec, int kR, int kL>
 struct Batch {
   static constexpr int kScales = sizeof(TX) == 1 ? (kVec ? 1 : 2) : 0;
-  Strip<TX, kVec> x[kR];
-  Strip<T, kVec> dy[kR];
+  Strip<TX, kVec, kL> x[kR];
+  Strip<T, kVec, kL> dy[kR];
   float mu[kR], rs[kR], sx[kR][kScales ? kScales : 1];
   __device__ __forceinline__ void load(const TX* px, const float* xs, const T* pdy,
                                        const float* mean, const float* rstd, int64_t row0,
@@ -513,7 +517,8 @@ __device__ __forceinline__ const uint8_t* take_strip(const uint8_t* at, int thre
 
 // blockDim.x = 32 * W * groups.  partials [gridDim.x][2][cols], or null: the
 // grid is one cluster, and dgamma and dbeta (null: not wanted) are written.
-template <typename T, typename TX, bool kVec, int kThreads, int kR>
+// kL < 32 (W is 1): each kL lanes take rows of their own, of 8 kL columns at most.
+template <typename T, typename TX, bool kVec, int kThreads, int kR, int kL>
 __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
     norm_bwd_kernel(const TX* __restrict__ x, const float* __restrict__ xs,
                     const T* __restrict__ dy, const float* __restrict__ mean,
@@ -527,14 +532,17 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
   __shared__ float red[2][kThreads / 32][2 * kR];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int strip = warp % W, grp = warp / W, groups = static_cast<int>(blockDim.x) / 32 / W;
-  const int col = strip * 256 + (kVec ? lane * 8 : lane);
+  const int sub = lane % kL;
+  const int col = strip * 256 + (kVec ? sub * 8 : sub);
   pdl_launch_dependents();
   pdl_wait();
   const int cb = (cols + kQBlock - 1) / kQBlock;
   const float inv_c = 1.f / static_cast<float>(cols);
   const int Wp = strips_pow2(W), at_w = lane % Wp, at_i = lane / Wp;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * groups * kR;
-  int64_t row0 = (static_cast<int64_t>(blockIdx.x) * groups + grp) * kR;
+  constexpr int kBatch = kR * (32 / kL);  // rows of a group
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * groups * kBatch;
+  int64_t first = (static_cast<int64_t>(blockIdx.x) * groups + grp) * kBatch;
+  const int own = lane / kL * kR;  // the lane's rows among them
   using Rg = Ring<T, TX, kR>;
   const uint32_t ring = smem_u32(norm_smem);
   const bool in = col < cols;
@@ -557,27 +565,28 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   int slot = 0;
-  [[maybe_unused]] Batch<T, TX, kVec, kR> next;
+  [[maybe_unused]] Batch<T, TX, kVec, kR, kL> next;
   if constexpr (kRing) {
 #pragma unroll
-    for (int d = 0; d < Rg::kDepth - 1; ++d) issue(d, row0 + d * stride);
+    for (int d = 0; d < Rg::kDepth - 1; ++d) issue(d, first + d * stride);
   } else {
-    next.load(x, xs, dy, mean, rstd, row0, rows, cols, cb, col);
+    next.load(x, xs, dy, mean, rstd, first + own, rows, cols, cb, col);
   }
   F2 ag[4], ab[4], gm[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     ag[e] = ab[e] = both(0.f);
-    const int c0 = col + (kVec ? 2 * e : 64 * e), c1 = c0 + (kVec ? 1 : 32);
+    const int c0 = col + (kVec ? 2 * e : 2 * kL * e), c1 = c0 + (kVec ? 1 : kL);
     gm[e] = {c0 < cols ? gamma[c0] : 0.f, c1 < cols ? gamma[c1] : 0.f};
   }
   int buf = 0;
-  for (; row0 < rows; row0 += stride, buf ^= 1) {
-    Batch<T, TX, kVec, kR> now;
+  for (; first < rows; first += stride, buf ^= 1) {
+    const int64_t row0 = first + own;
+    Batch<T, TX, kVec, kR, kL> now;
     if constexpr (kRing) {
       asm volatile("cp.async.wait_group %0;" ::"n"(Rg::kDepth - 2) : "memory");
       __syncwarp();  // the warp's floats are there; the slot before has been read
-      issue(slot == 0 ? Rg::kDepth - 1 : slot - 1, row0 + (Rg::kDepth - 1) * stride);
+      issue(slot == 0 ? Rg::kDepth - 1 : slot - 1, first + (Rg::kDepth - 1) * stride);
       const uint8_t* at = norm_smem + slot * Rg::kSlot;
       const float* of_warp = reinterpret_cast<const float*>(at + kThreads * Rg::kBytes) + warp * 16;
 #pragma unroll
@@ -605,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
         if constexpr (kCodes) {
           // (code * scale - mean) * rstd with the constants multiplied first: a
           // mean so large that its rounding shows here leaves eight bits nothing
-          const float k = now.sx[r][kVec ? 0 : e >> 1] * now.rs[r];
+          const float k = now.sx[r][kVec || kL < 32 ? 0 : e >> 1] * now.rs[r];
           u[r][e] = fma2(xv, both(k), both(-now.mu[r] * now.rs[r]));
         } else {
           u[r][e] = mul2(add2(xv, both(-now.mu[r])), both(now.rs[r]));
@@ -620,12 +629,12 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
       part[kR + r] = c2.a + c2.b;
     }
     // lanes past the columns hold x = 0 and dy = 0: nothing but zeros added
-    const float mine = warp_sums(part, lane);
-    constexpr int kHold = 16 / kR;  // lanes that hold each sum
+    const float mine = warp_sums<kL>(part, lane);
+    constexpr int kHold = kL / 2 / kR;  // lanes that hold each sum
     float s[2 * kR];
-    if (W == 1) {
+    if (kL < 32 || W == 1) {
 #pragma unroll
-      for (int i = 0; i < 2 * kR; ++i) s[i] = __shfl_sync(0xffffffffu, mine, kHold * i);
+      for (int i = 0; i < 2 * kR; ++i) s[i] = __shfl_sync(0xffffffffu, mine, kHold * i, kL);
     } else {
       if (lane % kHold == 0) red[buf][warp][lane / kHold] = mine;
       named_bar_sync(1 + grp, 32 * W);
@@ -648,16 +657,27 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
         o[2 * e] = v.a;
         o[2 * e + 1] = v.b;
       }
-      store_strip<T, kVec>(dx + (row0 + r) * cols, col, cols, o);
+      store_strip<T, kVec, kL>(dx + (row0 + r) * cols, col, cols, o);
     }
   }
   if constexpr (kRing) asm volatile("cp.async.wait_all;" ::: "memory");
   if (!partials && !dgamma) return;
   if constexpr (kRing) __syncthreads();  // the sums take its place
+  // the lanes' rows apart hold the same columns
+#pragma unroll
+  for (int o = 16; o >= kL; o /= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      ag[e] = add2(ag[e], {__shfl_xor_sync(0xffffffffu, ag[e].a, o),
+                           __shfl_xor_sync(0xffffffffu, ag[e].b, o)});
+      ab[e] = add2(ab[e], {__shfl_xor_sync(0xffffffffu, ab[e].a, o),
+                           __shfl_xor_sync(0xffffffffu, ab[e].b, o)});
+    }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int c0 = col + (kVec ? 2 * e : 64 * e), c1 = c0 + (kVec ? 1 : 32);
+    const int c0 = col + (kVec ? 2 * e : 2 * kL * e), c1 = c0 + (kVec ? 1 : kL);
     float* to = col_sums + 2 * grp * cols;
+    if (lane >= kL) break;
     if (c0 < cols) to[c0] = ag[e].a, to[cols + c0] = ab[e].a;
     if (c1 < cols) to[c1] = ag[e].b, to[cols + c1] = ab[e].b;
   }
@@ -834,11 +854,11 @@ struct BwdArgs {
 };
 
 // parts: the CTAs, which is the partial rows written.
-template <typename T, typename TX, bool kVec, int kThreads, int kR>
+template <typename T, typename TX, bool kVec, int kThreads, int kR, int kL = 32>
 cudaError_t bwd_strips(const TX* x, const T* dy, T* dx, const BwdArgs& a, int& parts,
                        cudaStream_t stream) {
   const int W = strip_warps(a.cols), groups = strip_groups(a.cols, kThreads);
-  const int per = groups * kR;
+  const int per = groups * kR * (32 / kL);
   const int64_t batches = (a.rows + per - 1) / per;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute la[2];
@@ -860,7 +880,7 @@ cudaError_t bwd_strips(const TX* x, const T* dy, T* dx, const BwdArgs& a, int& p
   cfg.blockDim = dim3(32 * W * groups);
   parts = static_cast<int>(cfg.gridDim.x);
   // groups * W <= 16 warps of 256 columns: 32 KB of sums at most
-  auto* kernel = norm_bwd_kernel<T, TX, kVec, kThreads, kR>;
+  auto* kernel = norm_bwd_kernel<T, TX, kVec, kThreads, kR, kL>;
   const size_t sums = a.dgamma ? 8 * static_cast<size_t>(groups) * a.cols : 0;
   cfg.dynamicSmemBytes = sums;
   if constexpr (kR == 4) {
@@ -885,12 +905,14 @@ cudaError_t bwd(const TX* x, const T* dy, T* dx, const BwdArgs& a, cudaStream_t 
     if (parts == 0)
       return vec ? bwd_strips<T, TX, true, kFewThreads, 2>(x, dy, dx, a, parts, stream)
                  : bwd_strips<T, TX, false, kFewThreads, 2>(x, dy, dx, a, parts, stream);
-    bool four = false;
-    if constexpr (sizeof(T) == 2) {
-      four = vec && strip_warps(a.cols) <= kRingWarps;
-      if (four) e = bwd_strips<T, TX, true, kManyThreads, 4>(x, dy, dx, a, parts, stream);
-    }
-    if (!four)
+    constexpr int kBest = sizeof(T) == 2 ? 4 : 2;
+    if (a.cols <= kNarrow)
+      e = vec ? bwd_strips<T, TX, true, kManyThreads, 2, kNarrowLanes>(x, dy, dx, a, parts, stream)
+              : bwd_strips<T, TX, false, kManyThreads, 2, kNarrowLanes>(x, dy, dx, a, parts,
+                                                                        stream);
+    else if (vec && strip_warps(a.cols) <= kRingWarps)
+      e = bwd_strips<T, TX, true, kManyThreads, kBest>(x, dy, dx, a, parts, stream);
+    else
       e = vec ? bwd_strips<T, TX, true, kManyThreads, 2>(x, dy, dx, a, parts, stream)
               : bwd_strips<T, TX, false, kManyThreads, 2>(x, dy, dx, a, parts, stream);
   } else {

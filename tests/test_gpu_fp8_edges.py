@@ -295,11 +295,14 @@ def test_statistics_and_sums_are_tensors_of_their_own(nrp):
 
 
 @pytest.mark.parametrize("rows,cols", [(128, 512), (129, 512), (32, 2048), (33, 2048), (256, 200),
-                                       (257, 200), (86, 768), (4097, 8), (3, 2056)])
+                                       (257, 200), (86, 768), (4097, 8), (3, 2056), (5000, 1),
+                                       (5001, 16), (4999, 77), (3000, 128), (3001, 127),
+                                       (300, 129)])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_norm_gradient_on_both_sides_of_one_launch(nrp, rows, cols, dtype):
     """Where one cluster takes all rows and where two launches do, with the
-    workspace that the size asks for: dgamma and dbeta against 64 bits."""
+    workspace that the size asks for, and rows of half a warp: all gradients
+    against 64 bits."""
     import ctypes as C
     import torch
     dt = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
@@ -314,6 +317,15 @@ def test_norm_gradient_on_both_sides_of_one_launch(nrp, rows, cols, dtype):
     dx, dg, db = nrp.layer_norm_backward(dy, x, mean, rstd, gamma)
     u = (x.double() - mean.double()[:, None]) * rstd.double()[:, None]
     d = dy.double()
+    w = d * gamma.double()
+    c2 = (w * u).mean(1, keepdim=True)
+    ref = rstd.double()[:, None] * (w - w.mean(1, keepdim=True) - u * c2)
+    size = rstd.double()[:, None] * (w.abs() + w.abs().mean(1, keepdim=True)
+                                     + u.abs() * (w * u).abs().mean(1, keepdim=True))
+    # row sums: chains of cols / 32 + 16 at most, in rows over 2048 of cols / 256 + 16
+    half = 2.0 ** -8 if dt == torch.bfloat16 else 2.0 ** -24
+    assert ((dx.double() - ref).abs() <= size * (cols / 32 + 20) * 2.0 ** -24
+            + ref.abs() * half + 2.0 ** -30).all()
     # u takes two roundings, dy u one, a column's chain rows + 16
     assert ((dg.double() - (d * u).sum(0)).abs()
             <= (rows + 20) * 2.0 ** -24 * (d * u).abs().sum(0) + 2.0 ** -30).all()
