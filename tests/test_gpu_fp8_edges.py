@@ -367,3 +367,25 @@ def test_norm_gradient_of_odd_rows(nrp, rows, cols, off):
     assert ((dg.double() - (d * u).sum(0)).abs()
             <= (rows + 20) * 2.0 ** -24 * (d * u).abs().sum(0) + 2.0 ** -30).all()
     assert ((db.double() - d.sum(0)).abs() <= (rows + 16) * 2.0 ** -24 * d.abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(20, 512), (5000, 64), (5000, 1024), (3000, 777), (700, 2048),
+                                       (50, 4096)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_norm_gradient_without_parameters(nrp, rows, cols, dtype):
+    """dgamma, dbeta and workspace NULL: the same dx, in every kernel."""
+    import torch
+    dt = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn(rows, cols, device="cuda", generator=g).to(dt)
+    dy = torch.randn(rows, cols, device="cuda", generator=g).to(dt)
+    gamma = torch.randn(cols, device="cuda", generator=g)
+    _, mean, rstd = nrp.layer_norm(x, gamma, gamma)
+    want = nrp.layer_norm_backward(dy, x, mean, rstd, gamma)[0]
+    ctx, st = nrp.Context.default(), torch.cuda.current_stream().cuda_stream
+    dx = torch.empty_like(x)
+    code = nrp.BF16 if dt == torch.bfloat16 else nrp.F32
+    assert nrp.lib().nrp_layer_norm_backward(
+        ctx.handle, st, code, x.data_ptr(), None, dy.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+        gamma.data_ptr(), rows, cols, dx.data_ptr(), None, None, None, 0) == 0
+    assert torch.equal(dx, want)
