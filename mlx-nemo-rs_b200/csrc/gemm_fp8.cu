@@ -25,11 +25,11 @@
 // Bound by getting the operands to the tensor cores: a 256-wide block is 48 KB
 // into shared memory and 48 KB out of it for 256 cycles of MMA (768 at 128
 // bytes a cycle; measured 930), and the chip takes them from L2 at 11 TB/s.
-// Measured from codes to bf16: 16000 x 4096 to 1024 68 us (1.97 PFLOP/s; 3.4 waves
-// of tiles take four), 16000 x 1024 to 4096 with bias 78 us (9 of
-// them the output, 131 MB), 896 x 1024 to 1024 6.3 us.  Tried and slower: CTA pairs (256 x 256 tiles,
-// 76 us against 71: the hand-off over the cluster), sixteen epilogue warps (80
-// against 71), the last wave's tiles in halves (68.3 against 68.2).
+// Measured from codes to bf16: 16000 x 4096 to 1024 68 us (1.97 PFLOP/s; 3.4
+// waves of tiles take four), 16000 x 1024 to 4096 with bias 78 us (9 of them the
+// output, 131 MB), 896 x 1024 to 1024 6.3 us.  Tried and slower: CTA pairs (256 x
+// 256 tiles, 76 us against 71: the hand-off over the cluster), sixteen epilogue
+// warps (80 against 71), the last wave's tiles in halves (68.3 against 68.2).
 #include <algorithm>
 
 #include "fp8.h"
@@ -64,7 +64,8 @@ struct Cfg {
   static constexpr int kBufs = 512 / kBN;  // accumulators in TMEM
   static constexpr uint32_t kBBytes = kBN * kBR;
   static constexpr size_t kSmem =
-      1024 + kStages * (kABytes + kBBytes) + 8 * (kSlabBytes + 4 * kScaleFloats + 2 * kBiasBytes) + 256;
+      1024 + kStages * (kABytes + kBBytes) +
+      8 * (kSlabBytes + 4 * kScaleFloats + 2 * kBiasBytes) + 256;
 };
 static_assert(Cfg<256>::kSmem <= 232448 && Cfg<128>::kSmem <= 232448,
               "shared memory budget");
