@@ -224,7 +224,8 @@ CALLS = {
 
 @pytest.mark.parametrize("name", sorted(CALLS))
 def test_overlaps_and_alignment(nrp, mem, name):
-    """An output at the place of an input or of another output, and any argument off its alignment, is refused."""
+    """An output at the place of an input or of another output, and any argument
+    off its alignment, is refused."""
     p, _ = mem
     fn, call, outs, ins = CALLS[name]
     place = dict(zip(list(outs) + list(ins), AT))

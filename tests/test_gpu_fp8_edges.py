@@ -369,8 +369,8 @@ def test_norm_gradient_of_odd_rows(nrp, rows, cols, off):
     assert ((db.double() - d.sum(0)).abs() <= (rows + 16) * 2.0 ** -24 * d.abs().sum(0)).all()
 
 
-@pytest.mark.parametrize("rows,cols", [(20, 512), (5000, 64), (5000, 1024), (3000, 777), (700, 2048),
-                                       (50, 4096)])
+@pytest.mark.parametrize("rows,cols", [(20, 512), (5000, 64), (5000, 1024), (3000, 777),
+                                       (700, 2048), (50, 4096)])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_norm_gradient_without_parameters(nrp, rows, cols, dtype):
     """dgamma, dbeta and workspace NULL: the same dx, in every kernel."""
