@@ -164,8 +164,8 @@ __device__ __forceinline__ F2 both(float v) { return {v, v}; }
 // it are joined through shared memory, one barrier per batch (double
 // buffered): with n_w columns each,
 //   mean = sum n_w mean_w / C,  M2 = sum M2_w + n_w (mean_w - mean)^2.
-constexpr int kStripWarps = 8;  // W at most: 2048 columns
-constexpr int kStripCols = 256 * kStripWarps;
+constexpr int kStripCols = 2048;  // W at most 8, in CTAs of 256 threads
+constexpr int kWideCols = 4096;   // W at most 16, in CTAs of 512
 int strip_warps(int cols) { return (cols + 255) / 256; }
 int strip_groups(int cols, int threads) { return std::max(1, threads / 32 / strip_warps(cols)); }
 
@@ -193,16 +193,16 @@ __device__ __forceinline__ float warp_sums(const float (&v)[kN], int lane) {
 }
 
 constexpr int kFwdThreads = 256;
-// CTAs per SM of a kernel that takes kR rows at a time (kR kStripWarps <= 32).
-template <int kR>
-constexpr int kFwdCtas = kR == 4 ? 2 : 3;
+// CTAs per SM of a kernel that takes kR rows at a time (kR W <= 32).
+template <int kR, int kThreads>
+constexpr int kFwdCtas = kThreads > kFwdThreads ? 1 : kR == 4 ? 2 : 3;
 
-template <typename T, bool kVec, int kR>
-__global__ void __launch_bounds__(kFwdThreads, kFwdCtas<kR>)
+template <typename T, bool kVec, int kR, int kThreads>
+__global__ void __launch_bounds__(kThreads, kFwdCtas<kR, kThreads>)
     norm_fwd_kernel(const T* x, int64_t rows, int cols, int W, const float* __restrict__ gamma,
                     const float* __restrict__ beta, float eps, T* y, float* __restrict__ mean_out,
                     float* __restrict__ rstd_out) {
-  __shared__ float2 red[2][kFwdThreads / 32][kR];
+  __shared__ float2 red[2][kThreads / 32][kR];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int strip = warp % W, grp = warp / W, groups = static_cast<int>(blockDim.x) / 32 / W;
   const int col = strip * 256 + (kVec ? lane * 8 : lane);
@@ -421,7 +421,8 @@ constexpr int kManyParts = 2 * 148;    // CTAs of the persistent grid at most
 
 // The most partial rows of dgamma | dbeta that go through the workspace (0: none).
 int norm_parts(int64_t rows, int cols) {
-  if (cols > kStripCols) return static_cast<int>(std::min<int64_t>((rows + 7) / 8, kManyParts));
+  if (cols > kWideCols) return static_cast<int>(std::min<int64_t>((rows + 7) / 8, kManyParts));
+  if (cols > kStripCols) return static_cast<int>(std::min<int64_t>(rows, kManyParts / 2));
   if (rows <= kFewElements / (256 * strip_warps(cols))) return 0;
   const int per = strip_groups(cols, kManyThreads) * 2;
   return static_cast<int>(std::min<int64_t>((rows + per - 1) / per, kManyParts));
@@ -808,12 +809,13 @@ struct FwdArgs {
   float *mean, *rstd;
 };
 
-template <typename T, bool kVec, int kR>
+template <typename T, bool kVec, int kR, int kThreads = kFwdThreads>
 cudaError_t fwd_strips(const T* x, T* y, const FwdArgs& a, int num_sms, cudaStream_t stream) {
-  const int W = strip_warps(a.cols), groups = strip_groups(a.cols, kFwdThreads);
+  const int W = strip_warps(a.cols), groups = strip_groups(a.cols, kThreads);
   const int per = groups * kR;
-  const int64_t grid = std::min<int64_t>((a.rows + per - 1) / per, kFwdCtas<kR> * num_sms);
-  return launch_pdl(norm_fwd_kernel<T, kVec, kR>, dim3(static_cast<unsigned>(grid)),
+  const int64_t grid =
+      std::min<int64_t>((a.rows + per - 1) / per, kFwdCtas<kR, kThreads> * num_sms);
+  return launch_pdl(norm_fwd_kernel<T, kVec, kR, kThreads>, dim3(static_cast<unsigned>(grid)),
                     dim3(32 * W * groups), 0, stream, x, a.rows, a.cols, W, a.gamma, a.beta, a.eps,
                     y, a.mean, a.rstd);
 }
@@ -841,6 +843,10 @@ cudaError_t fwd(const T* x, T* y, const FwdArgs& a, int num_sms, cudaStream_t st
   // long rows as strips all the same (30000 x 1999 bf16: 65 us, 106 with a warp to a
   // row, which 30000 x 333 favours: 13.7 against 16.0)
   if (a.cols <= kStripCols) return fwd_strips<T, false, 4>(x, y, a, num_sms, stream);
+  // (4000 x 4096 bf16: 18.6 us, 28.9 by the kernel below)
+  if (a.cols <= kWideCols)
+    return vec ? fwd_strips<T, true, 2, 512>(x, y, a, num_sms, stream)
+               : fwd_strips<T, false, 2, 512>(x, y, a, num_sms, stream);
   const int grid = static_cast<int>(std::min<int64_t>(a.rows, 8 * num_sms));
   return launch_pdl(norm_fwd_wide_kernel<T>, dim3(grid), dim3(256), 0, stream, x, a.rows, a.cols,
                     a.gamma, a.beta, a.eps, y, a.mean, a.rstd);
@@ -865,7 +871,8 @@ cudaError_t bwd_strips(const TX* x, const T* dy, T* dx, const BwdArgs& a, int& p
   la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   la[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 1;
-  if (kThreads == kFewThreads && a.dgamma) {  // one cluster
+  constexpr bool kOne = kThreads == kFewThreads && kR > 1;  // one cluster (kR 1: wide rows)
+  if (kOne && a.dgamma) {
     unsigned c = 1;
     while (c < 8 && c < batches) c *= 2;
     cfg.gridDim = dim3(c);
@@ -875,7 +882,8 @@ cudaError_t bwd_strips(const TX* x, const T* dy, T* dx, const BwdArgs& a, int& p
     la[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
   } else {
-    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(batches, kManyParts)));
+    const int most = kThreads == kManyThreads ? kManyParts : kManyParts / 2;
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(batches, most)));
   }
   cfg.blockDim = dim3(32 * W * groups);
   parts = static_cast<int>(cfg.gridDim.x);
@@ -891,9 +899,9 @@ cudaError_t bwd_strips(const TX* x, const T* dy, T* dx, const BwdArgs& a, int& p
   }
   cfg.stream = stream;
   cfg.attrs = la;
-  float* partials = kThreads == kFewThreads ? nullptr : a.partials;
-  return cudaLaunchKernelEx(&cfg, kernel, x, a.xs, dy, a.mean,
-                            a.rstd, a.gamma, a.rows, a.cols, W, dx, partials, a.dgamma, a.dbeta);
+  float* partials = kOne ? nullptr : a.partials;
+  return cudaLaunchKernelEx(&cfg, kernel, x, a.xs, dy, a.mean, a.rstd, a.gamma, a.rows, a.cols, W,
+                            dx, partials, a.dgamma, a.dbeta);
 }
 
 template <typename T, typename TX>
@@ -915,6 +923,10 @@ cudaError_t bwd(const TX* x, const T* dy, T* dx, const BwdArgs& a, cudaStream_t 
     else
       e = vec ? bwd_strips<T, TX, true, kManyThreads, 2>(x, dy, dx, a, parts, stream)
               : bwd_strips<T, TX, false, kManyThreads, 2>(x, dy, dx, a, parts, stream);
+  } else if (a.cols <= kWideCols) {
+    // (4000 x 4096 bf16: 31.5 us, 103 by the kernels below)
+    e = vec ? bwd_strips<T, TX, true, kFewThreads, 1>(x, dy, dx, a, parts, stream)
+            : bwd_strips<T, TX, false, kFewThreads, 1>(x, dy, dx, a, parts, stream);
   } else {
     const int grid = static_cast<int>(std::min<int64_t>(a.rows, 4 * kManyParts));
     e = launch_pdl(norm_bwd_wide_kernel<T, TX>, dim3(grid), dim3(256), 0, stream, x, a.xs, dy,
