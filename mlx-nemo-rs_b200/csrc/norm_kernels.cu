@@ -371,28 +371,63 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
   return s;
 }
 
+// A thread's consecutive elements of a wide row, 8 where its address allows 16-byte
+// loads (4000 x 8192 bf16: forward 41 us, 60 by single elements; backward 88, 206).
+template <bool kVec>
+constexpr int kPiece = kVec ? 8 : 1;
+template <typename T, bool kVec>
+struct Piece {
+  float v[kPiece<kVec>];
+  __device__ __forceinline__ explicit Piece(const T* p) {
+    if constexpr (kVec) {
+      Strip<T, true> s;
+      s.load(p, 0, 1);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = s.get(e);
+    } else {
+      v[0] = get(p);
+    }
+  }
+};
+template <bool kVec, typename T>
+__device__ __forceinline__ void put_piece(T* p, const float* v) {
+  if constexpr (kVec) store8(p, v);
+  else put(p, v[0]);
+}
+
 // Any width: one CTA per row, x read three times.
-template <typename T>
+template <typename T, bool kVec>
 __global__ void __launch_bounds__(256)
     norm_fwd_wide_kernel(const T* x, int64_t rows, int cols, const float* __restrict__ gamma,
                          const float* __restrict__ beta, float eps, T* y,
                          float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+  constexpr int kE = kPiece<kVec>;
   __shared__ float part[8];
   pdl_launch_dependents();
   pdl_wait();
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * cols;
     float s = 0.f;
-    for (int c = threadIdx.x; c < cols; c += 256) s += get(xr + c);
+    for (int c = threadIdx.x * kE; c < cols; c += 256 * kE) {
+      const Piece<T, kVec> p(xr + c);
+#pragma unroll
+      for (int e = 0; e < kE; ++e) s += p.v[e];
+    }
     const float mean = block_sum(s, part) / static_cast<float>(cols);
     float q = 0.f;
-    for (int c = threadIdx.x; c < cols; c += 256) {
-      const float d = get(xr + c) - mean;
-      q = fmaf(d, d, q);
+    for (int c = threadIdx.x * kE; c < cols; c += 256 * kE) {
+      const Piece<T, kVec> p(xr + c);
+#pragma unroll
+      for (int e = 0; e < kE; ++e) q = fmaf(p.v[e] - mean, p.v[e] - mean, q);
     }
     const float rstd = 1.f / sqrtf(block_sum(q, part) / static_cast<float>(cols) + eps);
-    for (int c = threadIdx.x; c < cols; c += 256)
-      put(y + row * cols + c, fmaf((get(xr + c) - mean) * rstd, gamma[c], beta[c]));
+    for (int c = threadIdx.x * kE; c < cols; c += 256 * kE) {
+      Piece<T, kVec> p(xr + c);
+      const Piece<float, kVec> gm(gamma + c), bt(beta + c);
+#pragma unroll
+      for (int e = 0; e < kE; ++e) p.v[e] = fmaf((p.v[e] - mean) * rstd, gm.v[e], bt.v[e]);
+      put_piece<kVec>(y + row * cols + c, p.v);
+    }
     if (threadIdx.x == 0 && mean_out) {
       mean_out[row] = mean;
       rstd_out[row] = rstd;
@@ -707,70 +742,94 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
 }
 
 // Any width, dx: one CTA per row, x and dy read twice.
-template <typename T, typename TX>
+template <typename T, typename TX, bool kVec>
 __global__ void __launch_bounds__(256)
     norm_bwd_wide_kernel(const TX* __restrict__ x, const float* __restrict__ xs,
                          const T* __restrict__ dy, const float* __restrict__ mean,
                          const float* __restrict__ rstd, const float* __restrict__ gamma,
                          int64_t rows, int cols, T* __restrict__ dx) {
-  constexpr bool kCodes = sizeof(TX) == 1;
+  constexpr int kE = kPiece<kVec>;
   __shared__ float part[8];
   pdl_launch_dependents();
   pdl_wait();
   const int cb = (cols + kQBlock - 1) / kQBlock;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const float mu = mean[row], rs = rstd[row];
-    auto u_at = [&](int c) {
-      float v = get(x + row * cols + c);
-      if (kCodes) v *= xs[row * cb + (c >> 7)];
-      return (v - mu) * rs;
-    };
+    // (a piece lies in one block)
+    auto scale = [&](int c) { return sizeof(TX) == 1 ? xs[row * cb + (c >> 7)] : 1.f; };
     float c1 = 0.f, c2 = 0.f;
-    for (int c = threadIdx.x; c < cols; c += 256) {
-      const float g = get(dy + row * cols + c) * gamma[c];
-      c1 += g;
-      c2 = fmaf(g, u_at(c), c2);
+    for (int c = threadIdx.x * kE; c < cols; c += 256 * kE) {
+      const Piece<TX, kVec> px(x + row * cols + c);
+      const Piece<T, kVec> pd(dy + row * cols + c);
+      const Piece<float, kVec> gm(gamma + c);
+      const float k = scale(c);
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+        const float g = pd.v[e] * gm.v[e];
+        c1 += g;
+        c2 = fmaf(g, (px.v[e] * k - mu) * rs, c2);
+      }
     }
     c1 = block_sum(c1, part) / static_cast<float>(cols);
     c2 = block_sum(c2, part) / static_cast<float>(cols);
-    for (int c = threadIdx.x; c < cols; c += 256)
-      put(dx + row * cols + c, rs * (get(dy + row * cols + c) * gamma[c] - c1 - u_at(c) * c2));
+    for (int c = threadIdx.x * kE; c < cols; c += 256 * kE) {
+      const Piece<TX, kVec> px(x + row * cols + c);
+      Piece<T, kVec> pd(dy + row * cols + c);
+      const Piece<float, kVec> gm(gamma + c);
+      const float k = scale(c);
+#pragma unroll
+      for (int e = 0; e < kE; ++e)
+        pd.v[e] = rs * (pd.v[e] * gm.v[e] - c1 - (px.v[e] * k - mu) * rs * c2);
+      put_piece<kVec>(dx + row * cols + c, pd.v);
+    }
   }
 }
 
-// Any width, the partial column sums: CTA (x, y) takes 32 columns and every
-// gridDim.y-th group of 8 rows.
-template <typename T, typename TX>
+// Any width, the partial column sums: CTA (x, y) takes 32 pieces of columns and
+// every gridDim.y-th group of 8 rows.
+template <typename T, typename TX, bool kVec>
 __global__ void __launch_bounds__(256)
     norm_bwd_cols_kernel(const TX* __restrict__ x, const float* __restrict__ xs,
                          const T* __restrict__ dy, const float* __restrict__ mean,
                          const float* __restrict__ rstd, int64_t rows, int cols,
                          float* __restrict__ partials) {
-  constexpr bool kCodes = sizeof(TX) == 1;
-  __shared__ float red[2][8][32];
+  constexpr int kE = kPiece<kVec>;
+  __shared__ float red[2][8][32 * kE];
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + lane;
+  const int col = (blockIdx.x * 32 + lane) * kE;
   const int cb = (cols + kQBlock - 1) / kQBlock;
-  float ag = 0.f, ab = 0.f;
+  float ag[kE], ab[kE];
+#pragma unroll
+  for (int e = 0; e < kE; ++e) ag[e] = ab[e] = 0.f;
   if (col < cols)
     for (int64_t row = static_cast<int64_t>(blockIdx.y) * 8 + warp; row < rows;
          row += static_cast<int64_t>(gridDim.y) * 8) {
-      float v = get(x + row * cols + col);
-      if (kCodes) v *= xs[row * cb + (col >> 7)];
-      const float d = get(dy + row * cols + col);
-      ag = fmaf(d, (v - mean[row]) * rstd[row], ag);
-      ab += d;
+      const Piece<TX, kVec> px(x + row * cols + col);
+      const Piece<T, kVec> pd(dy + row * cols + col);
+      const float k = sizeof(TX) == 1 ? xs[row * cb + (col >> 7)] : 1.f;
+      const float mu = mean[row], rs = rstd[row];
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+        ag[e] = fmaf(pd.v[e], (px.v[e] * k - mu) * rs, ag[e]);
+        ab[e] += pd.v[e];
+      }
     }
-  red[0][warp][lane] = ag;
-  red[1][warp][lane] = ab;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+    red[0][warp][32 * e + lane] = ag[e];
+    red[1][warp][32 * e + lane] = ab[e];
+  }
   __syncthreads();
-  if (warp < 2 && col < cols) {
+  for (int i = threadIdx.x; i < 64 * kE; i += 256) {
+    const int which = i / (32 * kE), at = i % (32 * kE);
+    const int c = (blockIdx.x * 32 + at % 32) * kE + at / 32;
+    if (c >= cols) continue;
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) s += red[warp][w][lane];
-    partials[(static_cast<int64_t>(blockIdx.y) * 2 + warp) * cols + col] = s;
+    for (int w = 0; w < 8; ++w) s += red[which][w][at];
+    partials[(static_cast<int64_t>(blockIdx.y) * 2 + which) * cols + c] = s;
   }
 }
 
@@ -848,8 +907,10 @@ cudaError_t fwd(const T* x, T* y, const FwdArgs& a, int num_sms, cudaStream_t st
     return vec ? fwd_strips<T, true, 2, 512>(x, y, a, num_sms, stream)
                : fwd_strips<T, false, 2, 512>(x, y, a, num_sms, stream);
   const int grid = static_cast<int>(std::min<int64_t>(a.rows, 8 * num_sms));
-  return launch_pdl(norm_fwd_wide_kernel<T>, dim3(grid), dim3(256), 0, stream, x, a.rows, a.cols,
-                    a.gamma, a.beta, a.eps, y, a.mean, a.rstd);
+  const bool all = vec && aligned16(a.gamma) && aligned16(a.beta);
+  return launch_pdl(all ? norm_fwd_wide_kernel<T, true> : norm_fwd_wide_kernel<T, false>,
+                    dim3(grid), dim3(256), 0, stream, x, a.rows, a.cols, a.gamma, a.beta, a.eps, y,
+                    a.mean, a.rstd);
 }
 
 struct BwdArgs {
@@ -929,11 +990,15 @@ cudaError_t bwd(const TX* x, const T* dy, T* dx, const BwdArgs& a, cudaStream_t 
             : bwd_strips<T, TX, false, kFewThreads, 1>(x, dy, dx, a, parts, stream);
   } else {
     const int grid = static_cast<int>(std::min<int64_t>(a.rows, 4 * kManyParts));
-    e = launch_pdl(norm_bwd_wide_kernel<T, TX>, dim3(grid), dim3(256), 0, stream, x, a.xs, dy,
-                   a.mean, a.rstd, a.gamma, a.rows, a.cols, dx);
+    const bool all = vec && aligned16(a.gamma);
+    e = launch_pdl(all ? norm_bwd_wide_kernel<T, TX, true> : norm_bwd_wide_kernel<T, TX, false>,
+                   dim3(grid), dim3(256), 0, stream, x, a.xs, dy, a.mean, a.rstd, a.gamma, a.rows,
+                   a.cols, dx);
+    const int across = 32 * (vec ? kPiece<true> : kPiece<false>);
     if (e == cudaSuccess && a.dgamma)
-      e = launch_pdl(norm_bwd_cols_kernel<T, TX>, dim3((a.cols + 31) / 32, parts), dim3(256), 0,
-                     stream, x, a.xs, dy, a.mean, a.rstd, a.rows, a.cols, a.partials);
+      e = launch_pdl(vec ? norm_bwd_cols_kernel<T, TX, true> : norm_bwd_cols_kernel<T, TX, false>,
+                     dim3((a.cols + across - 1) / across, parts), dim3(256), 0, stream, x, a.xs, dy,
+                     a.mean, a.rstd, a.rows, a.cols, a.partials);
   }
   if (e != cudaSuccess || !a.dgamma) return e;
   return launch_pdl(norm_bwd_sum_kernel, dim3((2 * a.cols + 31) / 32), dim3(256), 0, stream,

@@ -297,7 +297,8 @@ def test_statistics_and_sums_are_tensors_of_their_own(nrp):
 @pytest.mark.parametrize("rows,cols", [(128, 512), (129, 512), (32, 2048), (33, 2048), (256, 200),
                                        (257, 200), (86, 768), (4097, 8), (3, 2056), (5000, 1),
                                        (5001, 16), (4999, 77), (3000, 128), (3001, 127),
-                                       (300, 129)])
+                                       (300, 129), (70, 4096), (33, 3001), (50, 6000),
+                                       (50, 6001), (120, 8200)])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_norm_gradient_on_both_sides_of_one_launch(nrp, rows, cols, dtype):
     """Where one cluster takes all rows and where two launches do, with the
@@ -369,8 +370,8 @@ def test_norm_gradient_of_odd_rows(nrp, rows, cols, off):
     assert ((db.double() - d.sum(0)).abs() <= (rows + 16) * 2.0 ** -24 * d.abs().sum(0)).all()
 
 
-@pytest.mark.parametrize("rows,cols", [(20, 512), (5000, 64), (5000, 1024), (3000, 777),
-                                       (700, 2048), (50, 4096)])
+@pytest.mark.parametrize("rows,cols", [(20, 512), (5000, 64), (5000, 1024), (3000, 777), (40, 6001),
+                                       (700, 2048), (50, 4096), (90, 8192)])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_norm_gradient_without_parameters(nrp, rows, cols, dtype):
     """dgamma, dbeta and workspace NULL: the same dx, in every kernel."""
