@@ -155,6 +155,27 @@ __device__ __forceinline__ F2 fma2(F2 x, F2 y, F2 z) {
 }
 __device__ __forceinline__ F2 both(float v) { return {v, v}; }
 
+// gamma or beta at a strip's eight columns of a lane (zeros off the end); kVec:
+// all of them are inside or none.
+template <bool kVec, int kL = 32>
+__device__ __forceinline__ void lane_columns(const float* __restrict__ p, int col, int cols,
+                                             F2 (&v)[4]) {
+  if (kVec && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    if (col < cols) {
+      a = reinterpret_cast<const float4*>(p + col)[0];
+      b = reinterpret_cast<const float4*>(p + col)[1];
+    }
+    v[0] = {a.x, a.y}, v[1] = {a.z, a.w}, v[2] = {b.x, b.y}, v[3] = {b.z, b.w};
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int c0 = col + (kVec ? 2 * e : 2 * kL * e), c1 = c0 + (kVec ? 1 : kL);
+    v[e] = {c0 < cols ? p[c0] : 0.f, c1 < cols ? p[c1] : 0.f};
+  }
+}
+
 // ------------------------------------------------------------- forward
 // A group of W = ceil(cols / 256) warps takes kR rows at a time, each warp a
 // strip of 256 columns, a lane eight of them, with the next rows' loads in
@@ -223,15 +244,12 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas<kR, kThreads>)
     }
   };
   load(row0);
-  // columns of the lane's pair e; kVec: all of a lane's columns are inside or none
+  // columns of the lane's pair e
   auto c0 = [&](int e) { return col + (kVec ? 2 * e : 64 * e); };
   auto c1 = [&](int e) { return c0(e) + (kVec ? 1 : 32); };
   F2 gm[4], bt[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    gm[e] = {c0(e) < cols ? gamma[c0(e)] : 0.f, c1(e) < cols ? gamma[c1(e)] : 0.f};
-    bt[e] = {c0(e) < cols ? beta[c0(e)] : 0.f, c1(e) < cols ? beta[c1(e)] : 0.f};
-  }
+  lane_columns<kVec>(gamma, col, cols, gm);
+  lane_columns<kVec>(beta, col, cols, bt);
   int buf = 0;
   for (; row0 < rows; row0 += stride, buf ^= 1) {
     F2 v[kR][4];
@@ -610,11 +628,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
   }
   F2 ag[4], ab[4], gm[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    ag[e] = ab[e] = both(0.f);
-    const int c0 = col + (kVec ? 2 * e : 2 * kL * e), c1 = c0 + (kVec ? 1 : kL);
-    gm[e] = {c0 < cols ? gamma[c0] : 0.f, c1 < cols ? gamma[c1] : 0.f};
-  }
+  for (int e = 0; e < 4; ++e) ag[e] = ab[e] = both(0.f);
+  lane_columns<kVec, kL>(gamma, col, cols, gm);
   int buf = 0;
   for (; first < rows; first += stride, buf ^= 1) {
     const int64_t row0 = first + own;
