@@ -599,7 +599,8 @@ int nrp_qlinear(nrp_context* ctx, void* stream, const void* x, int M, int K, con
  * of the unquantised operands and outputs (NRP_DTYPE_F32 or _BF16); sums are
  * f32.  A matrix without rows is allowed; its pointers are not looked at.
  * Every pointer is aligned to its elements (to 16 bytes where a call says so);
- * no output overlaps another argument, unless a call says so.
+ * no output overlaps another argument, unless a call says so.  The products'
+ * sizes are at most 2^31 - 4096.
  * These calls allocate nothing and use no buffers but their arguments,
  * so calls and captured graphs on different streams do not share state. */
 

@@ -30,6 +30,15 @@ int check_dtype(int dtype) {
   return failf(NRP_ERR_UNSUPPORTED, "dtype %d", dtype);
 }
 
+// The largest row and column counts of a product: the kernels round them up to
+// whole tiles and look a few tiles ahead in 32-bit indices.
+constexpr int kMaxSize = INT32_MAX - 4095;
+int check_sizes(const char* what, std::initializer_list<int> sizes) {
+  for (int n : sizes)
+    if (n > kMaxSize) return failf(NRP_ERR_UNSUPPORTED, "%s: size %d (at most %d)", what, n, kMaxSize);
+  return NRP_OK;
+}
+
 // A matrix of codes: 16-byte rows (TMA and 16-byte loads), 16-byte aligned.
 // One without rows may have null pointers (an empty tensor's).
 int check_codes(const char* name, const void* codes, const void* scales, int64_t cols,
@@ -171,6 +180,7 @@ int nrp_fp8_linear(nrp_context* ctx, void* stream, int dtype, const void* x, uin
   if (!ctx || (M && !y) || M < 0 || K <= 0 || N <= 0)
     return failf(NRP_ERR_INVALID, "invalid fp8 linear arguments");
   if (int rc = check_dtype(dtype)) return rc;
+  if (int rc = check_sizes("fp8 linear", {M, K, N})) return rc;
   if (int rc = check_codes("fp8 linear: input", xq, xs, K, M == 0)) return rc;
   if (int rc = check_codes("fp8 linear: weight", wq, ws, K)) return rc;
   if (int rc = check_product("fp8 linear", dtype, x, xq, xs, M, K, wq, ws, N, K, bias, y, N))
@@ -186,6 +196,7 @@ int nrp_fp8_linear_input_grad(nrp_context* ctx, void* stream, int dtype, const v
   if (!ctx || (M && !dx) || M < 0 || K <= 0 || N <= 0)
     return failf(NRP_ERR_INVALID, "invalid fp8 input gradient arguments");
   if (int rc = check_dtype(dtype)) return rc;
+  if (int rc = check_sizes("fp8 input gradient", {M, N, K})) return rc;
   if (int rc = check_codes("fp8 input gradient: output gradient", gq, gs, N, M == 0)) return rc;
   if (int rc = check_codes("fp8 input gradient: weight", wq, ws, K)) return rc;
   if (int rc = check_product("fp8 input gradient", dtype, dy, gq, gs, M, N, wq, ws, N, K, nullptr,
@@ -202,6 +213,7 @@ int nrp_fp8_linear_weight_grad(nrp_context* ctx, void* stream, const void* dy, c
   if (!ctx || (M && !dy) || !dw || M < 0 || K <= 0 || N <= 0)
     return failf(NRP_ERR_INVALID, "invalid fp8 weight gradient arguments");
   if (int rc = check_dtype(dtype)) return rc;
+  if (int rc = check_sizes("fp8 weight gradient", {M, N, K})) return rc;
   if (int rc = check_codes("fp8 weight gradient: input", xq, xs, K, M == 0)) return rc;
   if (N % 8)
     return failf(NRP_ERR_UNSUPPORTED, "fp8 weight gradient: N = %d (needs a multiple of 8)", N);

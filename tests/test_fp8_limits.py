@@ -1,0 +1,56 @@
+"""The ends of the 8-bit operators' and the LayerNorm's argument ranges without
+a GPU: what the kernels' 32-bit indices cannot take is refused before the device
+is touched."""
+import ctypes as C
+
+import pytest
+
+from __graft_entry__ import load_package
+
+INVALID, UNSUPPORTED = -1, -3
+F32, BF16 = 0, 1
+MOST = 2 ** 31 - 4096  # the largest size of a product
+
+# pointers far enough apart that no argument of any size meets another
+AT = [(i + 1) << 52 for i in range(10)]
+
+
+@pytest.fixture(scope="module")
+def nrp():
+    from __graft_entry__ import _load_build_script
+    _load_build_script().build()
+    return load_package()
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    buf = C.create_string_buffer(8192)
+    return (C.addressof(buf) + 255) // 256 * 256, buf
+
+
+def status(nrp, fn, *args):
+    rc = getattr(nrp.lib(), fn)(*args)
+    return rc, nrp.lib().nrp_last_error().decode()
+
+
+def product(fn, ctx, m, red, cols):
+    x, xq, xs, wq, ws, y = AT[:6]
+    a = [ctx, None, BF16, None, xq, xs, m, red, wq, ws, cols]
+    return a + ([None, y] if fn == "nrp_fp8_linear" else [y])
+
+
+@pytest.mark.parametrize("fn", ["nrp_fp8_linear", "nrp_fp8_linear_input_grad"])
+@pytest.mark.parametrize("sizes", [(2 ** 31 - 1, 16, 16), (MOST + 1, 16, 16), (16, 2 ** 31 - 16, 16),
+                                   (16, 16, 2 ** 31 - 16)])
+def test_product_sizes(nrp, ctx, fn, sizes):
+    rc, msg = status(nrp, fn, *product(fn, ctx[0], *sizes))
+    assert rc == UNSUPPORTED and "size" in msg
+
+
+@pytest.mark.parametrize("m,n,k", [(2 ** 31 - 1, 8, 16), (2 ** 31 - 63, 8, 16), (MOST + 1, 8, 16),
+                                   (64, 2 ** 31 - 8, 16), (64, 8, 2 ** 31 - 16)])
+def test_weight_gradient_sizes(nrp, ctx, m, n, k):
+    """From 2^31 - 63 rows on the count of 64-token steps would be negative."""
+    rc, msg = status(nrp, "nrp_fp8_linear_weight_grad", ctx[0], None, AT[0], AT[1], AT[2], m, n, k,
+                     F32, AT[3], AT[4])
+    assert rc == UNSUPPORTED and "size" in msg
