@@ -600,7 +600,7 @@ int nrp_qlinear(nrp_context* ctx, void* stream, const void* x, int M, int K, con
  * f32.  A matrix without rows is allowed; its pointers are not looked at.
  * Every pointer is aligned to its elements (to 16 bytes where a call says so);
  * no output overlaps another argument, unless a call says so.  The products'
- * sizes are at most 2^31 - 4096.
+ * sizes and the LayerNorm's columns are at most 2^31 - 4096.
  * These calls allocate nothing and use no buffers but their arguments,
  * so calls and captured graphs on different streams do not share state. */
 

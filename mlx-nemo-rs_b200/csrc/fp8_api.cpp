@@ -30,8 +30,8 @@ int check_dtype(int dtype) {
   return failf(NRP_ERR_UNSUPPORTED, "dtype %d", dtype);
 }
 
-// The largest row and column counts of a product: the kernels round them up to
-// whole tiles and look a few tiles ahead in 32-bit indices.
+// The largest row and column counts of a product and columns of a LayerNorm: the
+// kernels round them up to whole tiles and look a few tiles ahead in 32-bit indices.
 constexpr int kMaxSize = INT32_MAX - 4095;
 int check_sizes(const char* what, std::initializer_list<int> sizes) {
   for (int n : sizes)
@@ -237,6 +237,7 @@ int nrp_layer_norm(nrp_context* ctx, void* stream, int dtype, const void* x, int
                    float* mean, float* rstd) {
   if (!ctx || !gamma || !beta || (rows && (!x || !y)) || rows < 0 || cols <= 0)
     return failf(NRP_ERR_INVALID, "invalid layer norm arguments");
+  if (int rc = check_sizes("layer norm", {cols})) return rc;
   if (rows && !mean != !rstd)
     return failf(NRP_ERR_INVALID, "layer norm: mean and rstd go together");
   if (!(eps >= 0.f)) return failf(NRP_ERR_INVALID, "layer norm: eps must not be negative");
@@ -258,6 +259,7 @@ int nrp_layer_norm(nrp_context* ctx, void* stream, int dtype, const void* x, int
 
 int nrp_layer_norm_backward_workspace(int64_t rows, int cols, int64_t* bytes) {
   if (!bytes || rows < 0 || cols <= 0) return failf(NRP_ERR_INVALID, "invalid layer norm size");
+  if (int rc = check_sizes("layer norm backward", {cols})) return rc;
   *bytes = 4 * nrp::norm_bwd_partials(rows, cols);
   return NRP_OK;
 }
@@ -269,6 +271,7 @@ int nrp_layer_norm_backward(nrp_context* ctx, void* stream, int dtype, const voi
                             int64_t workspace_bytes) {
   if (!ctx || !gamma || (rows && (!x || !dy || !mean || !rstd || !dx)) || rows < 0 || cols <= 0)
     return failf(NRP_ERR_INVALID, "invalid layer norm backward arguments");
+  if (int rc = check_sizes("layer norm backward", {cols})) return rc;
   if (!dgamma != !dbeta) return failf(NRP_ERR_INVALID, "layer norm: dgamma and dbeta go together");
   if (int rc = check_dtype(dtype)) return rc;
   if (x_scales)

@@ -856,15 +856,16 @@ __global__ void __launch_bounds__(256)
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int i = blockIdx.x * 32 + lane;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  const int64_t all = 2 * static_cast<int64_t>(cols);
   float s = 0.f;
-  if (i < 2 * cols) {
+  if (i < all) {
 #pragma unroll 8
-    for (int p = warp; p < parts; p += 8) s += partials[static_cast<int64_t>(p) * 2 * cols + i];
+    for (int p = warp; p < parts; p += 8) s += partials[p * all + i];
   }
   red[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && i < 2 * cols) {
+  if (warp == 0 && i < all) {
     s = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) s += red[w][lane];
@@ -1016,7 +1017,8 @@ cudaError_t bwd(const TX* x, const T* dy, T* dx, const BwdArgs& a, cudaStream_t 
                      a.mean, a.rstd, a.rows, a.cols, a.partials);
   }
   if (e != cudaSuccess || !a.dgamma) return e;
-  return launch_pdl(norm_bwd_sum_kernel, dim3((2 * a.cols + 31) / 32), dim3(256), 0, stream,
+  const auto grid = static_cast<unsigned>((2 * static_cast<int64_t>(a.cols) + 31) / 32);
+  return launch_pdl(norm_bwd_sum_kernel, dim3(grid), dim3(256), 0, stream,
                     static_cast<const float*>(a.partials), parts, a.cols, a.dgamma, a.dbeta);
 }
 

@@ -54,3 +54,18 @@ def test_weight_gradient_sizes(nrp, ctx, m, n, k):
     rc, msg = status(nrp, "nrp_fp8_linear_weight_grad", ctx[0], None, AT[0], AT[1], AT[2], m, n, k,
                      F32, AT[3], AT[4])
     assert rc == UNSUPPORTED and "size" in msg
+
+
+@pytest.mark.parametrize("cols", [MOST + 1, 2 ** 31 - 2048, 2 ** 31 - 1])
+def test_norm_columns(nrp, ctx, cols):
+    """The last columns' indices would pass 2^31 and come back negative."""
+    p = ctx[0]
+    rc, msg = status(nrp, "nrp_layer_norm", p, None, BF16, AT[0], 1, cols, AT[1], AT[2], 1e-5, AT[3],
+                     AT[4], AT[5])
+    assert rc == UNSUPPORTED and "size" in msg
+    n = C.c_int64()
+    rc, msg = status(nrp, "nrp_layer_norm_backward_workspace", 1, cols, C.byref(n))
+    assert rc == UNSUPPORTED and "size" in msg
+    rc, msg = status(nrp, "nrp_layer_norm_backward", p, None, BF16, AT[0], None, AT[1], AT[2], AT[3],
+                     AT[4], 1, cols, AT[5], AT[6], AT[7], AT[8], 1 << 40)
+    assert rc == UNSUPPORTED and "size" in msg

@@ -1,0 +1,44 @@
+"""What the 8-bit operators' and the LayerNorm's documentation allows beyond the
+ordinary calls: the ends of the sizes, scales of every f32 value, rows of very
+large values, profiling from several threads, autograd's view of the outputs.
+
+u = 2^-24 is half a step of f32."""
+import math
+
+import pytest
+
+from __graft_entry__ import load_package
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def nrp():
+    import torch
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    return load_package()
+
+
+def test_norm_gradient_of_a_billion_columns(nrp):
+    """One row whose dgamma and dbeta are more than 2^31 values together.  With
+    mean and rstd given, dgamma = dy u is two f32 roundings of u and one of the
+    product off, dbeta = dy exact."""
+    import torch
+    torch.cuda.empty_cache()
+    cols = 2 ** 30 + 24
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(1, cols, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    dy = torch.empty_like(x).normal_(generator=g)
+    gamma = torch.ones(cols, device="cuda")
+    mean, rstd = torch.full((1,), 0.25, device="cuda"), torch.full((1,), 1.5, device="cuda")
+    dx, dgamma, dbeta = nrp.layer_norm_backward(dy, x, mean, rstd, gamma)
+    for at in (slice(0, 1 << 20), slice(2 ** 29, 2 ** 29 + (1 << 20)), slice(cols - (1 << 20), cols)):
+        d, u = dy[0, at].double(), (x[0, at].double() - 0.25) * 1.5
+        assert ((dgamma[at].double() - d * u).abs() <= 4 * U * (d * u).abs()).all()
+        assert torch.equal(dbeta[at], dy[0, at].float())
+        assert dx[0, at].isfinite().all()
+    del x, dy, gamma, dx, dgamma, dbeta
+    torch.cuda.empty_cache()
