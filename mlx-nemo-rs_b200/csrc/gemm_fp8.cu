@@ -201,13 +201,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = uniform(ss->tmem_base);
   volatile int* abort_flag = &ss->abort;
+  // Whether a wait of this CTA has expired, alike in a warp's lanes: what follows
+  // is for whole warps.
+  auto aborted = [&] { return __any_sync(0xffffffffu, *abort_flag) != 0; };
   pdl_launch_dependents();
   pdl_wait();
 
   if (warp == 0) {
     // ---------------------------------------------------------- producer
     uint32_t it = 0;
-    for (int t = first; t < num_tiles && !*abort_flag; t += step) {
+    for (int t = first; t < num_tiles && !aborted(); t += step) {
       const int m0 = t / tiles_n * kBM, n0 = t % tiles_n * kBN;
       for (int b = 0; b < blocks; ++b, ++it) {
         const int s = it % kStages;
@@ -232,14 +235,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     // after an abort: the copies in flight land before the CTA goes
-    if (*abort_flag && lane == 0)
+    if (aborted() && lane == 0)
       for (uint32_t j = it > static_cast<uint32_t>(kStages) ? it - kStages : 0; j < it; ++j)
         mbar_wait(&ss->full[j % kStages], (j / kStages) & 1, nullptr, 0);
   } else if (warp == 1) {
     // -------------------------------------------------------- MMA issuer
     constexpr uint32_t idesc = idesc_e4m3_f32(kBM, kBN, kTrans ? 1 : 0);
     uint32_t it = 0;
-    for (int t = first; t < num_tiles && !*abort_flag; t += step) {
+    for (int t = first; t < num_tiles && !aborted(); t += step) {
       for (int b = 0; b < blocks; ++b, ++it) {
         const int s = it % kStages, buf = it % kBufs;
         if (!warp_mbar_wait(&ss->tempty[buf], ((it / kBufs) & 1) ^ 1, a.err, kDevTimeoutEpi) ||
@@ -265,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
     }
-    if (*abort_flag) {
+    if (aborted()) {
       if (elect_one()) umma_commit(&ss->drain);
       __syncwarp();
       mbar_wait(&ss->drain, 0, nullptr, 0);
@@ -318,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (first < num_tiles) prefetch(first, 0, 0, 0);
     commit();
     uint32_t it = 0;
-    for (int t = first; t < num_tiles && !*abort_flag; t += step) {
+    for (int t = first; t < num_tiles && !aborted(); t += step) {
       const int m0 = t / tiles_n * kBM, n0 = t % tiles_n * kBN + group * kHalfN;
       float acc[kHalfN];
 #pragma unroll
@@ -339,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float* sc = scales + sbuf * kScaleBuf;
         const float s =
             sc[lane * kScalePitch + b % kChunk] * sc[32 * kScalePitch + b % kChunk];
-        if (!mbar_wait(&ss->tfull[buf], (it / kBufs) & 1, a.err, kDevTimeoutMma)) {
+        if (!warp_mbar_wait(&ss->tfull[buf], (it / kBufs) & 1, a.err, kDevTimeoutMma)) {
           *abort_flag = 1;
           ok = false;
           break;

@@ -222,13 +222,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = uniform(ss->tmem_base);
   volatile int* abort_flag = &ss->abort;
+  // Whether a wait of this CTA has expired, alike in a warp's lanes: what follows
+  // is for whole warps.
+  auto aborted = [&] { return __any_sync(0xffffffffu, *abort_flag) != 0; };
   pdl_launch_dependents();
   pdl_wait();
 
   if (warp == 0) {
     // ---------------------------------------------------- producer of dy
     int i = 0;
-    for (; i < steps && !*abort_flag; ++i) {
+    for (; i < steps && !aborted(); ++i) {
       const int s = i % kStages;
       if (!warp_mbar_wait_hot(&ss->empty[s], ((i / kStages) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
         *abort_flag = 1;
@@ -243,13 +246,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     }
-    if (*abort_flag && lane == 0)  // the copies in flight land before the CTA goes
+    if (aborted() && lane == 0)  // the copies in flight land before the CTA goes
       for (int j = i > kStages ? i - kStages : 0; j < i; ++j)
         mbar_wait(&ss->full[j % kStages], (j / kStages) & 1, nullptr, 0);
   } else if (warp == 2) {
     // ------------------------------------------------- producer of the codes
     int i = 0;
-    for (; i < steps && !*abort_flag; ++i) {
+    for (; i < steps && !aborted(); ++i) {
       const int s = i % kStages;
       if (!warp_mbar_wait_hot(&ss->rempty[s], ((i / kStages) & 1) ^ 1, a.err, kDevTimeoutLoad)) {
         *abort_flag = 1;
@@ -261,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     }
-    if (*abort_flag && lane == 0)
+    if (aborted() && lane == 0)
       for (int j = i > kStages ? i - kStages : 0; j < i; ++j)
         mbar_wait(&ss->rfull[j % kStages], (j / kStages) & 1, nullptr, 0);
   } else if (warp == 1) {
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < steps; ++i) {
       const int s = i % kStages;
       const uint32_t parity = (i / kStages) & 1;
-      if (*abort_flag || !warp_mbar_wait_hot(&ss->full[s], parity, a.err, kDevTimeoutLoad) ||
+      if (aborted() || !warp_mbar_wait_hot(&ss->full[s], parity, a.err, kDevTimeoutLoad) ||
           !warp_mbar_wait_hot(&ss->deq[s], parity, a.err, kDevTimeoutLoad)) {
         *abort_flag = 1;
         break;
@@ -294,6 +297,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (elect_one()) umma_commit(&ss->done);
     __syncwarp();
+    // (the other warps wait at the CTA's barrier: its end bounds no wait)
+    if (!warp_mbar_wait(&ss->done, 0, a.err, kDevTimeoutMma)) *abort_flag = 1;
   } else if (warp >= kBiasWarp0 && warp < kDeqWarp0) {
     // ----------------------------------------------------------- bias sums
     // the tile's 8-column chunks kt, kt + tiles_k, ...: four to a round over
@@ -308,8 +313,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < 8; ++e) sum[j][e] = 0.f;
       for (int i = 0; i < steps; ++i) {
         const int s = i % kStages;
-        if (*abort_flag ||
-            !mbar_wait_hot(&ss->full[s], (i / kStages) & 1, a.err, kDevTimeoutLoad)) {
+        if (aborted() ||
+            !warp_mbar_wait_hot(&ss->full[s], (i / kStages) & 1, a.err, kDevTimeoutLoad)) {
           *abort_flag = 1;
           break;
         }
@@ -375,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Behind its first step of a segment, which the MMAs then find ready, a set
     // takes its quarter of the segment before.
     auto take_segment = [&](int b) -> bool {
-      if (!*abort_flag &&
+      if (!aborted() &&
           add_segment<kTN>(quarter, b > 1, &ss->seg_full, &ss->seg_empty, (b - 1) & 1, a.err))
         return true;
       *abort_flag = 1;
@@ -389,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int h = 0; h < kRowsT; ++h) sn[h] = sc[h];
       scales(i + kSets);
-      if (*abort_flag || !mbar_wait_hot(&ss->rfull[s], round & 1, a.err, kDevTimeoutLoad)) {
+      if (aborted() || !warp_mbar_wait_hot(&ss->rfull[s], round & 1, a.err, kDevTimeoutLoad)) {
         *abort_flag = 1;
         break;
       }
@@ -431,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // only the stores wait for the MMAs that still read the stage
-      if (!mbar_wait_hot(&ss->empty[s], (round & 1) ^ 1, a.err, kDevTimeoutLoad)) {
+      if (!warp_mbar_wait_hot(&ss->empty[s], (round & 1) ^ 1, a.err, kDevTimeoutLoad)) {
         *abort_flag = 1;
         break;
       }
@@ -453,15 +458,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     // a last segment too short for this set to have a step in it
-    if (taken < (steps - 1) / kSeg && !*abort_flag) take_segment((steps - 1) / kSeg);
+    if (taken < (steps - 1) / kSeg && !aborted()) take_segment((steps - 1) / kSeg);
   }
 
   // ------------------------------------------------------------- the result
-  __syncwarp();
-  const bool fine = mbar_wait_hot(&ss->done, 0, a.err, kDevTimeoutMma);
-  if (!fine) *abort_flag = 1;
-  tc_fence_after();
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  // After an expired wait (the context's error word names it) this CTA's sums are
+  // NaN, in its tile or its share of one.
+  const bool lost = *abort_flag != 0;
   const int quad = warp & 3, grp = warp >> 2;  // 32 columns of n at a time
   const bool storer = threadIdx.x < kStoreThreads;
   const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16);
@@ -477,13 +483,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int e = 0; e < 16; ++e)
         v[h + e] = __uint_as_float(r[e]) + (steps > kSeg ? __uint_as_float(t[e]) : 0.f);
     }
+    if (lost) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(0x7fc00000u);
+    }
   };
+  if (lost && threadIdx.x < kTN) sBias[threadIdx.x] = __uint_as_float(0x7fc00000u);
   TO* dw = static_cast<TO*>(a.dw);
   TO* db = static_cast<TO*>(a.db);
   // bias columns this CTA summed (this rank writes its share of them)
   auto bias_here = [&](int c) { return db && (c >> 3) % tiles_k == kt && n0 + c < a.N; };
   if (a.split == 1) {
-    if (!*abort_flag && storer) {
+    if (storer) {
       const int k = k0 + quad * 32 + lane;
 #pragma unroll 1
       for (int c = grp * 32; c < kTN; c += 128) {
