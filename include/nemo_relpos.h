@@ -24,7 +24,9 @@
  *   - every call that launches work makes its context's device current on
  *     the calling thread (nrp_attn_forward_noalloc restores the caller's);
  *   - a handle is used by one host thread at a time (the reference's
- *     `&mut self` methods); one device per context.
+ *     `&mut self` methods); one device per context.  Of the calls on a context
+ *     alone, nrp_fp8_*, nrp_layer_norm*, nrp_profile_* and nrp_context_check
+ *     may come from several threads at once.
  */
 #ifndef NEMO_RELPOS_H
 #define NEMO_RELPOS_H

@@ -19,6 +19,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import os
+import threading
 from dataclasses import dataclass
 from typing import Dict, Optional, Tuple
 
@@ -215,6 +216,7 @@ class Context:
     """One CUDA device (nrp_context)."""
 
     _default: Dict[int, "Context"] = {}
+    _default_lock = threading.Lock()
 
     def __init__(self, device: int = 0):
         h = C.c_void_p()
@@ -224,9 +226,10 @@ class Context:
 
     @classmethod
     def default(cls, device: int = 0) -> "Context":
-        if device not in cls._default:
-            cls._default[device] = Context(device)
-        return cls._default[device]
+        with cls._default_lock:  # (making one releases the GIL)
+            if device not in cls._default:
+                cls._default[device] = Context(device)
+            return cls._default[device]
 
     def set_weight_cache(self, enable: bool = True):
         """Keep each quantised weight's bf16 copy for linears of >= 256 rows

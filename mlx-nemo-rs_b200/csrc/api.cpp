@@ -88,7 +88,7 @@ using nrp::bf16_round;
 
 namespace {
 
-// Folds finished records into the per-kind totals.
+// Folds finished records into the per-kind totals (with prof_mu held).
 int prof_collect(nrp_context* c) {
   for (auto& r : c->recs) {
     cudaError_t e = cudaEventSynchronize(r.stop);
@@ -571,7 +571,10 @@ int nrp_context_create(int device, nrp_context** out) {
 int nrp_context_destroy(nrp_context* ctx) {
   if (!ctx) return ok();
   cudaSetDevice(ctx->device);  // (errors of this teardown are dropped below)
-  prof_collect(ctx);
+  {
+    std::lock_guard<std::mutex> lock(ctx->prof_mu);
+    prof_collect(ctx);
+  }
   for (cudaEvent_t e : ctx->pool) cudaEventDestroy(e);
   if (ctx->side) {
     cudaStreamSynchronize(ctx->side);
@@ -1371,6 +1374,7 @@ int nrp_profile_enable(nrp_context* ctx, int enable) {
 
 int nrp_profile_reset(nrp_context* ctx) {
   if (!ctx) return fail(NRP_ERR_INVALID, "null context");
+  std::lock_guard<std::mutex> lock(ctx->prof_mu);
   int rc = prof_collect(ctx);
   for (int k = 0; k < NRP_KERNEL_KINDS; ++k) {
     ctx->prof_ms[k] = 0.0;
@@ -1384,6 +1388,7 @@ int nrp_profile_launches(nrp_context* ctx, int* kinds, float* ms, int64_t capaci
                          int64_t* count) {
   if (!ctx || !count || capacity < 0 || (capacity > 0 && (!kinds || !ms)))
     return fail(NRP_ERR_INVALID, "invalid profile log arguments");
+  std::lock_guard<std::mutex> lock(ctx->prof_mu);
   int rc = prof_collect(ctx);
   if (rc) return rc;
   const int64_t n = static_cast<int64_t>(ctx->prof_log.size());
@@ -1397,6 +1402,7 @@ int nrp_profile_launches(nrp_context* ctx, int* kinds, float* ms, int64_t capaci
 
 int nrp_profile_read(nrp_context* ctx, int kind, int64_t* launches, double* total_ms) {
   if (!ctx || kind < 0 || kind >= NRP_KERNEL_KINDS) return fail(NRP_ERR_INVALID, "bad kernel kind");
+  std::lock_guard<std::mutex> lock(ctx->prof_mu);
   int rc = prof_collect(ctx);
   if (rc) return rc;
   if (launches) *launches = ctx->prof_n[kind];

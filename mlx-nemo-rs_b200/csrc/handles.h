@@ -4,8 +4,10 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <memory>
+#include <mutex>
 #include <unordered_map>
 #include <utility>
 #include <vector>
@@ -77,7 +79,10 @@ struct nrp_context {
   int num_sms = 148;
   int* d_err = nullptr;
   uint32_t sched_seq = 0;
-  bool prof = false;
+  // The launch timing; prof_mu guards what follows `prof`, since the calls that
+  // keep no other state of the context may come from several threads.
+  std::atomic<bool> prof{false};
+  std::mutex prof_mu;
   std::vector<nrp::ProfRec> recs;
   std::vector<cudaEvent_t> pool;
   double prof_ms[NRP_KERNEL_KINDS] = {};

@@ -35,10 +35,13 @@ inline float bf16_round(float x) {
 int failf(int code, const char* fmt, ...);
 
 inline cudaEvent_t take_event(nrp_context* c) {
-  if (!c->pool.empty()) {
-    cudaEvent_t e = c->pool.back();
-    c->pool.pop_back();
-    return e;
+  {
+    std::lock_guard<std::mutex> lock(c->prof_mu);
+    if (!c->pool.empty()) {
+      cudaEvent_t e = c->pool.back();
+      c->pool.pop_back();
+      return e;
+    }
   }
   cudaEvent_t e = nullptr;
   cudaEventCreate(&e);
@@ -52,7 +55,7 @@ struct ProfScope {
   cudaStream_t st;
   cudaEvent_t a = nullptr;
   ProfScope(nrp_context* c_, int kind_, cudaStream_t st_) : c(c_), kind(kind_), st(st_) {
-    if (c && c->prof) {
+    if (c && c->prof.load(std::memory_order_relaxed)) {
       a = take_event(c);
       cudaEventRecord(a, st);
     }
@@ -61,6 +64,7 @@ struct ProfScope {
     if (a) {
       cudaEvent_t b = take_event(c);
       cudaEventRecord(b, st);
+      std::lock_guard<std::mutex> lock(c->prof_mu);
       c->recs.push_back({kind, a, b});
     }
   }

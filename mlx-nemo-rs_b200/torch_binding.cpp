@@ -196,8 +196,12 @@ nrp_context* context_of(PyObject* ctx, int dev) {
   if (!g_handle[dev]) {
     PyObject* c = PyObject_CallFunction(g_default_context, "i", dev);
     if (!c) throw PythonError{};
-    g_context[dev] = c;  // (the reference stays)
-    g_handle[dev] = handle_of(c, dev);
+    if (g_handle[dev]) {  // another thread came here meanwhile
+      Py_DECREF(c);
+    } else {
+      g_handle[dev] = handle_of(c, dev);
+      g_context[dev] = c;  // (the reference stays)
+    }
   }
   return g_handle[dev];
 }

@@ -69,3 +69,26 @@ def test_norm_columns(nrp, ctx, cols):
     rc, msg = status(nrp, "nrp_layer_norm_backward", p, None, BF16, AT[0], None, AT[1], AT[2], AT[3],
                      AT[4], 1, cols, AT[5], AT[6], AT[7], AT[8], 1 << 40)
     assert rc == UNSUPPORTED and "size" in msg
+
+
+def test_default_context_of_threads(nrp, monkeypatch):
+    """Threads that ask for a device's default context at once get the same one
+    (its making releases the GIL)."""
+    import threading
+    import time
+    made = []
+
+    def slow(self, device=0):
+        time.sleep(0.05)
+        self.handle, self.device = None, device
+        made.append(self)
+
+    monkeypatch.setattr(nrp.Context, "__init__", slow)
+    monkeypatch.setattr(nrp.Context, "_default", {})
+    got = []
+    ts = [threading.Thread(target=lambda: got.append(nrp.Context.default(3))) for _ in range(4)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert len(made) == 1 and all(c is made[0] for c in got) and len(got) == 4

@@ -42,3 +42,43 @@ def test_norm_gradient_of_a_billion_columns(nrp):
         assert dx[0, at].isfinite().all()
     del x, dy, gamma, dx, dgamma, dbeta
     torch.cuda.empty_cache()
+
+
+def test_threads_with_profiling(nrp):
+    """Four threads on one context with the launch timing on, and a fifth that
+    reads it: every launch is counted once, and the results stay the same."""
+    import threading
+    import torch
+    ctx = nrp.Context(0)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(40, 512, device="cuda", generator=g).bfloat16()
+    gamma, beta = torch.rand(512, device="cuda"), torch.rand(512, device="cuda")
+    w = nrp.fp8_quantize(torch.randn(256, 512, device="cuda", generator=g), 128)
+    want = nrp.fp8_linear(nrp.layer_norm(x, gamma, beta)[0], w)
+    torch.cuda.synchronize()
+    turns, threads, wrong = 60, 4, []
+
+    def work():
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(turns):
+                y = nrp.fp8_linear(nrp.layer_norm(x, gamma, beta, ctx=ctx)[0], w, ctx=ctx)
+                st.synchronize()
+                if not torch.equal(y, want):
+                    wrong.append(y)
+
+    ctx.profile_reset()
+    ctx.profile(True)
+    ts = [threading.Thread(target=work) for _ in range(threads)]
+    for t in ts:
+        t.start()
+    while any(t.is_alive() for t in ts):
+        ctx.profile_read()
+    for t in ts:
+        t.join()
+    ctx.profile(False)
+    read = ctx.profile_read()
+    assert not wrong
+    assert {k: n for k, (n, _) in read.items()} == {
+        "layernorm": turns * threads, "fp8_quant": turns * threads, "gemm_fp8": turns * threads}
+    ctx.check()
