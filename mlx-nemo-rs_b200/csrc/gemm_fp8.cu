@@ -9,7 +9,8 @@
 // into a TMEM accumulator, and the epilogue warps read it, multiply by the two
 // scales' product (one number per row and 128 columns) and add to f32
 // registers; TMEM holds two to four accumulators, so the next blocks run
-// meanwhile.  The scales may be any f32 values.
+// meanwhile.  The scales may be any f32 values: where their product leaves f32's
+// range, a sum is multiplied by one after the other.
 //
 // The weight is stored once, [out, in].  The forward product reads it with
 // the reduction contiguous (K-major B operand); the input's gradient reduces
@@ -33,6 +34,7 @@
 #include <algorithm>
 
 #include "fp8.h"
+#include "fp8_scales.cuh"
 #include "sm100.cuh"
 
 namespace nrp {
@@ -340,8 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
         const float* sc = scales + sbuf * kScaleBuf;
-        const float s =
-            sc[lane * kScalePitch + b % kChunk] * sc[32 * kScalePitch + b % kChunk];
+        const float s = sc[lane * kScalePitch + b % kChunk] * sc[32 * kScalePitch + b % kChunk];
         if (!warp_mbar_wait(&ss->tfull[buf], (it / kBufs) & 1, a.err, kDevTimeoutMma)) {
           *abort_flag = 1;
           ok = false;
@@ -350,9 +351,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t taddr =
             tmem + (static_cast<uint32_t>(quad * 32) << 16) + buf * kBN + group * kHalfN;
-        // 16 columns are added up while the next 16 come from TMEM
         uint32_t r[2][16];
         tmem_ld16(taddr, r[0]);
+        if (__any_sync(0xffffffffu, !scale_in_range(s))) {
+          // (a loop of its own: a branch in the one below makes it spill)
+          float p, q;
+          scale_factors(sc[lane * kScalePitch + b % kChunk], sc[32 * kScalePitch + b % kChunk], p,
+                        q);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < kHalfN; c += 16) {
+            tmem_ld16(taddr + c, r[1]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              acc[c + e] = fmaf(__uint_as_float(r[1][e]) * p, q, acc[c + e]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ss->tempty[buf]);
+          continue;
+        }
+        // 16 columns are added up while the next 16 come from TMEM
 #pragma unroll
         for (int c = 0; c < kHalfN; c += 16) {
           uint32_t(&cur)[16] = r[(c / 16) & 1];

@@ -20,6 +20,7 @@
 
 #include "fp8.h"
 #include "fp8_quant.cuh"
+#include "fp8_scales.cuh"
 
 namespace nrp {
 namespace {
@@ -100,8 +101,8 @@ __global__ void __launch_bounds__(kThreads) fp8_small_kernel(const Args a) {
   if (warp < nb) load_w(w, warp);
 
   // x's codes and scales: eight lanes of 16 columns to a block, columns past K
-  // as zeros (the last block's 64-byte pieces are read whole).  Tokens past M
-  // stay undefined: their results are not stored.
+  // as zeros (the last block's 64-byte pieces are read whole).  The codes of tokens
+  // past M stay undefined, as their results are not stored; their scales are 1.
   // The 32 lane groups of a pass tile (token, block) by powers of two.
   constexpr int kFly = sizeof(T) == 4 ? 2 : 4;
   const int sub = threadIdx.x & 7;
@@ -148,6 +149,8 @@ __global__ void __launch_bounds__(kThreads) fp8_small_kernel(const Args a) {
         }
       }
     }
+  for (int u = threadIdx.x; u < nb * kTok; u += kThreads)
+    if (u % kTok >= a.M) ss[u] = 1.f;
   __syncthreads();
 
   float acc[kRT][kNT][4];
@@ -185,18 +188,38 @@ __global__ void __launch_bounds__(kThreads) fp8_small_kernel(const Args a) {
       }
     }
     if (b + kWarps < nb) load_w(w, b + kWarps);
+    float s[kNT][2];
+    bool in_range = true;
 #pragma unroll
     for (int j = 0; j < kNT; ++j) {
       const float2 xsc = *reinterpret_cast<const float2*>(ss + b * kTok + 8 * j + 2 * t);
-      const float s0 = wscale * xsc.x, s1 = wscale * xsc.y;
+      s[j][0] = wscale * xsc.x;
+      s[j][1] = wscale * xsc.y;
+      in_range &= scale_in_range(s[j][0]) & scale_in_range(s[j][1]);
+    }
+    if (!in_range) {
+#pragma unroll
+      for (int j = 0; j < kNT; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float p;
+          scale_factors(ss[b * kTok + 8 * j + 2 * t + h], wscale, p, s[j][h]);
+#pragma unroll
+          for (int i = 0; i < kRT; ++i) {
+            c[i][j][h] *= p;
+            c[i][j][2 + h] *= p;
+          }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kNT; ++j)
 #pragma unroll
       for (int i = 0; i < kRT; ++i) {
-        acc[i][j][0] = fmaf(c[i][j][0], s0, acc[i][j][0]);
-        acc[i][j][1] = fmaf(c[i][j][1], s1, acc[i][j][1]);
-        acc[i][j][2] = fmaf(c[i][j][2], s0, acc[i][j][2]);
-        acc[i][j][3] = fmaf(c[i][j][3], s1, acc[i][j][3]);
+        acc[i][j][0] = fmaf(c[i][j][0], s[j][0], acc[i][j][0]);
+        acc[i][j][1] = fmaf(c[i][j][1], s[j][1], acc[i][j][1]);
+        acc[i][j][2] = fmaf(c[i][j][2], s[j][0], acc[i][j][2]);
+        acc[i][j][3] = fmaf(c[i][j][3], s[j][1], acc[i][j][3]);
       }
-    }
   }
   // the warps' partial sums, [token][row], in warp order
 #pragma unroll

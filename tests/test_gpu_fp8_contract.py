@@ -22,6 +22,88 @@ def nrp():
     return load_package()
 
 
+def values(q):
+    """float64 values of an Fp8Tensor on the CPU."""
+    c, s = q.codes.cpu().double(), q.scales.cpu().double()
+    s = s.repeat_interleave(q.block_rows, 0)[:c.shape[0]].repeat_interleave(128, 1)
+    return c * s[:, :c.shape[1]]
+
+
+def codes(shape, top, seed):
+    """e4m3 codes of magnitude up to `top`, an eighth of them zeros."""
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    v = (torch.rand(shape, generator=g) * 2 - 1) * top
+    v[torch.rand(shape, generator=g) < 0.125] = 0
+    return v.to(torch.float8_e4m3fn).cuda()
+
+
+# (exponents of x's and the weight's scales, largest code): products of scales
+# above and below f32's range whose block sums lie in it, and one of each kind in
+# range
+FAR = [(100, 30, 2.0 ** -7), (64, 66, 2.0 ** -7), (119, 119, 0.0), (-80, -70, 448.0),
+       (-117, -20, 448.0), (-20, -117, 448.0), (-117, -117, 448.0), (119, -110, 448.0),
+       (-110, 119, 448.0)]
+
+
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("m", [3, 20, 40, 300])
+def test_products_of_far_scales(nrp, m, trans):
+    """Rows and blocks whose scales' product leaves f32's range beside ordinary
+    ones.  Tolerance: as for other products 132 additions cut at 2^-23 within a
+    block, here two f32 roundings of a block's sum and its addition, and half of the
+    smallest f32 number for each of those."""
+    import torch
+    red, cols = 256 + 16, 192
+    blocks = 3
+    for ex, ew, top in FAR:
+        x = nrp.Fp8Tensor(codes((m, red), top, 1), torch.ones(m, blocks, device="cuda"), 1)
+        wshape = (red, cols) if trans else (cols, red)
+        w = nrp.Fp8Tensor(codes(wshape, top, 2),
+                          torch.ones([-(-n // 128) for n in wshape], device="cuda"), 128)
+        x.scales[:, 1] = 2.0 ** ex  # the middle block of the reduction
+        if trans:
+            w.scales[1] = 2.0 ** ew
+        else:
+            w.scales[:, 1] = -(2.0 ** ew)
+        x.scales[m // 2, 1] = 2.0 ** -ew  # one row's product is 1
+        xv, wv = values(x), values(w) if trans else values(w).t()
+        if abs(ex + ew) > 100:  # the far block by itself
+            for t in (x.scales, w.scales):
+                t[torch.where(t == 1)] = 0.0
+            xv, wv = values(x), values(w) if trans else values(w).t()
+        ref, size = xv @ wv, xv.abs() @ wv.abs()
+        assert (size < 3e38).all()
+        call = nrp.fp8_linear_input_grad if trans else nrp.fp8_linear
+        y = call(x, w, dtype=torch.float32).double().cpu()
+        tol = size * (132 * 2.0 ** -23 + 8 * U) + 3 * blocks * 2.0 ** -149
+        assert ((y - ref).abs() <= tol).all(), (ex, ew, float(((y - ref).abs() / tol).max()))
+
+
+@pytest.mark.parametrize("m", [3, 300])
+def test_zero_and_non_finite_scales(nrp, m):
+    """A zero scale gives zeros whatever the other's size, an infinite or NaN one
+    reaches its row (or its 128 features) only."""
+    import torch
+    x = nrp.fp8_quantize(torch.ones(m, 256, device="cuda"))
+    w = nrp.fp8_quantize(torch.ones(256, 256, device="cuda"), 128)
+    w.scales.fill_(2.0 ** 119)
+    x.scales.zero_()
+    assert (nrp.fp8_linear(x, w) == 0).all() and (nrp.fp8_linear_input_grad(x, w) == 0).all()
+    w.scales.fill_(1.0)
+    x.scales.fill_(1.0)
+    x.scales[1, 1] = float("inf")
+    x.scales[2, 0] = float("nan")
+    y = nrp.fp8_linear(x, w, dtype=torch.float32)
+    assert (y[1] == float("inf")).all() and y[2].isnan().all()
+    rest = torch.cat([y[:1], y[3:]])
+    assert rest.isfinite().all()
+    x.scales.fill_(1.0)
+    w.scales[1, 0] = float("nan")
+    y = nrp.fp8_linear(x, w)
+    assert y[:, 128:].isnan().all() and y[:, :128].isfinite().all()
+
+
 def test_norm_gradient_of_a_billion_columns(nrp):
     """One row whose dgamma and dbeta are more than 2^31 values together.  With
     mean and rstd given, dgamma = dy u is two f32 roundings of u and one of the
