@@ -148,8 +148,15 @@ __global__ void __launch_bounds__(256)
       const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
           static_cast<__nv_fp8x2_storage_t>((w[e >> 1] >> (16 * (e & 1))) & 0xffffu), __NV_E4M3);
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-      v[2 * e] = f.x * s;
-      v[2 * e + 1] = f.y * s;
+      v[2 * e] = f.x;
+      v[2 * e + 1] = f.y;
+    }
+    if (sizeof(T) == 4 || is_power_of_two(s)) {  // f32 holds the product
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] *= s;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = code_times(v[e], s);
     }
     T* o = x + row * cols + col;
     if constexpr (sizeof(T) == 4) {

@@ -108,6 +108,20 @@ __device__ __forceinline__ uint4 codes16(const uint4* raw, float inv, bool finit
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// code * scale on its way to bf16: cut off to f32, with the last bit set where that
+// loses some of the product's up to 28 bits, so that the rounding to bf16 is the only
+// one (rounded to f32 first, one product in 2^17 lands on a tie that it is not).
+__device__ __forceinline__ float code_times(float code, float scale) {
+  const float v = __fmul_rz(code, scale);
+  return __fmul_ru(code, scale) == __fmul_rd(code, scale)
+             ? v
+             : __uint_as_float(__float_as_uint(v) | 1u);
+}
+// A power of two, whose products with codes f32 holds.
+__device__ __forceinline__ bool is_power_of_two(float scale) {
+  return (__float_as_uint(scale) & 0x807fffffu) == 0;
+}
+
 // A 1 x 128 block held by eight lanes (a quarter of a warp), 16 elements each
 // (zeros off its end): the lane's codes and, in all eight, the scale.
 template <typename T>

@@ -44,6 +44,7 @@
 #include <cuda_fp8.h>
 
 #include "fp8.h"
+#include "fp8_quant.cuh"
 #include "sm100.cuh"
 
 namespace nrp {
@@ -413,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                flip ? q[h].x : q[h].z, flip ? q[h].y : q[h].w};
         uint32_t(&o)[8] = out[h];
         // a power of two in [2^-117, 2^7] and no NaN code: the product is
-        // exact, by bits; anything else through f32 (rounded once)
+        // exact, by bits; anything else rounded once
         const uint32_t fb = __float_as_uint(f);
         const bool nan = has_nan_code(w[0]) | has_nan_code(w[1]) | has_nan_code(w[2]) |
                          has_nan_code(w[3]);
@@ -431,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 static_cast<__nv_fp8x2_storage_t>((w[e >> 1] >> (16 * (e & 1))) & 0xffffu),
                 __NV_E4M3);
             const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hr));
-            o[e] = pack_bf16x2(v.x * f, v.y * f);
+            o[e] = pack_bf16x2(code_times(v.x, f), code_times(v.y, f));
           }
         }
       }

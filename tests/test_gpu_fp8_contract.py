@@ -3,8 +3,7 @@ ordinary calls: the ends of the sizes, scales of every f32 value, rows of very
 large values, profiling from several threads, autograd's view of the outputs.
 
 u = 2^-24 is half a step of f32."""
-import math
-
+import numpy as np
 import pytest
 
 from __graft_entry__ import load_package
@@ -27,6 +26,74 @@ def values(q):
     c, s = q.codes.cpu().double(), q.scales.cpu().double()
     s = s.repeat_interleave(q.block_rows, 0)[:c.shape[0]].repeat_interleave(128, 1)
     return c * s[:, :c.shape[1]]
+
+
+def bf16(v):
+    """float64 numpy values rounded once to bf16 (torch's conversion goes through
+    f32), as float64."""
+    _, e = np.frexp(v)
+    step = np.exp2(np.maximum(e - 8, -133).astype(np.float64))
+    return np.where(np.isfinite(v), np.round(v / step) * step, v)
+
+
+def scales_on_ties():
+    """Scales and codes whose product, rounded to f32 first, lands on a tie of bf16
+    that it is not, with the other scales of the same draw."""
+    g = np.random.default_rng(5)
+    s = (g.integers(2 ** 23, 2 ** 24, 1 << 22) * 2.0 ** -30).astype(np.float32)
+    found = []
+    for c in (9.0, 11.0, 13.0, 15.0):
+        v = s.astype(np.float64) * c
+        off = bf16(v) != bf16(v.astype(np.float32).astype(np.float64))
+        found += [(float(x), c) for x in s[off][:16]]
+    assert len(found) == 64
+    return found
+
+
+def test_values_are_rounded_once(nrp):
+    """Codes times scales of 24 bits in bf16, by fp8_dequantize and on the weight
+    gradient's way into its products (dy the identity: dw is x^)."""
+    import torch
+    pairs = scales_on_ties()
+    q = nrp.Fp8Tensor(codes((64, 128), 448.0, 1), torch.tensor([[s] for s, _ in pairs]).cuda(), 1)
+    q.codes[:, 0] = torch.tensor([c for _, c in pairs]).to(torch.float8_e4m3fn).cuda()
+    q.scales[5:9] *= -1
+    want = torch.from_numpy(bf16(values(q).numpy()))
+    assert not torch.equal(values(q).float().bfloat16().double(), want)  # (through f32)
+    assert torch.equal(nrp.fp8_dequantize(q).double().cpu(), want)
+    dw, _ = nrp.fp8_linear_weight_grad(torch.eye(64, device="cuda", dtype=torch.bfloat16), q)
+    assert torch.equal(dw.double().cpu(), want)
+
+
+@pytest.mark.parametrize("m,k,n", [(3, 16, 8), (70, 272, 264), (515, 400, 2000), (749, 1024, 1024),
+                                   (2500, 256, 256), (5000, 560, 120), (1, 1040, 2504)])
+def test_weight_gradient_of_any_scales(nrp, m, k, n):
+    """Scales of any size and sign beside the quantiser's in one tile, a zero one, and
+    a NaN code that reaches its column only: against the products of the values
+    rounded to bf16, within (m + m/16 + 16) additions cut at 2^-23."""
+    import torch
+    g = torch.Generator().manual_seed(m)
+    blocks = -(-k // 128)
+    scales = torch.randn(m, blocks, generator=g) * torch.exp2(torch.randn(m, blocks, generator=g) * 6)
+    tame = torch.rand(m, blocks, generator=g) < 0.5
+    scales[tame] = torch.exp2(torch.randint(-20, 20, (m, blocks), generator=g).float())[tame]
+    scales[m // 2] = 0.0
+    q = nrp.Fp8Tensor(codes((m, k), 448.0, 2), scales.cuda(), 1)
+    dy = (torch.randn(m, n, generator=g) * 1e-3).bfloat16()
+    x, d = torch.from_numpy(bf16(values(q).numpy())), dy.double()
+    ref, size = d.t() @ x, d.abs().t() @ x.abs()
+    tol = size * (m + m / 16 + 16) * 2.0 ** -23
+    for bias in (False, True):
+        dw, _ = nrp.fp8_linear_weight_grad(dy.cuda(), q, bias=bias)
+        assert ((dw.double().cpu() - ref).abs() <= tol + ref.abs() * U).all()
+    q.codes.view(torch.uint8)[m - 1, k - 3] = 0xFF
+    q.codes.view(torch.uint8)[m - 1, 1] = 0x7F
+    dw = nrp.fp8_linear_weight_grad(dy.cuda(), q)[0].cpu()
+    bad = torch.zeros(k, dtype=torch.bool)
+    bad[[k - 3, 1]] = True
+    assert dw[:, bad].isnan().all()
+    assert ((dw[:, ~bad].double() - ref[:, ~bad]).abs() <= (tol + ref.abs() * U)[:, ~bad]).all()
+    nrp.Context.default().check()
 
 
 def codes(shape, top, seed):
