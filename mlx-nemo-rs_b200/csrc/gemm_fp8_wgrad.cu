@@ -226,6 +226,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Whether a wait of this CTA has expired, alike in a warp's lanes: what follows
   // is for whole warps.
   auto aborted = [&] { return __any_sync(0xffffffffu, *abort_flag) != 0; };
+  // A lane's wait, given up at once when another of the CTA has expired; the lanes
+  // agree on it by `agreed`, at the latest where the warp comes together anyway.
+  auto lane_wait = [&](uint64_t* bar, uint32_t parity, int code) {
+    return !*abort_flag && mbar_wait_hot(bar, parity, a.err, code);
+  };
+  auto agreed = [&](bool fine) {
+    if (__all_sync(0xffffffffu, fine)) return true;
+    *abort_flag = 1;
+    return false;
+  };
   pdl_launch_dependents();
   pdl_wait();
 
@@ -314,11 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < 8; ++e) sum[j][e] = 0.f;
       for (int i = 0; i < steps; ++i) {
         const int s = i % kStages;
-        if (aborted() ||
-            !warp_mbar_wait_hot(&ss->full[s], (i / kStages) & 1, a.err, kDevTimeoutLoad)) {
-          *abort_flag = 1;
-          break;
-        }
+        const bool fine = lane_wait(&ss->full[s], (i / kStages) & 1, kDevTimeoutLoad);
 #pragma unroll
         for (int j = 0; j < kOwn; ++j) {
           const int c = c0 + j * cstep;
@@ -336,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         reads_done();
-        __syncwarp();
+        if (!agreed(fine)) break;
         if (lane == 0) mbar_arrive(&ss->empty[s]);
       }
 #pragma unroll
@@ -395,16 +401,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int h = 0; h < kRowsT; ++h) sn[h] = sc[h];
       scales(i + kSets);
-      if (aborted() || !warp_mbar_wait_hot(&ss->rfull[s], round & 1, a.err, kDevTimeoutLoad)) {
-        *abort_flag = 1;
-        break;
-      }
+      bool fine = lane_wait(&ss->rfull[s], round & 1, kDevTimeoutLoad);
       uint4 q[kRowsT];
 #pragma unroll
       for (int h = 0; h < kRowsT; ++h)
         q[h] = *reinterpret_cast<const uint4*>(sR + s * kRawBytes + (row + 16 * h) * 128 + c * 16);
       reads_done();
-      __syncwarp();
+      if (!agreed(fine)) break;
       if (lane == 0) mbar_arrive(&ss->rempty[s]);
       uint32_t out[kRowsT][8];
 #pragma unroll
@@ -437,10 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // only the stores wait for the MMAs that still read the stage
-      if (!warp_mbar_wait_hot(&ss->empty[s], (round & 1) ^ 1, a.err, kDevTimeoutLoad)) {
-        *abort_flag = 1;
-        break;
-      }
+      fine = lane_wait(&ss->empty[s], (round & 1) ^ 1, kDevTimeoutLoad);
       uint8_t* dst = sA + s * kABytes;
 #pragma unroll
       for (int h = 0; h < kRowsT; ++h) {
@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             make_uint4(out[h][4], out[h][5], out[h][6], out[h][7]);
       }
       fence_proxy_async_smem();
-      __syncwarp();
+      if (!agreed(fine)) break;
       if (lane == 0) mbar_arrive(&ss->deq[s]);
       if (i >= kSeg && i % kSeg < kSets) {
         if (!take_segment(i / kSeg)) break;
