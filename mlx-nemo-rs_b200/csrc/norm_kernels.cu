@@ -500,7 +500,8 @@ struct Batch {
       if (row < rows) {
         x[r].load(px + row * cols, col, cols);
         dy[r].load(pdy + row * cols, col, cols);
-        mu[r] = mean[row];
+        // (lanes past the columns keep u = 0, whatever the row's mean times rstd)
+        if (!kVec || col < cols) mu[r] = mean[row];
         rs[r] = rstd[row];
         // a lane's columns lie in one block (kVec), or in two
 #pragma unroll
@@ -630,6 +631,9 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
 #pragma unroll
   for (int e = 0; e < 4; ++e) ag[e] = ab[e] = both(0.f);
   lane_columns<kVec, kL>(gamma, col, cols, gm);
+  // columns of the lane's pair e
+  auto col0 = [&](int e) { return col + (kVec ? 2 * e : 2 * kL * e); };
+  auto col1 = [&](int e) { return col0(e) + (kVec ? 1 : kL); };
   int buf = 0;
   for (; first < rows; first += stride, buf ^= 1) {
     const int64_t row0 = first + own;
@@ -642,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
       const float* of_warp = reinterpret_cast<const float*>(at + kThreads * Rg::kBytes) + warp * 16;
 #pragma unroll
       for (int r = 0; r < kR; ++r) {
-        now.mu[r] = of_warp[r];
+        now.mu[r] = in ? of_warp[r] : 0.f;
         now.rs[r] = of_warp[4 + r];
         if constexpr (kCodes) now.sx[r][0] = of_warp[8 + r + 4 * (lane >> 4)];
         at = take_strip(at, kThreads, now.x[r]);
@@ -662,14 +666,12 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
       for (int e = 0; e < 4; ++e) {
         const F2 xv = {now.x[r].get(2 * e), now.x[r].get(2 * e + 1)};
         const F2 d = {now.dy[r].get(2 * e), now.dy[r].get(2 * e + 1)};
-        if constexpr (kCodes) {
-          // (code * scale - mean) * rstd with the constants multiplied first: a
-          // mean so large that its rounding shows here leaves eight bits nothing
-          const float k = now.sx[r][kVec || kL < 32 ? 0 : e >> 1] * now.rs[r];
-          u[r][e] = fma2(xv, both(k), both(-now.mu[r] * now.rs[r]));
-        } else {
-          u[r][e] = mul2(add2(xv, both(-now.mu[r])), both(now.rs[r]));
-        }
+        // (code * scale - mean) * rstd, the product exact in the fma
+        const F2 c = kCodes ? fma2(xv, both(now.sx[r][kVec || kL < 32 ? 0 : e >> 1]),
+                                   both(-now.mu[r]))
+                            : add2(xv, both(-now.mu[r]));
+        u[r][e] = mul2(c, both(now.rs[r]));
+        if (!kVec) u[r][e] = {col0(e) < cols ? u[r][e].a : 0.f, col1(e) < cols ? u[r][e].b : 0.f};
         ag[e] = fma2(d, u[r][e], ag[e]);
         ab[e] = add2(ab[e], d);
         g[r][e] = mul2(d, gm[e]);
@@ -679,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
       part[r] = c1.a + c1.b;
       part[kR + r] = c2.a + c2.b;
     }
-    // lanes past the columns hold x = 0 and dy = 0: nothing but zeros added
+    // columns past the end hold u = 0 and dy = 0: nothing but zeros added
     const float mine = warp_sums<kL>(part, lane);
     constexpr int kHold = kL / 2 / kR;  // lanes that hold each sum
     float s[2 * kR];
@@ -726,11 +728,10 @@ __global__ void __launch_bounds__(kThreads, kThreads == kManyThreads ? 2 : 1)
     }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int c0 = col + (kVec ? 2 * e : 2 * kL * e), c1 = c0 + (kVec ? 1 : kL);
     float* to = col_sums + 2 * grp * cols;
     if (lane >= kL) break;
-    if (c0 < cols) to[c0] = ag[e].a, to[cols + c0] = ab[e].a;
-    if (c1 < cols) to[c1] = ag[e].b, to[cols + c1] = ab[e].b;
+    if (col0(e) < cols) to[col0(e)] = ag[e].a, to[cols + col0(e)] = ab[e].a;
+    if (col1(e) < cols) to[col1(e)] = ag[e].b, to[cols + col1(e)] = ab[e].b;
   }
   __syncthreads();
   if (groups > 1) {
@@ -782,7 +783,7 @@ __global__ void __launch_bounds__(256)
       for (int e = 0; e < kE; ++e) {
         const float g = pd.v[e] * gm.v[e];
         c1 += g;
-        c2 = fmaf(g, (px.v[e] * k - mu) * rs, c2);
+        c2 = fmaf(g, fmaf(px.v[e], k, -mu) * rs, c2);
       }
     }
     c1 = block_sum(c1, part) / static_cast<float>(cols);
@@ -794,7 +795,7 @@ __global__ void __launch_bounds__(256)
       const float k = scale(c);
 #pragma unroll
       for (int e = 0; e < kE; ++e)
-        pd.v[e] = rs * (pd.v[e] * gm.v[e] - c1 - (px.v[e] * k - mu) * rs * c2);
+        pd.v[e] = rs * (pd.v[e] * gm.v[e] - c1 - fmaf(px.v[e], k, -mu) * rs * c2);
       put_piece<kVec>(dx + row * cols + c, pd.v);
     }
   }
@@ -827,7 +828,7 @@ __global__ void __launch_bounds__(256)
       const float mu = mean[row], rs = rstd[row];
 #pragma unroll
       for (int e = 0; e < kE; ++e) {
-        ag[e] = fmaf(pd.v[e], (px.v[e] * k - mu) * rs, ag[e]);
+        ag[e] = fmaf(pd.v[e], fmaf(px.v[e], k, -mu) * rs, ag[e]);
         ab[e] += pd.v[e];
       }
     }

@@ -231,3 +231,53 @@ def test_threads_with_profiling(nrp):
     assert {k: n for k, (n, _) in read.items()} == {
         "layernorm": turns * threads, "fp8_quant": turns * threads, "gemm_fp8": turns * threads}
     ctx.check()
+
+
+@pytest.mark.parametrize("rows,cols", [(20, 512), (3000, 64), (700, 112), (2500, 1024), (600, 784),
+                                       (300, 2048), (50, 4096), (40, 6000)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("shift", [0, 16])
+def test_norm_gradient_of_codes_far_from_zero(nrp, rows, cols, dtype, shift):
+    """x in 8 bits, its mean up to a thousand spreads or so large that mean * rstd
+    passes f32: u = (code * scale - mean) * rstd has two roundings of the difference
+    in every kernel (not of the mean), which dgamma = dy u shows where one row alone
+    has gradients.  Kernels by elements: x shifted `shift` bytes off the allocation,
+    dy and dx by an element."""
+    import torch
+    dt = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    blocks, one = -(-cols // 128), rows - 3
+
+    def off(t):
+        held = torch.zeros(t.numel() + 1, device="cuda", dtype=t.dtype)
+        v = held[1:].view(t.shape) if shift else held[:-1].view(t.shape)
+        return v.copy_(t)
+
+    q = nrp.Fp8Tensor(codes((rows, cols), 448.0, 1),
+                      torch.randn(rows, blocks, device="cuda", generator=g), 1)
+    mean = torch.randn(rows, device="cuda", generator=g)
+    rstd = torch.exp2(torch.randn(rows, device="cuda", generator=g))
+    dy = torch.zeros(rows, cols, device="cuda", dtype=dt)
+    dy[one] = torch.randn(cols, device="cuda", generator=g)
+    dy = off(dy)
+    gamma = torch.randn(cols, device="cuda", generator=g)
+    even = torch.arange(cols, device="cuda") % 2 == 0
+    for top, scale, mu, r in ((448.0, 0.7, 0.7 * 448.4, 1.3), (448.0, 2.0 ** 91, 448 * 2.0 ** 91,
+                                                              2.0 ** 40)):
+        q.codes[one] = torch.where(even & (scale < 1), 416.0, top).to(torch.float8_e4m3fn)
+        q.scales[one], mean[one], rstd[one] = scale, mu, r
+        dx, dg, db = nrp.layer_norm_backward(dy, q, mean, rstd, gamma, out=off(dy))
+        x = q.codes[one].double() * q.scales[one].double().repeat_interleave(128)[:cols]
+        r = rstd[one].double()
+        u = (x - mean[one].double()) * r
+        d = dy[one].double()
+        assert ((dg.double() - d * u).abs() <= 4 * U * (d * u).abs()).all()
+        assert torch.equal(db.double(), d)
+        w = d * gamma.double()
+        ref = r * (w - w.mean() - u * (w * u).mean())
+        size = r * (w.abs() + w.abs().mean() + u.abs() * (w * u).abs().mean())
+        chain = cols / 32 + 20 if cols <= 2048 else cols / 256 + 20
+        assert ((dx[one].double() - ref).abs() <= size * chain * U
+                + ref.abs() * torch.finfo(dt).eps / 2).all()
+        dx[one] = 0
+        assert (dx == 0).all()
