@@ -6,7 +6,8 @@
 //   dgamma = sum_rows dy * u, dbeta = sum_rows dy
 //
 // in f32, each output rounded once.  The variance is summed about the mean
-// (two passes over the registers), so a large mean costs no precision.  The
+// (two passes over the registers), so a large mean costs it no digits; a row whose
+// sums overflow f32 is taken again in smaller units.  The
 // backward pass takes x as it was or as the e4m3 checkpoint (codes and one
 // scale per 128 columns), with the saved mean and rstd of the exact row.
 //
@@ -22,6 +23,7 @@
 // and codes 49 us with its second kernel (5.2 TB/s; instruction issue, at 60%,
 // comes close to being the bound), 749 x 512 bf16 6.2 us in two launches.
 #include <algorithm>
+#include <cfloat>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -213,6 +215,25 @@ __device__ __forceinline__ float warp_sums(const float (&v)[kN], int lane) {
   return a[0];
 }
 
+// Rows whose sum or sum of squares overflows f32 (a spread of about 2^64) are taken
+// again times 2^-84: the squares of any f32 values are then in range, over 2^31
+// columns too.
+constexpr float kFar = 0x1p-84f, kFarInv = 0x1p84f;
+__device__ __forceinline__ bool variance_overflows(float v) { return !(v <= FLT_MAX); }
+// 1 / sqrt(variance + eps) of a row, times 2^84, from the variance v of the row times
+// 2^-84.
+__device__ __forceinline__ float far_rstd(float v, float eps) {
+  if (v >= 0x1p-120f) return 1.f / sqrtf(v + eps * kFar * kFar);
+  return kFarInv / sqrtf(v * kFarInv * kFarInv + eps);  // next to no spread: the sum overflowed
+}
+
+// The row's mean from that of the row times 2^-84, which may have been rounded past
+// the largest value.
+__device__ __forceinline__ float far_mean(float m) {
+  return fabsf(m) <= FLT_MAX * kFar * 1.001f ? fminf(fmaxf(m * kFarInv, -FLT_MAX), FLT_MAX)
+                                             : m * kFarInv;
+}
+
 constexpr int kFwdThreads = 256;
 // CTAs per SM of a kernel that takes kR rows at a time (kR W <= 32).
 template <int kR, int kThreads>
@@ -251,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas<kR, kThreads>)
   lane_columns<kVec>(gamma, col, cols, gm);
   lane_columns<kVec>(beta, col, cols, bt);
   int buf = 0;
-  for (; row0 < rows; row0 += stride, buf ^= 1) {
+  for (; row0 < rows; row0 += stride) {
     F2 v[kR][4];
     float part[kR];
 #pragma unroll
@@ -267,28 +288,28 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas<kR, kThreads>)
     // (y may be x: these rows are in registers, and the next are others)
     load(row0 + stride);
     constexpr int kHold = 32 / kR;  // lanes that hold each sum
-    // lane l: the strip's mean of row l / kHold, then its sum of squares
-    const float mean_w = warp_sums(part, lane) * inv_n;
+    const int per = W == 1 ? kHold : Wp;  // ... and each row's when the strips are joined
     float mean[kR], rstd[kR];
+    // From the lane's sums of the rows: the rows' means and, in lane l, the variance of
+    // row l / per.
+    auto stats = [&]() {
+      // lane l: the strip's mean of row l / kHold, then its sum of squares
+      const float mean_w = warp_sums(part, lane) * inv_n;
 #pragma unroll
-    for (int r = 0; r < kR; ++r) mean[r] = __shfl_sync(0xffffffffu, mean_w, kHold * r);
+      for (int r = 0; r < kR; ++r) mean[r] = __shfl_sync(0xffffffffu, mean_w, kHold * r);
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {
-      F2 q = both(0.f);
+      for (int r = 0; r < kR; ++r) {
+        F2 q = both(0.f);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        F2 d = add2(v[r][e], both(-mean[r]));
-        if (!kVec) d = {c0(e) < cols ? d.a : 0.f, c1(e) < cols ? d.b : 0.f};
-        q = fma2(d, d, q);
+        for (int e = 0; e < 4; ++e) {
+          F2 d = add2(v[r][e], both(-mean[r]));
+          if (!kVec) d = {c0(e) < cols ? d.a : 0.f, c1(e) < cols ? d.b : 0.f};
+          q = fma2(d, d, q);
+        }
+        part[r] = !kVec || col < cols ? q.a + q.b : 0.f;  // (the others hold -mean)
       }
-      part[r] = !kVec || col < cols ? q.a + q.b : 0.f;  // (the others hold -mean)
-    }
-    const float m2_w = warp_sums(part, lane);
-    if (W == 1) {
-      const float rs = 1.f / sqrtf(m2_w * inv_c + eps);
-#pragma unroll
-      for (int r = 0; r < kR; ++r) rstd[r] = __shfl_sync(0xffffffffu, rs, kHold * r);
-    } else {
+      const float m2_w = warp_sums(part, lane);
+      if (W == 1) return m2_w * inv_c;
       if (lane % kHold == 0) red[buf][warp][lane / kHold] = make_float2(mean_w, m2_w);
       named_bar_sync(1 + grp, 32 * W);
       // lane (r, w) takes strip w's share of row r
@@ -299,13 +320,32 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas<kR, kThreads>)
       const float d = p.x - m;
       float t = fmaf(d * d, at_n, p.y);
       for (int o = Wp / 2; o; o /= 2) t += __shfl_xor_sync(0xffffffffu, t, o);
-      const float rs = 1.f / sqrtf(t * inv_c + eps);
+#pragma unroll
+      for (int r = 0; r < kR; ++r) mean[r] = __shfl_sync(0xffffffffu, m, Wp * r);
+      buf ^= 1;
+      return t * inv_c;
+    };
+    const float var = stats() + eps;
+    float rs = 1.f / sqrtf(var);
+    // (alike in a group's warps, which hold the same sums)
+    const uint32_t far = __ballot_sync(0xffffffffu, variance_overflows(var));
+    if (far) {
 #pragma unroll
       for (int r = 0; r < kR; ++r) {
-        mean[r] = __shfl_sync(0xffffffffu, m, Wp * r);
-        rstd[r] = __shfl_sync(0xffffffffu, rs, Wp * r);
+        const F2 f = both(far >> (per * r) & 1 ? kFar : 1.f);
+        F2 s = both(0.f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[r][e] = mul2(v[r][e], f);
+          s = add2(s, v[r][e]);
+        }
+        part[r] = s.a + s.b;
       }
+      const float far_var = stats();
+      if (far >> lane & 1) rs = far_rstd(far_var, eps);
     }
+#pragma unroll
+    for (int r = 0; r < kR; ++r) rstd[r] = __shfl_sync(0xffffffffu, rs, per * r);
 #pragma unroll
     for (int r = 0; r < kR; ++r) {
       if (row0 + r >= rows) break;
@@ -319,18 +359,44 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas<kR, kThreads>)
       }
       store_strip<T, kVec>(y + (row0 + r) * cols, col, cols, o);
       if (mean_out && strip == 0 && lane == 0) {
-        mean_out[row0 + r] = mean[r];
-        rstd_out[row0 + r] = rstd[r];
+        const bool up = far >> (per * r) & 1;
+        mean_out[row0 + r] = up ? far_mean(mean[r]) : mean[r];
+        rstd_out[row0 + r] = up ? rstd[r] * kFar : rstd[r];
       }
     }
+  }
+}
+
+// A row whose variance overflows, by a warp, x read three times.
+template <typename T>
+__device__ __noinline__ void far_row(const T* x, int cols, const float* gamma, const float* beta,
+                                     float eps, T* y, float* mean_out, float* rstd_out) {
+  const int lane = threadIdx.x & 31;
+  const float inv_c = 1.f / static_cast<float>(cols);
+  float s = 0.f, q = 0.f;
+  for (int c = lane; c < cols; c += 32) s = fmaf(get(x + c), kFar, s);
+  const float mean = warp_sum(s) * inv_c;
+  for (int c = lane; c < cols; c += 32) {
+    const float d = fmaf(get(x + c), kFar, -mean);
+    q = fmaf(d, d, q);
+  }
+  const float rstd = far_rstd(warp_sum(q) * inv_c, eps);
+  for (int c = lane; c < cols; c += 32)
+    put(y + c, fmaf(fmaf(get(x + c), kFar, -mean) * rstd, gamma[c], beta[c]));
+  if (lane == 0 && mean_out) {
+    *mean_out = far_mean(mean);
+    *rstd_out = rstd * kFar;
   }
 }
 
 // Columns or pointers that do not allow 16-byte loads: a warp's whole row, of at
 // most kCh strips, a lane's elements 32 apart.
 constexpr int kRowThreads = 128;
+// CTAs per SM by strips: 64, 48 and 40 registers.
+template <int kCh>
+constexpr int kRowCtas = kCh == 4 ? 8 : kCh == 2 ? 10 : 12;
 template <typename T, int kCh>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, kRowCtas<kCh>)
     norm_fwd_rows_kernel(const T* x, int64_t rows, int cols, const float* __restrict__ gamma,
                          const float* __restrict__ beta, float eps, T* y,
                          float* __restrict__ mean_out, float* __restrict__ rstd_out) {
@@ -360,7 +426,13 @@ __global__ void __launch_bounds__(kRowThreads)
       const float d = v[c].get(e) - mean;
       if (col_of(c, e) < cols) q = fmaf(d, d, q);
     }
-  const float rstd = 1.f / sqrtf(warp_sum(q) * inv_c + eps);
+  const float var = warp_sum(q) * inv_c + eps;
+  if (variance_overflows(var)) {  // (the whole warp)
+    far_row(x + row * cols, cols, gamma, beta, eps, y + row * cols,
+            mean_out ? mean_out + row : nullptr, mean_out ? rstd_out + row : nullptr);
+    return;
+  }
+  const float rstd = 1.f / sqrtf(var);
 #pragma unroll
   for (int c = 0; c < kCh; ++c) {
     float o[8];
@@ -425,30 +497,40 @@ __global__ void __launch_bounds__(256)
   pdl_wait();
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * cols;
-    float s = 0.f;
-    for (int c = threadIdx.x * kE; c < cols; c += 256 * kE) {
-      const Piece<T, kVec> p(xr + c);
+    float mean, rstd, f = 1.f;  // (f 1: the fma with it is an addition)
+    while (true) {
+      float s = 0.f;
+      for (int c = threadIdx.x * kE; c < cols; c += 256 * kE) {
+        const Piece<T, kVec> p(xr + c);
 #pragma unroll
-      for (int e = 0; e < kE; ++e) s += p.v[e];
-    }
-    const float mean = block_sum(s, part) / static_cast<float>(cols);
-    float q = 0.f;
-    for (int c = threadIdx.x * kE; c < cols; c += 256 * kE) {
-      const Piece<T, kVec> p(xr + c);
+        for (int e = 0; e < kE; ++e) s = fmaf(p.v[e], f, s);
+      }
+      mean = block_sum(s, part) / static_cast<float>(cols);
+      float q = 0.f;
+      for (int c = threadIdx.x * kE; c < cols; c += 256 * kE) {
+        const Piece<T, kVec> p(xr + c);
 #pragma unroll
-      for (int e = 0; e < kE; ++e) q = fmaf(p.v[e] - mean, p.v[e] - mean, q);
+        for (int e = 0; e < kE; ++e) {
+          const float d = fmaf(p.v[e], f, -mean);
+          q = fmaf(d, d, q);
+        }
+      }
+      const float var = block_sum(q, part) / static_cast<float>(cols);
+      rstd = f == 1.f ? 1.f / sqrtf(var + eps) : far_rstd(var, eps);
+      if (f != 1.f || !variance_overflows(var + eps)) break;  // (the whole CTA)
+      f = kFar;
     }
-    const float rstd = 1.f / sqrtf(block_sum(q, part) / static_cast<float>(cols) + eps);
     for (int c = threadIdx.x * kE; c < cols; c += 256 * kE) {
       Piece<T, kVec> p(xr + c);
       const Piece<float, kVec> gm(gamma + c), bt(beta + c);
 #pragma unroll
-      for (int e = 0; e < kE; ++e) p.v[e] = fmaf((p.v[e] - mean) * rstd, gm.v[e], bt.v[e]);
+      for (int e = 0; e < kE; ++e)
+        p.v[e] = fmaf(fmaf(p.v[e], f, -mean) * rstd, gm.v[e], bt.v[e]);
       put_piece<kVec>(y + row * cols + c, p.v);
     }
     if (threadIdx.x == 0 && mean_out) {
-      mean_out[row] = mean;
-      rstd_out[row] = rstd;
+      mean_out[row] = f == 1.f ? mean : far_mean(mean);
+      rstd_out[row] = rstd * f;
     }
   }
 }

@@ -281,3 +281,58 @@ def test_norm_gradient_of_codes_far_from_zero(nrp, rows, cols, dtype, shift):
                 + ref.abs() * torch.finfo(dt).eps / 2).all()
         dx[one] = 0
         assert (dx == 0).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(14, 64), (37, 256), (23, 512), (50, 1024), (9, 2048),
+                                       (40, 77), (11, 300), (21, 999), (13, 1999), (700, 512),
+                                       (12, 4096), (8, 3001), (10, 6000), (9, 5001)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_norm_of_very_large_values(nrp, rows, cols, dtype):
+    """Rows whose sum of squares, or sum, passes f32's range beside ordinary ones: the
+    largest finite values of both signs, a single large one, a constant row, with NaN
+    and infinities in others.  Tolerances in u = 2^-24: a row's sums are chains of
+    n = cols / 32 + 8 additions (over 2048 columns cols / 256 + 16), the mean off by
+    dm = (n + 2) u mean|x|, rstd by (n + 8) u, y by those and three roundings; rstd
+    by half of the smallest f32 number too."""
+    import torch
+    dt = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    g = torch.Generator().manual_seed(cols)
+    x = torch.randn(rows, cols, generator=g).double()
+    top = torch.finfo(dt).max
+    x[1] *= 1e20
+    x[2] = (torch.rand(cols, generator=g) * 2 - 1).double() * top
+    x[3] *= 1e-3
+    x[3, cols // 2] = 1e38
+    x[4] = top
+    x[5] = x[5] * 1e18 + 1e22
+    x[6, 1] = float("inf")
+    x[7, 0] = float("nan")
+    x = x.to(dt)
+    gamma, beta = 1 + 0.2 * torch.randn(cols, generator=g), 0.1 * torch.randn(cols, generator=g)
+    y, mean, rstd = (t.double().cpu() for t in nrp.layer_norm(x.cuda(), gamma.cuda(), beta.cuda()))
+    assert y[6:8].isnan().all() and mean[7].isnan() and rstd[7].isnan()
+    keep = [r for r in range(rows) if r not in (6, 7)]
+    xd, ga, be = x.double()[keep], gamma.double(), beta.double()
+    m = xd.mean(1, keepdim=True)
+    r = ((xd - m).square().mean(1, keepdim=True) + float(torch.tensor(1e-5))) ** -0.5
+    n = cols / 32 + 8 if cols <= 2048 else cols / 256 + 16
+    dm = (n + 2) * U * xd.abs().mean(1, keepdim=True)
+    u = (xd - m) * r
+    ref = u * ga + be
+    dr = (n + 8) * U + (r * dm).square()
+    assert ((mean[keep][:, None] - m).abs() <= dm).all()
+    assert ((rstd[keep][:, None] - r).abs() <= r * dr + 2.0 ** -149).all()
+    tol = (ga.abs() * (r * dm + u.abs() * ((n + 12) * U + dr)) + (be.abs() + ref.abs()) * 2 * U
+           + ref.abs() * torch.finfo(dt).eps / 2)
+    assert ((y[keep] - ref).abs() <= tol).all()
+    z = x.cuda()  # in place
+    nrp.layer_norm(z, gamma.cuda(), beta.cuda(), out=z)
+    assert torch.equal(z.double().cpu()[keep], y[keep])
+    # the gradients take such a row's statistics (within +-2^126 of its mean)
+    s = [1, 3, 5]
+    dy = torch.randn(3, cols, generator=g).to(dt)
+    _, mean, rstd = nrp.layer_norm(x[s].cuda(), gamma.cuda(), beta.cuda())
+    dg = nrp.layer_norm_backward(dy.cuda(), x[s].cuda(), mean, rstd, gamma.cuda())[1]
+    u = (x[s].double() - mean.double().cpu()[:, None]) * rstd.double().cpu()[:, None]
+    assert ((dg.double().cpu() - (dy.double() * u).sum(0)).abs()
+            <= 23 * U * (dy.double() * u).abs().sum(0)).all()
