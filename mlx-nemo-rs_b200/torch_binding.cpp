@@ -141,6 +141,12 @@ Tensor output(const char* name, PyObject* out, at::IntArrayRef shape, ScalarType
   return t;
 }
 
+// A tensor of the caller's that a call has written: autograd sees by its version
+// that a value it saved is gone.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 bool is_fp8(PyObject* o) { return PyObject_TypeCheck(o, g_fp8) && PyTuple_GET_SIZE(o) == 3; }
 struct Codes {
   const Tensor* codes;
@@ -168,6 +174,10 @@ Codes codes_of(const char* name, PyObject* o, int64_t block_rows, int dev,
   if (block) *block = br;
   return {&c, static_cast<uint8_t*>(c.data_ptr()),
           static_cast<float*>(const_cast<void*>(s)), size};
+}
+void codes_written(PyObject* o) {
+  written(THPVariable_Unpack(PyTuple_GET_ITEM(o, 0)));
+  written(THPVariable_Unpack(PyTuple_GET_ITEM(o, 1)));
 }
 int codes_device(const char* name, PyObject* o) {
   if (!is_fp8(o)) fail(std::string(name) + ": an Fp8Tensor is needed");
@@ -277,7 +287,10 @@ PyObject* quantize(PyObject* const* a) {
     return nrp_fp8_quantize(ctx, stream_of(dev), dt, t.const_data_ptr(), n.rows,
                             static_cast<int>(n.cols), static_cast<int>(br), q.q, q.s);
   });
-  if (a[3] != Py_None) return Py_NewRef(a[3]);
+  if (a[3] != Py_None) {
+    codes_written(a[3]);
+    return Py_NewRef(a[3]);
+  }
   return new_fp8(codes, scales, br);
 }
 
@@ -295,6 +308,7 @@ PyObject* dequantize(PyObject* const* a) {
                               static_cast<int>(q.size.cols), static_cast<int>(br), dt,
                               out.data_ptr());
   });
+  if (a[3] != Py_None) written(out);
   return THPVariable_Wrap(out);
 }
 
@@ -364,6 +378,8 @@ PyObject* product(PyObject* const* a) {
                  : nrp_fp8_linear(ctx, stream_of(dev), dt, src, xq, xs, m, r, w.q, w.s, c, bias,
                                   out.data_ptr());
   });
+  if (a[5] != Py_None) written(out);
+  if (a[6] != Py_None) codes_written(a[6]);
   return THPVariable_Wrap(out);
 }
 
@@ -392,6 +408,8 @@ PyObject* weight_grad(PyObject* const* a) {
                                       static_cast<int>(n.cols), static_cast<int>(x.size.cols), dt,
                                       dw.data_ptr(), db.defined() ? db.data_ptr() : nullptr);
   });
+  if (a[5] != Py_None) written(dw);
+  if (a[6] != Py_None) written(db);
   PyObject* t = PyTuple_New(2);
   PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(dw));
   PyTuple_SET_ITEM(t, 1, db.defined() ? THPVariable_Wrap(db) : Py_NewRef(Py_None));
@@ -422,6 +440,7 @@ PyObject* layer_norm(PyObject* const* a) {
                           static_cast<const float*>(b), static_cast<float>(eps), y.data_ptr(),
                           stats[0], stats[1]);
   });
+  if (a[5] != Py_None) written(y);
   return tuple_of(y, mean, rstd);
 }
 
@@ -468,6 +487,7 @@ PyObject* layer_norm_backward(PyObject* const* a) {
         static_cast<const float*>(rs), static_cast<const float*>(g), n.rows, cols, dx.data_ptr(),
         sums[0], sums[1], bytes ? ws.data_ptr() : nullptr, bytes);
   });
+  if (a[6] != Py_None) written(dx);
   return tuple_of(dx, dgamma, dbeta);
 }
 

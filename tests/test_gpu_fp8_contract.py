@@ -336,3 +336,38 @@ def test_norm_of_very_large_values(nrp, rows, cols, dtype):
     u = (x[s].double() - mean.double().cpu()[:, None]) * rstd.double().cpu()[:, None]
     assert ((dg.double().cpu() - (dy.double() * u).sum(0)).abs()
             <= 23 * U * (dy.double() * u).abs().sum(0)).all()
+
+
+def test_outputs_raise_their_version(nrp):
+    """Every output of the caller's counts as written in place: autograd refuses a
+    gradient that needs the value which was there."""
+    import torch
+    x = torch.randn(20, 256, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    v = torch.ones(256, device="cuda")
+    w = nrp.fp8_quantize(torch.randn(128, 256, device="cuda"), 128)
+    q = nrp.fp8_quantize(x)
+    dy = torch.zeros(20, 128, device="cuda", dtype=torch.bfloat16)
+    y = nrp.fp8_linear(x, w)
+    _, mean, rstd = nrp.layer_norm(x, v, v)
+    dw, db = nrp.fp8_linear_weight_grad(dy, q, bias=True)
+    calls = [
+        ([*q[:2]], lambda: nrp.fp8_quantize(x, out=q)),
+        ([x], lambda: nrp.fp8_dequantize(q, torch.float32, out=x)),
+        ([y, *q[:2]], lambda: nrp.fp8_linear(x, w, out=y, codes=q)),
+        ([x], lambda: nrp.fp8_linear_input_grad(nrp.fp8_quantize(y), w, dtype=torch.float32, out=x)),
+        ([dw, db], lambda: nrp.fp8_linear_weight_grad(dy, q, out=dw, bias_out=db)),
+        ([x], lambda: nrp.layer_norm(x, v, v, out=x)),
+        ([x], lambda: nrp.layer_norm_backward(torch.ones_like(x), q, mean, rstd, v, out=x)),
+    ]
+    for i, (outs, call) in enumerate(calls):
+        before = [t._version for t in outs]
+        call()
+        assert [t._version for t in outs] == [n + 1 for n in before], i
+    p = torch.ones(20, 256, device="cuda", requires_grad=True)
+    loss = (p * x).sum()  # keeps x
+    nrp.layer_norm(x, v, v, out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():  # no version there
+        z = torch.empty_like(x)
+    assert nrp.layer_norm(x, v, v, out=z)[0] is z
