@@ -107,29 +107,17 @@ Tensor empty(at::IntArrayRef shape, ScalarType type, int dev) {
                                 c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(dev)),
                                 std::nullopt);
 }
-// A contiguous tensor in buf's storage, from byte `at` on.
-Tensor part_of(const Tensor& buf, int64_t at, at::IntArrayRef shape, ScalarType type) {
-  const auto meta = c10::scalarTypeToTypeMeta(type);
-  Tensor t = at::detail::make_tensor<c10::TensorImpl>(
-      c10::Storage(buf.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), meta);
-  t.unsafeGetTensorImpl()->set_storage_offset(at / static_cast<int64_t>(meta.itemsize()));
-  t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
-  return t;
-}
-// Two f32 tensors of one shape, or a matrix' codes and scales, in one allocation
-// (0.5 us less than two).
+// Two f32 tensors of one shape, and a matrix' codes and scales: each with a storage
+// of its own (one of both would save 0.5 us, but resize_ of one would grow into the
+// other, and either keep and save both).
 std::pair<Tensor, Tensor> empty_two(at::IntArrayRef shape, int dev) {
-  int64_t n = 1;
-  for (int64_t s : shape) n *= s;
-  const Tensor buf = empty({8 * n}, ScalarType::Byte, dev);
-  return {part_of(buf, 0, shape, ScalarType::Float), part_of(buf, 4 * n, shape, ScalarType::Float)};
+  Tensor first = empty(shape, ScalarType::Float, dev);
+  return {std::move(first), empty(shape, ScalarType::Float, dev)};
 }
 std::pair<Tensor, Tensor> empty_codes(at::IntArrayRef shape, Size n, int64_t block_rows, int dev) {
-  const int64_t rows = block_rows == 1 ? n.rows : blocks(n.rows);
-  const int64_t bytes = (n.rows * n.cols + 15) / 16 * 16;
-  const Tensor buf = empty({bytes + 4 * rows * blocks(n.cols)}, ScalarType::Byte, dev);
-  return {part_of(buf, 0, shape, ScalarType::Float8_e4m3fn),
-          part_of(buf, bytes, {rows, blocks(n.cols)}, ScalarType::Float)};
+  Tensor codes = empty(shape, ScalarType::Float8_e4m3fn, dev);
+  return {std::move(codes), empty({block_rows == 1 ? n.rows : blocks(n.rows), blocks(n.cols)},
+                                  ScalarType::Float, dev)};
 }
 // out= of the given shape and type, or a new tensor.
 Tensor output(const char* name, PyObject* out, at::IntArrayRef shape, ScalarType type, int dev) {

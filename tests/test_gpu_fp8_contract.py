@@ -371,3 +371,22 @@ def test_outputs_raise_their_version(nrp):
     with torch.inference_mode():  # no version there
         z = torch.empty_like(x)
     assert nrp.layer_norm(x, v, v, out=z)[0] is z
+
+
+def test_results_have_storages_of_their_own(nrp):
+    """Codes and scales, mean and rstd, dgamma and dbeta: growing one in place leaves
+    the other, and none holds more memory than its values."""
+    import torch
+    x = torch.randn(16, 256, device="cuda")
+    v = torch.ones(256, device="cuda")
+    q = nrp.fp8_quantize(x)
+    _, mean, rstd = nrp.layer_norm(x, v, v)
+    _, dg, db = nrp.layer_norm_backward(x, x, mean, rstd, v)
+    for first, second in ((q.codes, q.scales), (mean, rstd), (dg, db)):
+        for t in (first, second):
+            assert t.storage_offset() == 0
+            assert t.untyped_storage().nbytes() == t.numel() * t.element_size()
+        keep = second.clone()
+        n = first.numel()
+        first.resize_(2 * n).view(torch.uint8)[n * first.element_size():] = 7
+        assert torch.equal(second, keep)
