@@ -129,6 +129,13 @@ Tensor output(const char* name, PyObject* out, at::IntArrayRef shape, ScalarType
   return t;
 }
 
+// A Python int's value; -1 for another object, or one past 64 bits.
+int64_t int_or_none(PyObject* o) {
+  const int64_t v = PyLong_Check(o) ? PyLong_AsLongLong(o) : -1;
+  if (v == -1 && PyErr_Occurred()) PyErr_Clear();
+  return v;
+}
+
 // A tensor of the caller's that a call has written: autograd sees by its version
 // that a value it saved is gone.
 void written(const Tensor& t) {
@@ -146,9 +153,7 @@ struct Codes {
 Codes codes_of(const char* name, PyObject* o, int64_t block_rows, int dev,
                int64_t* block = nullptr) {
   if (!is_fp8(o)) fail(std::string(name) + ": an Fp8Tensor is needed");
-  PyObject* b = PyTuple_GET_ITEM(o, 2);
-  const int64_t br = PyLong_Check(b) ? PyLong_AsLongLong(b) : -1;
-  if (br == -1 && PyErr_Occurred()) PyErr_Clear();
+  const int64_t br = int_or_none(PyTuple_GET_ITEM(o, 2));
   if (block_rows ? br != block_rows : br != 1 && br != 128)
     fail(std::string(name) + ": block_rows " + std::to_string(br) + ", " +
          (block_rows ? std::to_string(block_rows) : "1 or 128") + " needed");
@@ -255,7 +260,7 @@ PyObject* quantize(PyObject* const* a) {
   const int dt = dtype_code("quantize", t.scalar_type());
   checked("quantize", a[0], t.scalar_type(), dev);
   const Size n = size_of("quantize", t);
-  const int64_t br = PyLong_Check(a[1]) ? PyLong_AsLongLong(a[1]) : -1;
+  const int64_t br = int_or_none(a[1]);
   if (br != 1 && br != 128)
     fail("quantize: block_rows " + std::to_string(br) + " (supported: 1, 128)",
          NRP_ERR_UNSUPPORTED);

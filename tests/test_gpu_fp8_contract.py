@@ -390,3 +390,15 @@ def test_results_have_storages_of_their_own(nrp):
         n = first.numel()
         first.resize_(2 * n).view(torch.uint8)[n * first.element_size():] = 7
         assert torch.equal(second, keep)
+
+
+@pytest.mark.parametrize("block_rows", [0, -1, 2, 2 ** 40, 2 ** 70, -2 ** 70, 1.0, None, "1"])
+def test_block_rows_of_any_kind_are_refused(nrp, block_rows):
+    """With the library's own error, also for an int past 64 bits."""
+    import torch
+    x = torch.zeros(4, 64, device="cuda")
+    q = nrp.fp8_quantize(x)
+    for call in (lambda: nrp.fp8_quantize(x, block_rows),
+                 lambda: nrp.fp8_dequantize(q._replace(block_rows=block_rows))):
+        with pytest.raises(nrp.NrpError):
+            call()
