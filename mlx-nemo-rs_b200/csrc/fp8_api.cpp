@@ -40,7 +40,7 @@ int check_sizes(const char* what, std::initializer_list<int> sizes) {
 }
 
 // A matrix of codes: 16-byte rows (TMA and 16-byte loads), 16-byte aligned.
-// One without rows may have null pointers (an empty tensor's).
+// Those of one without rows are not looked at.
 int check_codes(const char* name, const void* codes, const void* scales, int64_t cols,
                 bool empty = false) {
   if (!empty && (!codes || !scales))
@@ -48,7 +48,7 @@ int check_codes(const char* name, const void* codes, const void* scales, int64_t
   if (cols % 16)
     return failf(NRP_ERR_UNSUPPORTED, "%s: %lld columns (codes need a multiple of 16)", name,
                  static_cast<long long>(cols));
-  if (!aligned(codes, 16) || !aligned(scales, 4))
+  if (!empty && (!aligned(codes, 16) || !aligned(scales, 4)))
     return failf(NRP_ERR_INVALID, "%s: codes must be 16-byte and scales 4-byte aligned", name);
   return NRP_OK;
 }
@@ -275,7 +275,7 @@ int nrp_layer_norm_backward(nrp_context* ctx, void* stream, int dtype, const voi
   if (!dgamma != !dbeta) return failf(NRP_ERR_INVALID, "layer norm: dgamma and dbeta go together");
   if (int rc = check_dtype(dtype)) return rc;
   if (x_scales)
-    if (int rc = check_codes("layer norm backward: input", x, x_scales, cols)) return rc;
+    if (int rc = check_codes("layer norm backward: input", x, x_scales, cols, rows == 0)) return rc;
   const int64_t need = dgamma ? 4 * nrp::norm_bwd_partials(rows, cols) : 0;
   if (need) {
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16))

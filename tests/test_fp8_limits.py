@@ -92,3 +92,26 @@ def test_default_context_of_threads(nrp, monkeypatch):
     for t in ts:
         t.join()
     assert len(made) == 1 and all(c is made[0] for c in got) and len(got) == 4
+
+
+@pytest.mark.parametrize("off", [None, 1])
+def test_pointers_of_no_rows(nrp, ctx, off):
+    """A matrix without rows: its pointers may be null or anything.  What is asked
+    for is then nothing, or (without a device) the device."""
+    p, n = ctx[0], 0
+    q = None if off is None else AT[0] + off
+    g = AT[1]
+    calls = [
+        ("nrp_fp8_quantize", p, None, BF16, q, n, 64, 1, q, q),
+        ("nrp_fp8_quantize", p, None, F32, q, n, 64, 128, q, q),
+        ("nrp_fp8_dequantize", p, None, q, q, n, 64, 1, F32, q),
+        ("nrp_fp8_linear", p, None, BF16, None, q, q, n, 64, g, g, 32, None, q),
+        ("nrp_fp8_linear", p, None, BF16, q, q, q, n, 64, g, g, 32, None, q),
+        ("nrp_fp8_linear_input_grad", p, None, BF16, q, q, q, n, 64, g, g, 32, q),
+        ("nrp_layer_norm", p, None, F32, q, n, 64, g, g, 1e-5, q, q, q),
+        ("nrp_layer_norm_backward", p, None, F32, q, None, q, q, q, g, n, 64, q, None, None, None, 0),
+        ("nrp_layer_norm_backward", p, None, F32, q, g, q, q, q, g, n, 64, q, None, None, None, 0),
+    ]
+    for fn, *args in calls:
+        rc, msg = status(nrp, fn, *args)
+        assert rc in (0, -2), (fn, msg)
