@@ -12,13 +12,15 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libnemo_relpos.so")
 BINDING_SRC = os.path.join(HERE, "torch_binding.cpp")
-BINDING = os.path.join(HERE, "_nrp_torch.so")
+BINDING = os.path.join(HERE, "_nrp_torch" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+BINDING_STAMP = os.path.join(BUILD, "_nrp_torch.stamp")  # what it was built against
 NVCC = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
@@ -34,7 +36,6 @@ def _nccl_include():
     only: the library is loaded with dlopen at run time).  The header of the
     NCCL that torch ships comes first, as that is the copy a torch process
     has loaded."""
-    import sysconfig
     for base in (sysconfig.get_paths()["purelib"], sysconfig.get_paths()["platlib"]):
         d = os.path.join(base, "nvidia", "nccl", "include")
         if os.path.exists(os.path.join(d, "nccl.h")):
@@ -70,29 +71,55 @@ def _compile(src, force):
     return obj, r.stderr
 
 
+def _torch_version(torch):
+    """torch/version.py's __version__, without importing torch."""
+    try:
+        with open(os.path.join(torch, "version.py")) as f:
+            return next(line.split("'")[1] for line in f if line.startswith("__version__"))
+    except (OSError, StopIteration, IndexError):
+        return "unknown"
+
+
 def _build_binding(force):
-    """_nrp_torch.so against the running interpreter's torch (its headers
-    make this the slowest file: about a minute)."""
+    """The binding against the running interpreter's torch (its headers make
+    this the slowest file: about a minute).  The C library and the host-side
+    Python serve without it: where torch or its CUDA part or g++ is missing it
+    is left out, and what needs it says so when it is asked for."""
     import importlib.util
-    import sysconfig
     hdr = os.path.join(os.path.dirname(HERE), "include", "nemo_relpos.h")
-    if not force and not _stale(BINDING, [BINDING_SRC, hdr]):
-        return ""
     spec = importlib.util.find_spec("torch")
-    if spec is None:  # the C library serves without it
-        return ""
+    if spec is None or not spec.origin:
+        return "torch is not installed: no binding"
     torch = os.path.dirname(spec.origin)
+    libs = os.path.join(torch, "lib")
+    cxx = shutil.which("g++")
+    if not os.path.exists(os.path.join(libs, "libtorch_cuda.so")):
+        return f"{torch} has no CUDA part: no binding"
+    if cxx is None:
+        return "no g++: no binding"
+    stamp = f"torch {_torch_version(torch)} at {torch}\npython {sys.version}\n"
+    try:
+        with open(BINDING_STAMP) as f:
+            same = f.read() == stamp
+    except OSError:
+        same = False
+    if not force and same and not _stale(BINDING, [BINDING_SRC, hdr]):
+        return ""
     inc = [os.path.join(torch, "include"),
            os.path.join(torch, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], "/usr/local/cuda/include"]
-    libs = os.path.join(torch, "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-DTORCH_EXTENSION_NAME=_nrp_torch",
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-DTORCH_EXTENSION_NAME=_nrp_torch",
            *[f"-isystem{d}" for d in inc], BINDING_SRC, "-o", BINDING, f"-L{libs}", f"-L{HERE}",
            "-l:libnemo_relpos.so", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda",
            "-lc10", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    old = os.path.join(HERE, "_nrp_torch.so")  # (a name that any interpreter would load)
+    if old != BINDING and os.path.exists(old):
+        os.remove(old)
+    with open(BINDING_STAMP, "w") as f:
+        f.write(stamp)
     return r.stderr
 
 

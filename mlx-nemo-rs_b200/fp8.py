@@ -23,10 +23,15 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import Context, NrpError, lib
+from . import NRP_ERR_UNSUPPORTED, Context, NrpError, lib
 
 lib()  # (names the build command if the library is missing)
-from . import _nrp_torch as _native  # noqa: E402
+try:
+    from . import _nrp_torch as _native  # noqa: E402
+except ImportError as e:
+    raise NrpError(NRP_ERR_UNSUPPORTED,
+                   "the torch binding is missing or was built for another torch or Python: run "
+                   f"python mlx-nemo-rs_b200/build.py ({e})") from e
 
 
 class Fp8Tensor(NamedTuple):
