@@ -402,3 +402,48 @@ def test_block_rows_of_any_kind_are_refused(nrp, block_rows):
                  lambda: nrp.fp8_dequantize(q._replace(block_rows=block_rows))):
         with pytest.raises(nrp.NrpError):
             call()
+
+
+@pytest.mark.parametrize("m,k,n", [(16000, 1024, 4096), (12500, 512, 1024), (4000, 1024, 1024),
+                                   (16000, 144, 256), (8192, 400, 200)])
+def test_weight_gradient_precision(nrp, m, k, n):
+    """The gradients of many tokens as a whole.  A tensor-core addition is cut off by
+    up to 2^-23 of the sum, 2^-24 on average and always towards zero; over a segment
+    of 64 additions, whose partial sums grow like sqrt(j), these add up to 64 * 2/3 *
+    2^-24 of the segment's sum, and segments, added with rounding, are independent:
+    2.6e-6 of the norm.  (One chain of m / 16 additions is off by 8e-6 at 16000
+    tokens.)  dbias: chains of m / 32 rounded additions, sqrt(m / 32 / 6) 2^-24 of
+    the norm on average; twice that and eight more for the joins."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+    q = nrp.fp8_quantize(torch.randn(m, k, device="cuda", generator=g))
+    dy = torch.randn(m, n, device="cuda", generator=g).bfloat16()
+    dw, db = nrp.fp8_linear_weight_grad(dy, q, bias=True)
+    x = q.codes.double() * q.scales.double().repeat_interleave(128, 1)[:, :k]
+    ref, d = dy.double().t() @ x, dy.double().sum(0)
+    assert (dw.double() - ref).norm() <= 64 * 2 / 3 * U * ref.norm()
+    assert (db.double() - d).norm() <= (2 * (m / 192) ** 0.5 + 8) * U * d.norm()
+
+
+@pytest.mark.parametrize("rows,cols", [(20, 512), (3000, 64), (2500, 1024), (600, 784), (50, 4096),
+                                       (40, 6000)])
+def test_norm_gradient_of_a_nan_code(nrp, rows, cols):
+    """A NaN code, or an infinite scale's block, reaches its row of dx and its columns
+    of dgamma only."""
+    import torch
+    q = nrp.Fp8Tensor(codes((rows, cols), 448.0, 1),
+                      torch.ones(rows, -(-cols // 128), device="cuda"), 1)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    dy = torch.randn(rows, cols, device="cuda", generator=g).bfloat16()
+    mean = torch.randn(rows, device="cuda", generator=g)
+    rstd = torch.rand(rows, device="cuda", generator=g) + 0.5
+    gamma = torch.randn(cols, device="cuda", generator=g)
+    q.codes.view(torch.uint8)[7, 5] = 0x7F
+    q.codes.view(torch.uint8)[rows - 1, cols - 1] = 0xFF
+    dx, dg, db = nrp.layer_norm_backward(dy, q, mean, rstd, gamma)
+    bad = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    bad[[7, rows - 1]] = True
+    assert dx[bad].isnan().all() and dx[~bad].isfinite().all()
+    bad = torch.zeros(cols, dtype=torch.bool, device="cuda")
+    bad[[5, cols - 1]] = True
+    assert dg[bad].isnan().all() and dg[~bad].isfinite().all() and db.isfinite().all()
