@@ -65,6 +65,6 @@ int64_t norm_bwd_partials(int64_t rows, int cols);
 cudaError_t launch_norm_bwd(bool bf16, const void* x, const float* xs, const void* dy,
                             const float* mean, const float* rstd, const float* gamma,
                             int64_t rows, int cols, void* dx, float* dgamma, float* dbeta,
-                            float* partials, cudaStream_t stream);
+                            float* partials, int num_sms, cudaStream_t stream);
 
 }  // namespace nrp

@@ -298,7 +298,7 @@ int nrp_layer_norm_backward(nrp_context* ctx, void* stream, int dtype, const voi
   ProfScope ps(ctx, NRP_KERNEL_LAYERNORM_BWD, st);
   return status(nrp::launch_norm_bwd(dtype == NRP_DTYPE_BF16, x, x_scales, dy, mean, rstd, gamma,
                                      rows, cols, dx, dgamma, dbeta,
-                                     static_cast<float*>(workspace), st),
+                                     static_cast<float*>(workspace), ctx->num_sms, st),
                 "layer norm backward");
 }
 

@@ -552,7 +552,9 @@ constexpr int kManyThreads = 256;
 // Rows of up to 128 columns take half a warp each (30000 x 64 bf16: 8.7 us, 12.2 with
 // a warp to a row; x 77 10.5 against 14.4).
 constexpr int kNarrowLanes = 16, kNarrow = 8 * kNarrowLanes;
-constexpr int kManyParts = 2 * 148;    // CTAs of the persistent grid at most
+// CTAs of the persistent grid, two to an SM, at most: the workspace is asked for
+// without a device and has room for those of 148 SMs.
+constexpr int kManyParts = 2 * 148;
 
 // The most partial rows of dgamma | dbeta that go through the workspace (0: none).
 int norm_parts(int64_t rows, int cols) {
@@ -1017,6 +1019,7 @@ struct BwdArgs {
   int64_t rows;
   int cols;
   float *dgamma, *dbeta, *partials;
+  int num_sms;
 };
 
 // parts: the CTAs, which is the partial rows written.
@@ -1042,7 +1045,8 @@ cudaError_t bwd_strips(const TX* x, const T* dy, T* dx, const BwdArgs& a, int& p
     la[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
   } else {
-    const int most = kThreads == kManyThreads ? kManyParts : kManyParts / 2;
+    const int many = std::min(kManyParts, 2 * a.num_sms);
+    const int most = kThreads == kManyThreads ? many : many / 2;
     cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(batches, most)));
   }
   cfg.blockDim = dim3(32 * W * groups);
@@ -1088,7 +1092,7 @@ cudaError_t bwd(const TX* x, const T* dy, T* dx, const BwdArgs& a, cudaStream_t 
     e = vec ? bwd_strips<T, TX, true, kFewThreads, 1>(x, dy, dx, a, parts, stream)
             : bwd_strips<T, TX, false, kFewThreads, 1>(x, dy, dx, a, parts, stream);
   } else {
-    const int grid = static_cast<int>(std::min<int64_t>(a.rows, 4 * kManyParts));
+    const int grid = static_cast<int>(std::min<int64_t>(a.rows, 8 * a.num_sms));
     const bool all = vec && aligned16(a.gamma);
     e = launch_pdl(all ? norm_bwd_wide_kernel<T, TX, true> : norm_bwd_wide_kernel<T, TX, false>,
                    dim3(grid), dim3(256), 0, stream, x, a.xs, dy, a.mean, a.rstd, a.gamma, a.rows,
@@ -1134,13 +1138,14 @@ int64_t norm_bwd_partials(int64_t rows, int cols) {
 cudaError_t launch_norm_bwd(bool bf16, const void* x, const float* xs, const void* dy,
                             const float* mean, const float* rstd, const float* gamma,
                             int64_t rows, int cols, void* dx, float* dgamma, float* dbeta,
-                            float* partials, cudaStream_t stream) {
+                            float* partials, int num_sms, cudaStream_t stream) {
   if (rows <= 0) {
     if (!dgamma) return cudaSuccess;
     if (cudaError_t e = cudaMemsetAsync(dgamma, 0, 4 * static_cast<size_t>(cols), stream)) return e;
     return cudaMemsetAsync(dbeta, 0, 4 * static_cast<size_t>(cols), stream);
   }
-  const BwdArgs a{xs, mean, rstd, gamma, rows, cols, dgamma, dbeta, dgamma ? partials : nullptr};
+  const BwdArgs a{xs,   mean,   rstd,  gamma,    rows,
+                  cols, dgamma, dbeta, dgamma ? partials : nullptr, num_sms};
   return bf16 ? bwd_typed<__nv_bfloat16>(x, xs, dy, dx, a, stream)
               : bwd_typed<float>(x, xs, dy, dx, a, stream);
 }
