@@ -14,7 +14,8 @@
 // All are bound by HBM: they read and write each element once.  Measured: 16000
 // x 4096 bf16 by rows 32 us (6.2 TB/s, a plain copy's rate), 4096 x 1024 f32 by
 // 128 x 128 blocks 4.3 us (4.9 TB/s with the launch in it: 256 CTAs hold a block
-// each in registers between its maximum and its codes).
+// each in registers between its maximum and its codes); values of 16000 x 4096 codes
+// in bf16 42 us (4.7 TB/s: one unit of 16 codes in flight per thread).
 #include "fp8.h"
 #include "fp8_quant.cuh"
 

@@ -24,13 +24,16 @@
 // thread keeps 128 sums and two 16-column reads of TMEM in its 168 registers.
 //
 // Bound by getting the operands to the tensor cores: a 256-wide block is 48 KB
-// into shared memory and 48 KB out of it for 256 cycles of MMA (768 at 128
-// bytes a cycle; measured 930), and the chip takes them from L2 at 11 TB/s.
-// Measured from codes to bf16: 16000 x 4096 to 1024 68 us (1.97 PFLOP/s; 3.4
-// waves of tiles take four), 16000 x 1024 to 4096 with bias 78 us (9 of them the
-// output, 131 MB), 896 x 1024 to 1024 6.3 us.  Tried and slower: CTA pairs (256 x
-// 256 tiles, 76 us against 71: the hand-off over the cluster), sixteen epilogue
-// warps (80 against 71), the last wave's tiles in halves (68.3 against 68.2).
+// into shared memory and 48 KB out of it, 768 cycles at 128 bytes each, for 512
+// cycles of MMA (128 x 256 x 128 products at 16384 FLOP a cycle), and takes about
+// 940 (the tensor pipe is active for 55% of them).  A tile's store is not hidden:
+// the warps that add up the next tile's blocks make it, and TMEM holds two blocks.
+// Measured from codes to bf16: 16000 x 4096 to 1024 70 us (1.91 PFLOP/s; 3.4
+// waves of tiles take four), 16000 x 1024 to 4096 with bias 81 us, of whose 14 tiles
+// to an SM 8 blocks each account for 55, 896 x 1024 to 1024 6.3 us.  Tried and slower:
+// CTA pairs (256 x 256 tiles, 76 us against 71: the hand-off over the cluster),
+// sixteen epilogue warps (80 against 71), the last wave's tiles in halves (68.3
+// against 68.2).
 #include <algorithm>
 
 #include "fp8.h"

@@ -14,7 +14,7 @@
 // sides.  A block's sum is scaled by its two scales and added in f32; the warps'
 // partial results meet in shared memory, the CTAs' in the cluster's.
 //
-// Measured: 14 rows, 1024 to 4096, bf16 with bias 5.0 us (an empty kernel takes
+// Measured: 14 rows, 1024 to 4096, bf16 with bias 4.9 us (an empty kernel takes
 // 2.2), 0.8 TB/s of weight.
 #include <algorithm>
 

@@ -27,7 +27,7 @@
 // Bound by shared-memory traffic: per 64 tokens 48 KB of MMA operands, 40 KB of
 // TMA writes and 24 KB of conversion, 896 cycles at 128 bytes each against the
 // tensor cores' 512, which makes 121 us at 16000 x 4096 x 1024.  Measured there
-// with bias: 141 us, 0.95 PFLOP/s; 749 x 1024 x 1024 10.0 us.  TMEM holds a
+// with bias: 142 us, 0.95 PFLOP/s; 749 x 1024 x 1024 10.2 us.  TMEM holds a
 // segment's sums and the running ones (below), which leaves no room in it for
 // the converted operand.  Tried and slower (then against 126 to 135): CTA pairs
 // with 256 x 256 tiles (165, the hand-off of both CTAs' conversions to one
@@ -147,8 +147,9 @@ __device__ __forceinline__ void store_four(TO* p, float4 v, bool wide) {
 
 // Adds a segment's sums to the running sums kTN columns further on (`more`: there
 // are some) in a quarter of the tile's columns, once full completes the phase
-// `parity`, and arrives on empty.  Out of line: its registers would spill the
-// conversion's.
+// `parity`, and arrives on empty.  Out of line, as inlined it takes registers from the
+// conversion, which at 80 a thread (23 warps) spills 100 to 190 bytes all the same:
+// the addresses and counts around the loops.
 template <int kTN>
 __device__ __noinline__ bool add_segment(uint32_t at, bool more, uint64_t* full, uint64_t* empty,
                                          uint32_t parity, int* err) {

@@ -5,11 +5,11 @@
 //   g = dy * gamma, dx = rstd * (g - mean_C(g) - u * mean_C(g * u))
 //   dgamma = sum_rows dy * u, dbeta = sum_rows dy
 //
-// in f32, each output rounded once.  The variance is summed about the mean
-// (two passes over the registers), so a large mean costs it no digits; a row whose
-// sums overflow f32 is taken again in smaller units.  The
-// backward pass takes x as it was or as the e4m3 checkpoint (codes and one
-// scale per 128 columns), with the saved mean and rstd of the exact row.
+// in f32, each output rounded once.  The variance is summed about the mean (two
+// passes over the registers), so a large mean costs it no digits; a row whose sums
+// overflow f32 is taken again in smaller units.  The backward pass takes x as it
+// was or as the e4m3 checkpoint (codes and one scale per 128 columns), with the
+// saved mean and rstd of the exact row.
 //
 // Bound by HBM.  Up to 4096 columns, both passes take strips of 256 columns.
 // The backward's sums over rows are added up in registers, over the CTA's
@@ -18,9 +18,9 @@
 // workspace: fixed order, no atomics.  Wider rows take a CTA each and read their
 // inputs again from L1/L2.
 //
-// Measured: forward, 50000 x 1024 bf16 36 us (5.7 TB/s; a plain copy of that
+// Measured: forward, 50000 x 1024 bf16 37 us (5.5 TB/s; a plain copy of that
 // size runs at 6.2), 14 x 512 f32 2.6 us; backward of 50000 x 1024 from bf16 dy
-// and codes 49 us with its second kernel (5.2 TB/s; instruction issue, at 60%,
+// and codes 50 us with its second kernel (5.1 TB/s; instruction issue, at 60%,
 // comes close to being the bound), 749 x 512 bf16 6.2 us in two launches.
 #include <algorithm>
 #include <cfloat>
@@ -88,7 +88,7 @@ struct Strip {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         // as it is: a conversion here would wait for the load (30000 x 777 bf16
-        // backward: 47 us, 93 with it)
+        // backward: 49 us, 93 with it)
         w[e] = 0u;
         if (col + kL * e < cols) {
           if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(p[col + kL * e]);
@@ -462,7 +462,7 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
 }
 
 // A thread's consecutive elements of a wide row, 8 where its address allows 16-byte
-// loads (4000 x 8192 bf16: forward 41 us, 60 by single elements; backward 88, 206).
+// loads (4000 x 8192 bf16: forward 36 us, 60 by single elements; backward 88, 206).
 template <bool kVec>
 constexpr int kPiece = kVec ? 8 : 1;
 template <typename T, bool kVec>
