@@ -233,9 +233,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     return !*abort_flag && mbar_wait_hot(bar, parity, a.err, code);
   };
   auto agreed = [&](bool fine) {
-    if (__all_sync(0xffffffffu, fine)) return true;
-    *abort_flag = 1;
-    return false;
+    if (!__all_sync(0xffffffffu, fine)) {
+      *abort_flag = 1;
+      return false;
+    }
+    __syncwarp();  // (a vote orders no memory, which the arrivals after it need)
+    return true;
   };
   pdl_launch_dependents();
   pdl_wait();
