@@ -482,7 +482,8 @@ PyObject* layer_norm_backward(PyObject* const* a) {
   const auto [dgamma, dbeta] = empty_two({n.cols}, dev);
   int64_t bytes = 0;
   const int cols = static_cast<int>(n.cols);
-  if (nrp_layer_norm_backward_workspace(n.rows, cols, &bytes) < 0) fail(nrp_last_error());
+  if (const int rc = nrp_layer_norm_backward_workspace(n.rows, cols, &bytes); rc < 0)
+    fail(nrp_last_error(), rc);
   Tensor ws;
   if (bytes) ws = empty({bytes}, ScalarType::Byte, dev);
   nrp_context* ctx = context_of(a[5], dev);

@@ -447,3 +447,19 @@ def test_norm_gradient_of_a_nan_code(nrp, rows, cols):
     bad = torch.zeros(cols, dtype=torch.bool, device="cuda")
     bad[[5, cols - 1]] = True
     assert dg[bad].isnan().all() and dg[~bad].isfinite().all() and db.isfinite().all()
+
+
+def test_too_many_columns_are_refused_from_python(nrp):
+    """With the code of an unsupported size, whichever call inside sees it first."""
+    import torch
+    torch.cuda.empty_cache()
+    cols = 2 ** 31 - 1
+    x = torch.empty(1, cols, device="cuda", dtype=torch.bfloat16)
+    v = torch.empty(cols, device="cuda")
+    s = torch.ones(1, device="cuda")
+    for call in (lambda: nrp.layer_norm(x, v, v), lambda: nrp.layer_norm_backward(x, x, s, s, v)):
+        with pytest.raises(nrp.NrpError, match="size") as e:
+            call()
+        assert e.value.code == nrp.NRP_ERR_UNSUPPORTED
+    del x, v
+    torch.cuda.empty_cache()
