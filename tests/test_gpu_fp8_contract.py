@@ -463,3 +463,49 @@ def test_too_many_columns_are_refused_from_python(nrp):
         assert e.value.code == nrp.NRP_ERR_UNSUPPORTED
     del x, v
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows,cols", [(20, 64), (20, 77), (300, 77), (3000, 64), (700, 300),
+                                       (600, 999), (600, 1000), (300, 1999), (50, 3001), (40, 6001)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_norm_gradient_of_constant_large_rows(nrp, rows, cols, dtype):
+    """Rows of one large value, whose mean times rstd = eps^-1/2 passes f32's range:
+    u is 0 in them, also where a row ends inside a strip.  Row sums are chains of
+    cols / 32 + 20 additions (over 2048 columns cols / 256 + 20)."""
+    import torch
+    dt = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    x = torch.full((rows, cols), 2.0 ** 122, device="cuda", dtype=dt)
+    mean = torch.full((rows,), 2.0 ** 122, device="cuda")
+    rstd = torch.full((rows,), 1e-5 ** -0.5, device="cuda")
+    dy = torch.randn(rows, cols, device="cuda", generator=g).to(dt)
+    gamma = torch.randn(cols, device="cuda", generator=g)
+    dx, dg, db = nrp.layer_norm_backward(dy, x, mean, rstd, gamma)
+    w = dy.double() * gamma.double()
+    ref = rstd.double()[:, None] * (w - w.mean(1, keepdim=True))
+    size = rstd.double()[:, None] * (w.abs() + w.abs().mean(1, keepdim=True))
+    chain = cols / 32 + 20 if cols <= 2048 else cols / 256 + 20
+    assert ((dx.double() - ref).abs() <= size * chain * U
+            + ref.abs() * torch.finfo(dt).eps / 2).all()
+    assert (dg == 0).all()
+    d = dy.double()
+    assert ((db.double() - d.sum(0)).abs() <= (rows + 16) * U * d.abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("trans", [False, True])
+def test_shared_reduction_of_far_scales(nrp, trans):
+    """Scales of 2^100 by 2^30 (products of codes at most 2^-14: sums in range) where
+    several CTAs share a tile's reduction of 32 blocks; tolerance as above."""
+    import torch
+    m, red, cols = 64, 4096, 256
+    x = nrp.Fp8Tensor(codes((m, red), 2.0 ** -7, 1), torch.full((m, 32), 2.0 ** 100).cuda(), 1)
+    wshape = (red, cols) if trans else (cols, red)
+    w = nrp.Fp8Tensor(codes(wshape, 2.0 ** -7, 2),
+                      torch.full([n // 128 for n in wshape], -2.0 ** 30).cuda(), 128)
+    x.scales[:, ::2] = 2.0 ** -110
+    x.scales[5] = 1.0
+    xv, wv = values(x), values(w) if trans else values(w).t()
+    ref, size = xv @ wv, xv.abs() @ wv.abs()
+    call = nrp.fp8_linear_input_grad if trans else nrp.fp8_linear
+    y = call(x, w, dtype=torch.float32).double().cpu()
+    assert ((y - ref).abs() <= size * (132 * 2.0 ** -23 + 40 * U) + 96 * 2.0 ** -149).all()
